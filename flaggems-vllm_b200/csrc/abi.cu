@@ -5,6 +5,7 @@
 
 #include "../../include/dsv4_prologue.h"
 #include "dsv4_common.cuh"
+#include "latent_attention.cuh"
 
 namespace dsv4 {
 namespace {
@@ -447,6 +448,103 @@ int dsv4_act_quant(const void* x, int64_t x_row_stride, void* out, float* scales
                    int32_t round_scale, void* cuda_stream) {
     return group_quant(x, x_row_stride, out, scales, block_size > 0 ? num_cols / block_size : 0, 1, num_rows, num_cols, block_size, 1e-4f,
                        round_scale, 1, cuda_stream);
+}
+
+int dsv4_fused_add_rmsnorm_quant_fp8(const void* x, int64_t x_row_stride, void* residual, int64_t residual_row_stride, const void* weight,
+                                     void* out, float* scales, int64_t scale_stride_row, int64_t scale_stride_group, int64_t num_rows,
+                                     int64_t num_cols, int64_t group_size, float eps, int32_t is_fp16, int32_t weight_is_fp32,
+                                     int32_t scale_is_ue8m0, void* cuda_stream) {
+    if (num_rows < 0 || num_cols < 0 || num_cols % 8 != 0 || group_size <= 0 || num_cols % group_size != 0) return DSV4_ERR_BAD_SIZE;
+    if (group_size != num_cols && group_size != 32 && group_size != 64 && group_size != 128 && group_size != 256) return DSV4_ERR_BAD_SIZE;
+    if (num_rows > 1 && (x_row_stride < num_cols || (residual && residual_row_stride < num_cols))) return DSV4_ERR_BAD_SIZE;
+    if (num_rows == 0 || num_cols == 0) return DSV4_OK;
+    if (!x || !weight || !out || !scales) return DSV4_ERR_NULL_POINTER;
+    if (!aligned16(x) || !aligned16(residual) || !aligned16(weight) || !aligned16(out) || (reinterpret_cast<uintptr_t>(scales) & 3u) != 0 ||
+        (num_rows > 1 && (x_row_stride % 8 != 0 || (residual && residual_row_stride % 8 != 0))))
+        return DSV4_ERR_MISALIGNED;
+    if (num_rows >= (1LL << 31) || num_cols > 32768) return DSV4_ERR_TOO_LARGE;
+    return static_cast<int>(launch_add_rmsnorm_quant(x, x_row_stride, residual, residual_row_stride, weight, out, scales, scale_stride_row,
+                                                     scale_stride_group, num_rows, num_cols, group_size, eps, is_fp16 ? 1 : 0,
+                                                     weight_is_fp32 ? 1 : 0, scale_is_ue8m0 ? 1 : 0, static_cast<cudaStream_t>(cuda_stream)));
+}
+
+namespace {
+// The arguments that both forms of the latent attention share, checked.
+int latent_attention_common(LatentAttention& p, const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_cache,
+                            int64_t num_blocks, int64_t kv_block_stride_bytes, int64_t cache_block_size, const float* attn_sink,
+                            float softmax_scale, void* out, int64_t out_stride_token, int64_t out_stride_head, float* lse,
+                            int64_t lse_stride_token, int64_t lse_stride_head, int64_t num_tokens, int64_t num_heads, const void* workspace) {
+    const int64_t lim = 1LL << 31;
+    if (num_tokens < 0 || num_heads < 0 || num_blocks < 0 || cache_block_size <= 0) return DSV4_ERR_BAD_SIZE;
+    if (!holds(kv_block_stride_bytes, cache_block_size, kTokenDataBytes + kScaleBytes)) return DSV4_ERR_BAD_SIZE;
+    if (!(softmax_scale > 0.0f) || softmax_scale > 3.4e38f) return DSV4_ERR_BAD_SIZE;
+    if (num_tokens >= lim || num_heads >= lim || num_blocks >= lim || cache_block_size >= lim) return DSV4_ERR_TOO_LARGE;
+    if (num_heads > 0 && num_tokens > (lim - 1) / num_heads) return DSV4_ERR_TOO_LARGE;
+    if (num_tokens == 0 || num_heads == 0) return DSV4_OK;
+    if (!q || !out || (num_blocks > 0 && !k_cache) || (!workspace && latent_attention_workspace(num_tokens, num_heads) > 0))
+        return DSV4_ERR_NULL_POINTER;
+    if (!aligned16(q) || !aligned16(out) || !aligned16(k_cache) || !aligned16(workspace) || q_stride_token % 8 != 0 || q_stride_head % 8 != 0 ||
+        out_stride_token % 8 != 0 || out_stride_head % 8 != 0 || kv_block_stride_bytes % 16 != 0 ||
+        (reinterpret_cast<uintptr_t>(lse) & 3u) != 0 || (reinterpret_cast<uintptr_t>(attn_sink) & 3u) != 0)
+        return DSV4_ERR_MISALIGNED;
+    p.q = static_cast<const uint8_t*>(q), p.q_stride_token = 2 * q_stride_token, p.q_stride_head = 2 * q_stride_head;
+    p.out = static_cast<uint8_t*>(out), p.out_stride_token = 2 * out_stride_token, p.out_stride_head = 2 * out_stride_head;
+    p.lse = lse, p.lse_stride_token = lse_stride_token, p.lse_stride_head = lse_stride_head;
+    p.sink = attn_sink, p.scale = softmax_scale;
+    p.k_cache = static_cast<const uint8_t*>(k_cache), p.block_stride = kv_block_stride_bytes, p.num_blocks = static_cast<int32_t>(num_blocks);
+    p.num_tokens = static_cast<int32_t>(num_tokens), p.num_heads = static_cast<int32_t>(num_heads);
+    p.block_size = static_cast<uint32_t>(cache_block_size);
+    make_fast_divisor(p.block_size, &p.block_mul, &p.block_shift);
+    return DSV4_OK;
+}
+}  // namespace
+
+int64_t dsv4_latent_attention_workspace_bytes(int64_t num_tokens, int64_t num_heads) {
+    if (num_tokens <= 0 || num_heads <= 0) return 0;
+    return static_cast<int64_t>(latent_attention_workspace(num_tokens, num_heads));
+}
+
+int dsv4_paged_latent_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_cache, int64_t num_blocks,
+                                int64_t kv_block_stride_bytes, int64_t cache_block_size, const int32_t* block_table,
+                                int64_t block_table_stride, int64_t max_blocks_per_seq, const int32_t* seq_lens,
+                                const int32_t* query_start_loc, int64_t num_reqs, int64_t window_size, int64_t num_first_tokens,
+                                const float* attn_sink, float softmax_scale, void* out, int64_t out_stride_token, int64_t out_stride_head,
+                                float* lse, int64_t lse_stride_token, int64_t lse_stride_head, int64_t num_tokens, int64_t num_heads,
+                                void* workspace, void* cuda_stream) {
+    LatentAttention p{};
+    const int rc = latent_attention_common(p, q, q_stride_token, q_stride_head, k_cache, num_blocks, kv_block_stride_bytes, cache_block_size,
+                                           attn_sink, softmax_scale, out, out_stride_token, out_stride_head, lse, lse_stride_token,
+                                           lse_stride_head, num_tokens, num_heads, workspace);
+    if (rc != DSV4_OK) return rc;
+    const int64_t lim = 1LL << 31;
+    if (num_reqs < 0 || max_blocks_per_seq < 0 || window_size < 0 || num_first_tokens < 0) return DSV4_ERR_BAD_SIZE;
+    if (num_reqs >= lim || max_blocks_per_seq >= lim) return DSV4_ERR_TOO_LARGE;
+    if (num_tokens == 0 || num_heads == 0 || num_reqs == 0) return DSV4_OK;
+    if (!seq_lens || !query_start_loc || (!block_table && max_blocks_per_seq > 0)) return DSV4_ERR_NULL_POINTER;
+    p.block_table = block_table, p.table_stride = block_table_stride, p.seq_lens = seq_lens, p.query_start_loc = query_start_loc;
+    p.num_reqs = static_cast<int32_t>(num_reqs);
+    // (positions are below 2^31: larger windows, numbers of first tokens and tables are cut to that)
+    const auto cut = [lim](int64_t v) { return static_cast<int32_t>(v < lim - 1 ? v : lim - 1); };
+    p.window = cut(window_size), p.first = cut(num_first_tokens);
+    p.capacity = max_blocks_per_seq > lim / cache_block_size ? static_cast<int32_t>(lim - 1) : cut(max_blocks_per_seq * cache_block_size);
+    return static_cast<int>(launch_latent_attention(p, workspace, static_cast<cudaStream_t>(cuda_stream)));
+}
+
+int dsv4_sparse_latent_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_cache, int64_t num_blocks,
+                                 int64_t kv_block_stride_bytes, int64_t cache_block_size, const int32_t* indices, int64_t indices_stride,
+                                 int64_t topk, const int32_t* lens, const float* attn_sink, float softmax_scale, void* out,
+                                 int64_t out_stride_token, int64_t out_stride_head, float* lse, int64_t lse_stride_token,
+                                 int64_t lse_stride_head, int64_t num_tokens, int64_t num_heads, void* workspace, void* cuda_stream) {
+    LatentAttention p{};
+    const int rc = latent_attention_common(p, q, q_stride_token, q_stride_head, k_cache, num_blocks, kv_block_stride_bytes, cache_block_size,
+                                           attn_sink, softmax_scale, out, out_stride_token, out_stride_head, lse, lse_stride_token,
+                                           lse_stride_head, num_tokens, num_heads, workspace);
+    if (rc != DSV4_OK) return rc;
+    if (topk < 0 || topk >= (1LL << 31)) return DSV4_ERR_BAD_SIZE;
+    if (num_tokens == 0 || num_heads == 0) return DSV4_OK;
+    if (!lens || !indices) return DSV4_ERR_NULL_POINTER;
+    p.indices = indices, p.indices_stride = indices_stride, p.topk = static_cast<int32_t>(topk), p.lens = lens;
+    return static_cast<int>(launch_latent_attention(p, workspace, static_cast<cudaStream_t>(cuda_stream)));
 }
 
 int dsv4_fused_indexer_q_rope_quant(const int64_t* positions, const void* index_q, int64_t q_stride0, int64_t q_stride1,

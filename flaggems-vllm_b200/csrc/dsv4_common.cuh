@@ -646,6 +646,9 @@ cudaError_t launch_topk_per_row(const float* logits, int64_t stride0, int64_t st
 cudaError_t launch_group_quant_fp8(const void* x, int64_t x_stride, void* out, float* scales, int64_t scale_stride_row,
                                    int64_t scale_stride_group, int64_t num_rows, int64_t num_cols, int group_size, float eps, int ue8m0,
                                    int act_quant_rules, cudaStream_t stream);
+cudaError_t launch_add_rmsnorm_quant(const void* x, int64_t x_stride, void* residual, int64_t residual_stride, const void* weight, void* out,
+                                     float* scales, int64_t scale_stride_row, int64_t scale_stride_group, int64_t rows, int64_t cols,
+                                     int64_t group_size, float eps, int fp16, int weight_f32, int pow2, cudaStream_t stream);
 cudaError_t launch_indexer_q_rope_quant(const int64_t* positions, const void* q, int64_t q_stride0, int64_t q_stride1,
                                         const void* cos_sin, int64_t cos_sin_stride, int cos_sin_bf16, int rot_dim, void* out,
                                         int64_t out_stride0, int64_t out_stride1, void* scales, int64_t scale_stride0,

@@ -20,6 +20,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <cstdio>
 
 #include "../../include/dsv4_prologue.h"
@@ -102,6 +103,25 @@ struct Arguments {
 
 bool is(const Tensor& t, ScalarType type) { return t.scalar_type() == type; }
 bool on(const Tensor& t, const Tensor& first) { return t.is_cuda() && t.get_device() == first.get_device(); }
+
+// The bytes that a tensor's elements lie in: [first, second).
+std::pair<const uint8_t*, const uint8_t*> extent(const Tensor& t) {
+    const auto* at = static_cast<const uint8_t*>(t.data_ptr());
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return {at, at + (last + 1) * static_cast<int64_t>(t.element_size())};
+}
+// Whether two tensors that are not empty lie in ranges of memory apart from each other.
+bool apart(const Tensor& a, const Tensor& b) {
+    const auto x = extent(a), y = extent(b);
+    return x.second <= y.first || y.second <= x.first;
+}
+// Whether no two elements of [tokens, heads] or [tokens, heads, row], the last unit stride, share memory: one of the two outer strides spans
+// the other dimension's rows.
+bool rows_apart(const Tensor& t) {
+    const int64_t row = t.dim() == 3 ? t.size(2) : 1, n0 = t.size(0), n1 = t.size(1), s0 = t.stride(0), s1 = t.stride(1);
+    return (n1 == 1 || s1 >= row) && (n0 == 1 || s0 >= row) && (n0 == 1 || n1 == 1 || s0 >= (n1 - 1) * s1 + row || s1 >= (n0 - 1) * s0 + row);
+}
 
 using dsv4::OnDevice;
 OnDevice on_device_of(const Tensor& t, OnDevice::Use use = OnDevice::kAllocatesToo) { return OnDevice(static_cast<c10::DeviceIndex>(t.get_device()), use); }
@@ -582,6 +602,133 @@ PyObject* persistent_topk(Arguments& a) {
     Py_RETURN_TRUE;
 }
 
+// x, residual or None, weight, eps, group_size, column_major_scales, scale_ue8m0 -> (x_q, scales)
+PyObject* add_rmsnorm_quant(Arguments& a) {
+    const Tensor* x = a.tensor(0);
+    const Tensor* residual = a.is_none(1) ? nullptr : a.tensor(1);
+    const Tensor* weight = a.tensor(2);
+    const float eps = a.real(3);
+    const int64_t group = a.integer(4);
+    const bool column_major = a.truth(5), ue8m0 = a.truth(6);
+    if (!a.ok) Py_RETURN_NONE;
+    REQUIRE(x->is_cuda() && x->dim() == 2 && (is(*x, at::kBFloat16) || is(*x, at::kHalf)) && x->stride(1) == 1);
+    if (!a.ok) Py_RETURN_NONE;
+    const int64_t rows = x->size(0), cols = x->size(1);
+    REQUIRE(group == cols || group == 32 || group == 64 || group == 128 || group == 256);
+    REQUIRE(group > 0 && cols % group == 0 && cols % 8 == 0);
+    REQUIRE(cols <= 32768);
+    REQUIRE(!residual || (residual->dim() == 2 && residual->sizes() == x->sizes() && is(*residual, x->scalar_type()) && residual->stride(1) == 1 && on(*residual, *x)));
+    REQUIRE(weight->dim() == 1 && weight->size(0) == cols && weight->is_contiguous() && on(*weight, *x));
+    REQUIRE(is(*weight, x->scalar_type()) || is(*weight, at::kFloat));
+    REQUIRE(rows <= 1 || (x->stride(0) >= cols && (!residual || residual->stride(0) >= cols)));
+    if (!a.ok) Py_RETURN_NONE;
+    REQUIRE(!residual || rows == 0 || apart(*x, *residual));
+    if (!a.ok) Py_RETURN_NONE;
+    const int64_t groups = cols / group;
+    const OnDevice here = on_device_of(*x);
+    Tensor xq = make_empty({rows, cols}, at::kFloat8_e4m3fn, here), xs = make_empty({rows, groups}, at::kFloat, here);
+    const int64_t stride_row = column_major ? 1 : groups, stride_group = column_major ? std::max<int64_t>(rows, 1) : 1;
+    if (column_major) set_view(xs, {rows, groups}, {stride_row, stride_group});
+    if (rows > 0 && !launch_on(here, [&](void* stream) {
+            return dsv4_fused_add_rmsnorm_quant_fp8(x->data_ptr(), x->stride(0), residual ? residual->data_ptr() : nullptr,
+                                                    residual ? residual->stride(0) : 0, weight->data_ptr(), xq.data_ptr(),
+                                                    static_cast<float*>(xs.data_ptr()), stride_row, stride_group, rows, cols, group, eps,
+                                                    is(*x, at::kHalf) ? 1 : 0, is(*weight, at::kFloat) ? 1 : 0,
+                                                    ue8m0 ? 1 : 0, stream);
+        }))
+        return nullptr;
+    return pair(std::move(xq), std::move(xs));
+}
+
+// What both attention operators take: queries, cache, page size, scale, sink, out, lse.
+struct AttentionTensors {
+    const Tensor *q, *cache, *sink, *out, *lse;
+    int64_t block;
+    float scale;
+};
+
+void require_attention(Arguments& a, const AttentionTensors& t) {
+    REQUIRE(t.q->is_cuda() && t.q->dim() == 3 && t.q->size(2) == 512 && is(*t.q, at::kBFloat16) && t.q->stride(2) == 1);
+    REQUIRE(is(*t.cache, at::kByte) && t.cache->dim() == 2 && t.cache->stride(1) == 1 && t.block > 0 && t.cache->size(1) / 584 >= t.block);
+    REQUIRE(t.cache->size(0) <= 1 || t.cache->stride(0) >= t.cache->size(1));
+    REQUIRE(t.scale > 0.0f && t.scale < INFINITY);
+    REQUIRE(on(*t.cache, *t.q));
+    if (!a.ok) return;
+    const int64_t tokens = t.q->size(0), heads = t.q->size(1);
+    REQUIRE(!t.sink || (t.sink->dim() == 1 && t.sink->size(0) == heads && is(*t.sink, at::kFloat) && t.sink->is_contiguous() && on(*t.sink, *t.q)));
+    REQUIRE(!t.out || (t.out->dim() == 3 && t.out->sizes() == t.q->sizes() && is(*t.out, at::kBFloat16) && t.out->stride(2) == 1 && on(*t.out, *t.q)));
+    REQUIRE(!t.lse || (t.lse->dim() == 2 && t.lse->size(0) == tokens && t.lse->size(1) == heads && is(*t.lse, at::kFloat) && on(*t.lse, *t.q)));
+    if (!a.ok) return;
+    REQUIRE(!t.out || tokens == 0 || heads == 0 || (apart(*t.out, *t.q) && rows_apart(*t.out)));
+    REQUIRE(!t.lse || tokens == 0 || heads == 0 || rows_apart(*t.lse));
+}
+
+// q, k_cache, block_table, seq_lens, query_start_loc, cache_block_size, softmax_scale, window_size or None, num_first_tokens,
+// attn_sink or None, out or None, lse or None -> out
+PyObject* paged_latent_attention(Arguments& a) {
+    const Tensor *q = a.tensor(0), *cache = a.tensor(1), *table = a.tensor(2), *seq = a.tensor(3), *start = a.tensor(4);
+    const AttentionTensors t{q, cache, a.is_none(9) ? nullptr : a.tensor(9), a.is_none(10) ? nullptr : a.tensor(10),
+                             a.is_none(11) ? nullptr : a.tensor(11), a.integer_of(5), a.real(6)};
+    const bool windowed = !a.is_none(7);
+    const int64_t window = windowed ? a.integer_of(7) : 0, first = a.integer_of(8);
+    if (!a.ok) Py_RETURN_NONE;
+    require_attention(a, t);
+    REQUIRE(table->dim() == 2 && is(*table, at::kInt) && table->stride(1) == 1 && on(*table, *q));
+    REQUIRE(seq->dim() == 1 && is(*seq, at::kInt) && seq->is_contiguous() && on(*seq, *q));
+    REQUIRE(start->dim() == 1 && is(*start, at::kInt) && start->is_contiguous() && on(*start, *q));
+    REQUIRE((!windowed || window >= 1) && first >= 0);
+    if (!a.ok) Py_RETURN_NONE;
+    const int64_t tokens = q->size(0), heads = q->size(1), requests = seq->size(0);
+    REQUIRE(table->size(0) == requests && start->size(0) == requests + 1);
+    if (!a.ok) Py_RETURN_NONE;
+    const OnDevice here = on_device_of(*q);
+    Tensor made = t.out ? *t.out : make_empty({tokens, heads, 512}, at::kBFloat16, here);
+    if (tokens > 0 && heads > 0 && requests > 0) {
+        const Tensor workspace = make_empty({dsv4_latent_attention_workspace_bytes(tokens, heads)}, at::kByte, here);
+        if (!launch_on(here, [&](void* stream) {
+                return dsv4_paged_latent_attention(
+                    q->data_ptr(), q->stride(0), q->stride(1), cache->data_ptr(), cache->size(0), cache->stride(0), t.block,
+                    static_cast<const int32_t*>(table->data_ptr()), table->stride(0), table->size(1), static_cast<const int32_t*>(seq->data_ptr()),
+                    static_cast<const int32_t*>(start->data_ptr()), requests, window, first,
+                    t.sink ? static_cast<const float*>(t.sink->data_ptr()) : nullptr, t.scale, made.data_ptr(), made.stride(0), made.stride(1),
+                    t.lse ? static_cast<float*>(t.lse->data_ptr()) : nullptr, t.lse ? t.lse->stride(0) : 0, t.lse ? t.lse->stride(1) : 0, tokens,
+                    heads, workspace.data_ptr(), stream);
+            }))
+            return nullptr;
+    }
+    return wrap(std::move(made));
+}
+
+// q, k_cache, indices, lens, cache_block_size, softmax_scale, attn_sink or None, out or None, lse or None -> out
+PyObject* sparse_latent_attention(Arguments& a) {
+    const Tensor *q = a.tensor(0), *cache = a.tensor(1), *indices = a.tensor(2), *lens = a.tensor(3);
+    const AttentionTensors t{q, cache, a.is_none(6) ? nullptr : a.tensor(6), a.is_none(7) ? nullptr : a.tensor(7),
+                             a.is_none(8) ? nullptr : a.tensor(8), a.integer_of(4), a.real(5)};
+    if (!a.ok) Py_RETURN_NONE;
+    require_attention(a, t);
+    REQUIRE(indices->dim() == 2 && is(*indices, at::kInt) && indices->stride(1) == 1 && on(*indices, *q));
+    REQUIRE(lens->dim() == 1 && is(*lens, at::kInt) && lens->is_contiguous() && on(*lens, *q));
+    if (!a.ok) Py_RETURN_NONE;
+    const int64_t tokens = q->size(0), heads = q->size(1);
+    REQUIRE(indices->size(0) == tokens && lens->size(0) == tokens);
+    if (!a.ok) Py_RETURN_NONE;
+    const OnDevice here = on_device_of(*q);
+    Tensor made = t.out ? *t.out : make_empty({tokens, heads, 512}, at::kBFloat16, here);
+    if (tokens > 0 && heads > 0) {
+        const Tensor workspace = make_empty({dsv4_latent_attention_workspace_bytes(tokens, heads)}, at::kByte, here);
+        if (!launch_on(here, [&](void* stream) {
+                return dsv4_sparse_latent_attention(
+                    q->data_ptr(), q->stride(0), q->stride(1), cache->data_ptr(), cache->size(0), cache->stride(0), t.block,
+                    static_cast<const int32_t*>(indices->data_ptr()), indices->stride(0), indices->size(1), static_cast<const int32_t*>(lens->data_ptr()),
+                    t.sink ? static_cast<const float*>(t.sink->data_ptr()) : nullptr, t.scale, made.data_ptr(), made.stride(0), made.stride(1),
+                    t.lse ? static_cast<float*>(t.lse->data_ptr()) : nullptr, t.lse ? t.lse->stride(0) : 0, t.lse ? t.lse->stride(1) : 0, tokens,
+                    heads, workspace.data_ptr(), stream);
+            }))
+            return nullptr;
+    }
+    return wrap(std::move(made));
+}
+
 PyObject* bind(PyObject*, PyObject* check) {
     Py_XDECREF(g_check);
     g_check = Py_NewRef(check);
@@ -606,6 +753,9 @@ PyMethodDef kMethods[] = {
     DSV4_ENTRY(top_k_decode),
     DSV4_ENTRY(top_k_prefill),
     DSV4_ENTRY(persistent_topk),
+    DSV4_ENTRY(add_rmsnorm_quant),
+    DSV4_ENTRY(paged_latent_attention),
+    DSV4_ENTRY(sparse_latent_attention),
     {"bind", bind, METH_O, nullptr},
     {"_refusal", refusal, METH_NOARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -29,6 +29,10 @@ EXPORTS = (
     "dsv4_combine_topk_swa_indices",
     "dsv4_per_token_group_quant_fp8",
     "dsv4_act_quant",
+    "dsv4_fused_add_rmsnorm_quant_fp8",
+    "dsv4_latent_attention_workspace_bytes",
+    "dsv4_paged_latent_attention",
+    "dsv4_sparse_latent_attention",
     "dsv4_top_k_per_row_decode",
     "dsv4_top_k_per_row_prefill",
     "dsv4_fused_indexer_q_rope_quant",

@@ -323,6 +323,57 @@ int dsv4_fused_indexer_q_rope_quant(const int64_t* positions, const void* index_
                                     void* cuda_stream);
 
 /*
+ * The way into the FP8 projections: residual addition, weighted RMS norm and activation quantiser in one pass.  The reference has the
+ * pieces apart (residual addition and norm in the caller's model, quantiser
+ * src/flaggems_vllm/ops/per_token_group_quant_fp8.py:226-330).  Per row, with z = x + residual in fp32 (z = x where residual is NULL):
+ *   residual <- z, rounded to the tensors' type
+ *   y = (z * r) * weight, r = fp32(1 / sqrt(mean(z^2) + eps)), the mean in 64 bits
+ *   scale = max(amax, 1e-10) / 448 per group of group_size values, made 2^ceil(log2(scale)) when scale_is_ue8m0
+ *   out = e4m3(y / scale), contiguous [num_rows, num_cols] bytes; a group with a NaN has a NaN scale
+ * x, residual: bf16 (is_fp16 = 0) or fp16 (1), row strides in elements, unit inner stride; weight [num_cols] of that type or, with
+ * weight_is_fp32, fp32.  group_size: 32, 64, 128, 256, or num_cols (one scale per row); num_cols a multiple of it and of 8, at most 32768.
+ * All rows on 16-byte boundaries.  residual must not overlap x or out.
+ */
+int dsv4_fused_add_rmsnorm_quant_fp8(const void* x, int64_t x_row_stride, void* residual, int64_t residual_row_stride, const void* weight,
+                                     void* out, float* scales, int64_t scale_stride_row, int64_t scale_stride_group, int64_t num_rows,
+                                     int64_t num_cols, int64_t group_size, float eps, int32_t is_fp16, int32_t weight_is_fp32,
+                                     int32_t scale_is_ue8m0, void* cuda_stream);
+
+/*
+ * Attention over the paged latent cache that dsv4_qnorm_rope_kv_insert writes: what a caller of the reference runs between the prologue
+ * and the epilogue (dsv4_fused_inv_rope_fp8_quant).  One cached row of 512 values, shared by all heads, is key and value at once:
+ *   s_j = softmax_scale * q . k_j,  out = sum_j e^(s_j) k_j / (sum_j e^(s_j) + e^(sink[head])),  lse = ln sum_j e^(s_j)
+ * over the keys that the token sees; a row that sees none, or none with a score above -inf, has out = 0 and lse = -inf.  The e^(sink)
+ * term is there where attn_sink is not NULL; lse does not contain it, and is only written where it is not NULL.
+ *   q, out     bf16 [num_tokens, num_heads, 512], strides in elements (multiples of 8), 16-byte aligned, not overlapping
+ *   lse        fp32, strides in elements
+ *   k_cache    as written by the prologue, num_blocks blocks; base and block stride on 16-byte boundaries
+ *   workspace  dsv4_latent_attention_workspace_bytes(...) bytes, 16-byte aligned, of this call alone until it has run
+ * Keys never influence a row that does not see them, whatever their bytes.  A key with a value that is not finite makes the whole output of
+ * the rows that see it NaN.
+ *
+ * Paged: request r has the tokens query_start_loc[r] .. query_start_loc[r+1]-1 (non-decreasing, [num_reqs + 1]), the last of them at
+ * position seq_lens[r] - 1.  A token at position p sees position j if j <= p and, where window_size > 0, j > p - window_size or
+ * j < num_first_tokens; a page that is outside 0 .. num_blocks-1, or beyond max_blocks_per_seq, is seen by no token.  Rows of q behind the
+ * last request's are left as they are in out and lse.
+ * Sparse: token t sees the slots indices[t, 0 .. lens[t]-1] (block * cache_block_size + offset); negative ones and ones outside
+ * the cache are skipped, a slot that is named twice counts twice.
+ */
+int64_t dsv4_latent_attention_workspace_bytes(int64_t num_tokens, int64_t num_heads);
+int dsv4_paged_latent_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_cache, int64_t num_blocks,
+                                int64_t kv_block_stride_bytes, int64_t cache_block_size, const int32_t* block_table,
+                                int64_t block_table_stride, int64_t max_blocks_per_seq, const int32_t* seq_lens,
+                                const int32_t* query_start_loc, int64_t num_reqs, int64_t window_size, int64_t num_first_tokens,
+                                const float* attn_sink, float softmax_scale, void* out, int64_t out_stride_token, int64_t out_stride_head,
+                                float* lse, int64_t lse_stride_token, int64_t lse_stride_head, int64_t num_tokens, int64_t num_heads,
+                                void* workspace, void* cuda_stream);
+int dsv4_sparse_latent_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_cache, int64_t num_blocks,
+                                 int64_t kv_block_stride_bytes, int64_t cache_block_size, const int32_t* indices, int64_t indices_stride,
+                                 int64_t topk, const int32_t* lens, const float* attn_sink, float softmax_scale, void* out,
+                                 int64_t out_stride_token, int64_t out_stride_head, float* lse, int64_t lse_stride_token,
+                                 int64_t lse_stride_head, int64_t num_tokens, int64_t num_heads, void* workspace, void* cuda_stream);
+
+/*
  * Reads into *value_host, and clears, the error word the kernels of the current device keep:
  * bit 0 = a bounded wait inside the DSV4_VARIANT_BULK kernel ran out (its result is then
  * incomplete).  Synchronises the device.  0 after every healthy run.  No counterpart in the reference.
