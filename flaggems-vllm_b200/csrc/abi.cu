@@ -523,10 +523,11 @@ int dsv4_paged_latent_attention(const void* q, int64_t q_stride_token, int64_t q
     if (!seq_lens || !query_start_loc || (!block_table && max_blocks_per_seq > 0)) return DSV4_ERR_NULL_POINTER;
     p.block_table = block_table, p.table_stride = block_table_stride, p.seq_lens = seq_lens, p.query_start_loc = query_start_loc;
     p.num_reqs = static_cast<int32_t>(num_reqs);
-    // (positions are below 2^31: larger windows, numbers of first tokens and tables are cut to that)
-    const auto cut = [lim](int64_t v) { return static_cast<int32_t>(v < lim - 1 ? v : lim - 1); };
-    p.window = cut(window_size), p.first = cut(num_first_tokens);
-    p.capacity = max_blocks_per_seq > lim / cache_block_size ? static_cast<int32_t>(lim - 1) : cut(max_blocks_per_seq * cache_block_size);
+    // positions are below 2^31: larger windows are none, larger numbers of first tokens are cut, and keys are numbered up to a block short of it
+    const int64_t most = lim - 256;
+    p.window = window_size < lim ? static_cast<int32_t>(window_size) : 0;
+    p.first = static_cast<int32_t>(num_first_tokens < most ? num_first_tokens : most);
+    p.capacity = static_cast<int32_t>(max_blocks_per_seq > most / cache_block_size ? most : max_blocks_per_seq * cache_block_size);
     return static_cast<int>(launch_latent_attention(p, workspace, static_cast<cudaStream_t>(cuda_stream)));
 }
 
@@ -540,7 +541,7 @@ int dsv4_sparse_latent_attention(const void* q, int64_t q_stride_token, int64_t 
                                            attn_sink, softmax_scale, out, out_stride_token, out_stride_head, lse, lse_stride_token,
                                            lse_stride_head, num_tokens, num_heads, workspace);
     if (rc != DSV4_OK) return rc;
-    if (topk < 0 || topk >= (1LL << 31)) return DSV4_ERR_BAD_SIZE;
+    if (topk < 0 || topk >= (1LL << 31) - 256) return DSV4_ERR_BAD_SIZE;
     if (num_tokens == 0 || num_heads == 0) return DSV4_OK;
     if (!lens || !indices) return DSV4_ERR_NULL_POINTER;
     p.indices = indices, p.indices_stride = indices_stride, p.topk = static_cast<int32_t>(topk), p.lens = lens;
@@ -578,9 +579,10 @@ int dsv4_fused_indexer_q_rope_quant(const int64_t* positions, const void* index_
 
 int dsv4_device_error(int32_t* value_host) {
     if (!value_host) return DSV4_ERR_NULL_POINTER;
-    int v = 0;
-    const cudaError_t err = read_device_error(&v);
-    *value_host = v;
+    int v = 0, attention = 0;
+    cudaError_t err = read_device_error(&v);
+    if (err == cudaSuccess) err = read_attention_error(&attention);
+    *value_host = v | (attention ? 2 : 0);
     return static_cast<int>(err);
 }
 

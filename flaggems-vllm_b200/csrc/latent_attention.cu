@@ -3,116 +3,855 @@
 //
 //   s_j = scale * q . k_j over the keys a token sees, o = sum_j e^(s_j - m) k_j / (sum_j e^(s_j - m) + e^(sink - m)), lse = m + ln sum_j e^(s_j - m)
 //
-// One warp per (token, head): 16 dimensions a lane, one key after another with a running maximum and sum.
+// in one pass over the keys with a running maximum m and sum.  Both products run on the tensor cores with fp32 accumulators in TMEM.
+//
+// A tile is 64 rows of q that share a list of keys: the heads of one token (64 of them at a time), or of several neighbouring tokens of a
+// request where there are fewer heads.  A CTA holds a tile's q (64 KiB) and streams its keys in blocks of 64:
+//   warps 4-11  "readers": find the 64 cached rows, convert them to bf16 and store them swizzled, once; the same bytes are the K-major
+//               operand of S = Q K^T and the MN-major operand of O += P V.  A block is two halves of 256 dimensions, four halves in all
+//               in a ring, so that a half is refilled as soon as the product that reads it last is done with it.
+//   warp 12     one thread issues the products: S of the next block before O of this one, so that they run while the softmax does.
+//   warps 0-3   "softmax": S from TMEM, masks, running maximum and sum, P as bf16 to shared memory; O is multiplied by a correction only where
+//               a row's maximum has grown by more than a factor of 2^8 (P and the sum may exceed one by that factor; fp32 holds them).
+//   warp 13     copies q of the next tile as soon as the last S of this one is done.
+// O takes 64 x 512 accumulators: 256 columns, dimensions 0-255 in lanes 0-15 of each 32 and 256-511 in lanes 16-31 (a product of 64 rows uses
+// 16 lanes of each 32).
+//
+// Rows of work are few in decoding and of any length, so the blocks of all tiles are dealt out evenly: every CTA computes the same prefix sum
+// over the tiles' numbers of blocks and takes its share, which may begin and end inside a tile.  Pieces of a tile go to a workspace as
+// unnormalised sums and are joined, in a fixed order, by a second small kernel.
 #include "dsv4_common.cuh"
 #include "latent_attention.cuh"
 
 namespace dsv4 {
+
+__device__ int g_attention_error = 0;
+
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kRows = 64, kBlockKeys = 64;
+constexpr int kSoftmaxWarps = 4, kReaderWarps = 8, kIssuerWarp = 12, kThreads = 14 * 32;
+constexpr float kMostGrowth = 8.0f;  // log2 of the factor that a row's maximum may have grown by before O is corrected
+constexpr int kMaxCtas = 148;        // a B200's SMs: one CTA on each (its shared memory allows no second)
+// Cuts between CTAs are moved to a tile's border where a piece would be short of this many blocks, and fewer CTAs take part where each
+// would have less than kLeastShare of them: a piece costs 128 KiB of fp32 sums out and in.
+constexpr int kLeastPiece = 2, kLeastShare = 4, kLeastSplit = 8;
 
-__device__ __forceinline__ float ue8m0_to_float(uint32_t code) {
-    if (code == 0u) return __uint_as_float(0x00400000u);
-    if (code == 255u) return __uint_as_float(0x7f800000u);
-    return __uint_as_float(code << 23);
+// ---- shared memory -----------------------------------------------------------------------------------------------------------
+
+constexpr int kChunkBytes = kRows * 128;           // 64 rows of 64 dimensions: eight 8-row, 128-byte swizzle atoms
+constexpr int kHalfBytes = 4 * kChunkBytes;        // 64 keys x 256 dimensions
+constexpr int kQueryBytes = 8 * kChunkBytes;
+constexpr int kOffsetKeys = kQueryBytes, kOffsetP = kOffsetKeys + 4 * kHalfBytes, kOffsetRest = kOffsetP + 2 * kChunkBytes;
+
+struct Cut {
+    int request, token, group, block;
+};
+struct Rest {
+    uint64_t kv_full[4], kv_empty[4], s_full[2], p_full[2], pv_done[2], q_full, q_empty, o_empty, drained;
+    uint64_t sums[16];
+    uint8_t valid[2][8], bad[2][8];  // a bit per key of a block: it exists, it has a value that is not finite
+    Cut from, to;
+    uint32_t tmem;
+    int abort;
+};
+constexpr int kSharedBytes = kOffsetRest + static_cast<int>(sizeof(Rest)) + 1024;  // (the base is moved up to a multiple of 1024)
+
+// ---- PTX ----------------------------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void barrier_init(uint64_t* bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_address(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void barrier_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_address(bar)) : "memory");
+}
+__device__ __forceinline__ bool barrier_try(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done)
+                 : "r"(shared_address(bar)), "r"(parity)
+                 : "memory");
+    return done != 0;
+}
+// Bounded: false, and the CTA's other roles told to leave, where the phase does not complete within about a second.
+__device__ __noinline__ bool barrier_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    const long long start = clock64();
+    for (uint32_t i = 0; i < (1u << 24); ++i) {
+        if (barrier_try(bar, parity)) return true;
+        if (*abort) return false;
+        if (clock64() - start > 2000000000LL) break;
+    }
+    *abort = 1;
+    atomicOr(&g_attention_error, 1);
+    return false;
+}
+__device__ __forceinline__ bool barrier_wait(uint64_t* bar, uint32_t parity, int* abort) {
+    return barrier_try(bar, parity) || barrier_wait_long(bar, parity, abort);
+}
+// The same by a whole warp, with one answer.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* abort) {
+    return __all_sync(0xffffffffu, barrier_wait(bar, parity, abort));
+}
+__device__ __forceinline__ void fence_to_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void fence_tmem_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_tmem_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_tmem_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void commit_to(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_address(bar)) : "memory");
+}
+__device__ __forceinline__ void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t kind, bool accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+                 "l"(b), "r"(kind), "r"(static_cast<uint32_t>(accumulate))
+                 : "memory");
+}
+#define DSV4_R8(v, i) "=f"(v[i]), "=f"(v[i + 1]), "=f"(v[i + 2]), "=f"(v[i + 3]), "=f"(v[i + 4]), "=f"(v[i + 5]), "=f"(v[i + 6]), "=f"(v[i + 7])
+#define DSV4_W8(v, i) "f"(v[i]), "f"(v[i + 1]), "f"(v[i + 2]), "f"(v[i + 3]), "f"(v[i + 4]), "f"(v[i + 5]), "f"(v[i + 6]), "f"(v[i + 7])
+#define DSV4_LIST32                                                                                                                       \
+    "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}"
+// 16 lanes x 64 columns: lane l of the warp gets, of columns 8j + 2(l % 4) + {0, 1}, row l / 4 in v[4j], v[4j + 1] and row l / 4 + 8 in the
+// next two.
+__device__ __forceinline__ void load_scores(float (&v)[32], uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x8.b32 " DSV4_LIST32 ", [%32];"
+                 : DSV4_R8(v, 0), DSV4_R8(v, 8), DSV4_R8(v, 16), DSV4_R8(v, 24)
+                 : "r"(at));
+}
+// 32 lanes x 32 columns, one lane a thread.
+__device__ __forceinline__ void load_columns(float (&v)[32], uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 " DSV4_LIST32 ", [%32];"
+                 : DSV4_R8(v, 0), DSV4_R8(v, 8), DSV4_R8(v, 16), DSV4_R8(v, 24)
+                 : "r"(at));
+}
+// Behind the loads of v: names it, so that nothing that uses it moves ahead of the wait.
+#define DSV4_U8(v, i) "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]), "+f"(v[i + 6]), "+f"(v[i + 7])
+__device__ __forceinline__ void wait_tmem_loads(float (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : DSV4_U8(v, 0), DSV4_U8(v, 8), DSV4_U8(v, 16), DSV4_U8(v, 24)::"memory");
+}
+__device__ __forceinline__ void store_columns(const float (&v)[32], uint32_t at) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], " DSV4_LIST32 ";" ::DSV4_W8(v, 0), DSV4_W8(v, 8), DSV4_W8(v, 16), DSV4_W8(v, 24),
+                 "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ void store_shared16(uint32_t at, uint4 v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void store_shared4(uint32_t at, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
-__global__ void __launch_bounds__(128) latent_attention_kernel(const Launched<LatentAttention> p) {
-    begin_dependent_kernel();
-    const int lane = threadIdx.x & 31;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    const int token = static_cast<int>(row / p.num_heads), head = static_cast<int>(row % p.num_heads);
-    if (token >= p.num_tokens) return;
-    int request = 0, position = 0, first = 0, low = 0, keys;
-    if (p.indices) {
-        keys = min(max(__ldg(p.lens + token), 0), p.topk);
+// Shared-memory operand with 128-byte swizzle: atoms of 8 rows x 128 bytes, the next 8 rows 1024 bytes on.  `leading`: bytes between chunks of
+// 64 dimensions, used where the dimensions are the operand's outer direction.
+__device__ __forceinline__ uint64_t operand(uint32_t address, uint32_t leading) {
+    return static_cast<uint64_t>((address & 0x3ffffu) >> 4) | (static_cast<uint64_t>(leading >> 4) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+// bf16 x bf16 -> fp32, 64 rows, n columns; `transposed`: the second operand's columns are contiguous.
+constexpr uint32_t kind_of(uint32_t n, bool transposed) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (transposed ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((kRows >> 4) << 24);
+}
+
+constexpr uint32_t kKindS = kind_of(kBlockKeys, false), kKindO = kind_of(256, true);
+
+// ---- tiles and their order ------------------------------------------------------------------------------------------------------
+
+struct Tiles {
+    LatentAttention a;
+    int32_t tokens_per_tile, heads_per_tile, head_groups;
+    float* sums;      // workspace: [2 * kMaxCtas][64][512] unnormalised outputs,
+    float2* rows;     // [2 * kMaxCtas][64] their maximum and sum,
+    int4* pieces;     // [2 * kMaxCtas] what they belong to: token, first head, rows, and 0: nothing, 1: more follow, 2: the last
+};
+
+// The keys of a tile as one list: `first` first tokens, then the positions from `low` on.
+struct Tile {
+    int token, count, head, rows, position, first, low, keys, blocks;
+};
+
+__device__ __forceinline__ Tile tile_at(const Tiles& p, int request, int token, int group) {
+    Tile t;
+    t.token = token, t.head = group * kRows;
+    t.position = t.first = t.low = 0;
+    if (p.a.indices) {
+        t.count = 1;
+        t.keys = min(max(__ldg(p.a.lens + token), 0), p.a.topk);
     } else {
-        while (request < p.num_reqs && __ldg(p.query_start_loc + request + 1) <= token) ++request;
-        const int start = request < p.num_reqs ? __ldg(p.query_start_loc + request) : 0;
-        if (request == p.num_reqs || token < start) return;
-        position = max(__ldg(p.seq_lens + request), 0) - __ldg(p.query_start_loc + request + 1) + token;
-        low = p.window > 0 ? max(0, position - p.window + 1) : 0;
-        first = min(min(low, p.first), p.capacity);
-        keys = max(0, min(position + 1, p.capacity) - low) + first;
+        const int end = min(__ldg(p.a.query_start_loc + request + 1), p.a.num_tokens);
+        t.count = min(p.tokens_per_tile, end - token);
+        t.position = max(__ldg(p.a.seq_lens + request), 0) - end + token;
+        t.low = p.a.window > 0 && t.position >= p.a.window ? t.position - p.a.window + 1 : 0;
+        t.first = min(min(t.low, p.a.first), p.a.capacity);
+        t.keys = max(0, min(t.position + t.count, p.a.capacity) - t.low) + t.first;
     }
-    const uint8_t* q = p.q + token * p.q_stride_token + head * p.q_stride_head + 32 * lane;
-    float qv[16], acc[16];
-    {
-        float a[8], b[8];
-        unpack8(*reinterpret_cast<const uint4*>(q), a), unpack8(*reinterpret_cast<const uint4*>(q + 16), b);
-        for (int i = 0; i < 8; ++i) qv[i] = a[i], qv[8 + i] = b[i];
-    }
-    for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    for (int j = 0; j < keys; ++j) {
-        int64_t block;
-        uint32_t in_block;
-        if (p.indices) {
-            const int slot = __ldg(p.indices + token * p.indices_stride + j);
-            if (slot < 0) continue;
-            block = fast_div(slot, p.block_mul, p.block_shift);
-            in_block = slot - static_cast<uint32_t>(block) * p.block_size;
-        } else {
-            const int pos = j < first ? j : j - first + low;
-            const uint32_t page = fast_div(pos, p.block_mul, p.block_shift);
-            in_block = pos - page * p.block_size;
-            block = __ldg(p.block_table + request * p.table_stride + page);
-        }
-        if (block < 0 || block >= p.num_blocks) continue;
-        const uint8_t* base = p.k_cache + block * p.block_stride;
-        const uint8_t* data = base + static_cast<int64_t>(in_block) * kTokenDataBytes;
-        float k[16];
-        if (lane < 28) {
-            const uint32_t code = base[static_cast<int64_t>(p.block_size) * kTokenDataBytes + static_cast<int64_t>(in_block) * kScaleBytes + (lane >> 2)];
-            const float scale = ue8m0_to_float(code);
-            const uint4 v = *reinterpret_cast<const uint4*>(data + 16 * lane);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-            for (int i = 0; i < 8; ++i) {
-                const float2 f = unpack_e4m3x2(static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1))));
-                k[2 * i] = f.x * scale, k[2 * i + 1] = f.y * scale;
-            }
-        } else {
-            float a[8], b[8];
-            const uint8_t* r = data + kNopeDim + 32 * (lane - 28);
-            unpack8(*reinterpret_cast<const uint4*>(r), a), unpack8(*reinterpret_cast<const uint4*>(r + 16), b);
-            for (int i = 0; i < 8; ++i) k[i] = a[i], k[8 + i] = b[i];
-        }
-        float s = 0.0f;
-        for (int i = 0; i < 16; ++i) s = fmaf(qv[i], k[i], s);
-        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        s *= p.scale * kLog2e;
-        if (!(s <= m)) {
-            const float to = s;
-            const float factor = m == -INFINITY ? 0.0f : exp2f(m - to);
-            l *= factor;
-            for (int i = 0; i < 16; ++i) acc[i] *= factor;
-            m = to;
-        }
-        const float w = m == -INFINITY ? 0.0f : exp2f(s - m);
-        l += w;
-        for (int i = 0; i < 16; ++i) acc[i] = fmaf(w, k[i], acc[i]);
-    }
-    if (p.lse && lane == 0)
-        p.lse[token * p.lse_stride_token + head * p.lse_stride_head] = l > 0.0f || l != l ? m / kLog2e + logf(l) : -INFINITY;
-    float total = l;
-    if (p.sink && l > 0.0f) total += exp2f(p.sink[head] * kLog2e - m);
-    const float inverse = l == 0.0f ? 0.0f : 1.0f / total;
-    uint8_t* out = p.out + token * p.out_stride_token + head * p.out_stride_head + 32 * lane;
-    float a[8], b[8];
-    for (int i = 0; i < 8; ++i) a[i] = acc[i] * inverse, b[i] = acc[8 + i] * inverse;
-    *reinterpret_cast<uint4*>(out) = pack8(a), *reinterpret_cast<uint4*>(out + 16) = pack8(b);
+    t.rows = p.head_groups > 1 ? min(kRows, p.a.num_heads - t.head) : t.count * p.a.num_heads;
+    t.blocks = static_cast<int>((static_cast<uint32_t>(t.keys) + kBlockKeys - 1) / kBlockKeys);
+    return t;
 }
+
+// Request of the first token at or behind `token` that belongs to one (num_reqs if none does), and that token.
+__device__ __forceinline__ int request_of(const Tiles& p, int& token) {
+    if (p.a.indices) return 0;
+    token = max(token, __ldg(p.a.query_start_loc));
+    int low = 0, high = p.a.num_reqs;  // the first request that ends behind the token
+    while (low < high) {
+        const int mid = (low + high) >> 1;
+        if (__ldg(p.a.query_start_loc + mid + 1) > token) high = mid;
+        else low = mid + 1;
+    }
+    return low;
+}
+
+// A CTA's share: pieces of tiles, in order.
+struct Walk {
+    Cut at, to;
+    Tile tile;
+    int begin, end;  // blocks of the tile
+    __device__ __forceinline__ void step(const Tiles& p) {
+        if (++at.group == p.head_groups) {
+            at.group = 0;
+            at.token += tile.count;
+            if (!p.a.indices)
+                while (at.request < p.a.num_reqs && __ldg(p.a.query_start_loc + at.request + 1) <= at.token) ++at.request;
+            if (at.request >= p.a.num_reqs && !p.a.indices) at.token = p.a.num_tokens;
+        }
+        at.block = 0;
+    }
+    // Makes `tile`, `begin` and `end` those of the piece at `at`, or of the first one behind it that is none of nothing; false at the end.
+    __device__ __forceinline__ bool settle(const Tiles& p) {
+        for (;;) {
+            if (at.token >= p.a.num_tokens || at.token > to.token || (at.token == to.token && at.group > to.group)) return false;
+            const bool last = at.token == to.token && at.group == to.group;
+            if (last && to.block == 0) return false;
+            tile = tile_at(p, at.request, at.token, at.group);
+            begin = at.block, end = last ? min(to.block, tile.blocks) : tile.blocks;
+            if (begin < end || tile.blocks == 0) return true;
+            step(p);
+        }
+    }
+    __device__ __forceinline__ bool whole() const { return begin == 0 && end == tile.blocks; }
+};
+
+// Every CTA's share has the same number of blocks, a tile counting one more for its own cost.  All threads take part; thread-uniform results in
+// rest.from and rest.to.
+__device__ __forceinline__ void make_plan(const Tiles& p, Rest& rest) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int each = (p.a.num_tokens + kThreads - 1) / kThreads;
+    const int begin = min(tid * each, p.a.num_tokens), end = min(begin + each, p.a.num_tokens);
+    // f(request, token, blocks) for the tiles' first tokens in [begin, end)
+    const auto for_tiles = [&](auto&& f) {
+        int token = begin, request = begin < end ? request_of(p, token) : 0;
+        while (token < end) {
+            if (!p.a.indices) {
+                while (request < p.a.num_reqs && __ldg(p.a.query_start_loc + request + 1) <= token) ++request;
+                if (request >= p.a.num_reqs) break;
+                const int start = __ldg(p.a.query_start_loc + request);
+                const int behind = (token - start) % p.tokens_per_tile;
+                if (behind != 0) {
+                    token += p.tokens_per_tile - behind;
+                    token = min(token, __ldg(p.a.query_start_loc + request + 1));
+                    continue;
+                }
+            }
+            const Tile t = tile_at(p, request, token, 0);
+            if (f(request, token, t.blocks)) break;
+            token += t.count;
+        }
+    };
+    uint64_t mine = 0;
+    for_tiles([&](int, int, int blocks) {
+        mine += static_cast<uint64_t>(blocks + 1) * p.head_groups;
+        return false;
+    });
+    uint64_t up_to = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint64_t other = __shfl_up_sync(0xffffffffu, up_to, d);
+        if (lane >= d) up_to += other;
+    }
+    if (lane == 31) rest.sums[warp] = up_to;
+    __syncthreads();
+    uint64_t total = 0, before = up_to - mine;
+    for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) before += rest.sums[w];
+        total += rest.sums[w];
+    }
+    const uint64_t ctas = min(static_cast<uint64_t>(gridDim.x), max(total / kLeastShare, static_cast<uint64_t>(1)));
+    if (tid == 0) rest.from = rest.to = Cut{p.a.num_reqs, p.a.num_tokens, 0, 0};
+    __syncthreads();
+    for (int side = 0; side < 2; ++side) {
+        const uint64_t cta = blockIdx.x + side;
+        if (cta >= ctas) continue;
+        const uint64_t cut = total * cta / ctas;
+        if (cut < before || cut >= before + mine) continue;
+        uint64_t at = before;
+        for_tiles([&](int request, int token, int blocks) {
+            const uint64_t next = at + static_cast<uint64_t>(blocks + 1) * p.head_groups;
+            if (cut >= next) {
+                at = next;
+                return false;
+            }
+            const int group = static_cast<int>((cut - at) / (blocks + 1)), offset = static_cast<int>((cut - at) % (blocks + 1));
+            int block = min(offset, blocks);
+            if (blocks < kLeastSplit) block = 2 * offset <= blocks ? 0 : blocks;
+            else if (block < kLeastPiece) block = 0;
+            else if (blocks - block < kLeastPiece) block = blocks;
+            (side == 0 ? rest.from : rest.to) = Cut{request, token, group, block};
+            return true;
+        });
+    }
+    __syncthreads();
+}
+
+// ---- the kernel -------------------------------------------------------------------------------------------------------------------
+
+// Two e4m3 bytes of `word` (the low ones, or the high ones) times a scale, as a bf16 pair.
+template <int HIGH>
+__device__ __forceinline__ uint32_t two_values(uint32_t word, float scale) {
+    uint32_t halves, out;
+    const auto pair = static_cast<uint16_t>(HIGH ? word >> 16 : word);
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(halves) : "h"(pair));
+    float lo, hi;
+    asm("{.reg .f16 l, h; mov.b32 {l, h}, %2; cvt.f32.f16 %0, l; cvt.f32.f16 %1, h;}" : "=f"(lo), "=f"(hi) : "r"(halves));
+    out = pack_bf16x2(__fmul_rn(lo, scale), __fmul_rn(hi, scale));
+    return out;
+}
+
+__device__ __forceinline__ float power_of_code(uint32_t code) {
+    return code == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(code << 23);  // (255: infinity)
+}
+
+// Whether one of a bf16 pair is infinite or NaN.
+__device__ __forceinline__ bool not_finite(uint32_t pair) { return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u; }
+__device__ __forceinline__ bool not_finite(const uint4& v) { return not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w); }
+
+// What a reader lane holds of its four keys of a block: 16 bytes of each half's values (32 of the rotary ones), scale codes.
+struct Held {
+    uint4 low[4], high[4], rotary[4];
+    uint2 codes[4];
+};
+
+__global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Launched<Tiles> p) {
+    extern __shared__ uint8_t raw[];
+    uint8_t* shared = raw + ((1024u - (shared_address(raw) & 1023u)) & 1023u);
+    Rest& rest = *reinterpret_cast<Rest*>(shared + kOffsetRest);
+    const uint32_t base = shared_address(shared);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 4; ++i) barrier_init(&rest.kv_full[i], kReaderWarps), barrier_init(&rest.kv_empty[i], 1);
+        for (int i = 0; i < 2; ++i) barrier_init(&rest.s_full[i], 1), barrier_init(&rest.p_full[i], kSoftmaxWarps), barrier_init(&rest.pv_done[i], 1);
+        barrier_init(&rest.q_full, 1), barrier_init(&rest.q_empty, 1), barrier_init(&rest.o_empty, kSoftmaxWarps), barrier_init(&rest.drained, 1);
+        rest.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_to_async();
+    }
+    if (warp == kIssuerWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(shared_address(&rest.tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    begin_dependent_kernel();
+    make_plan(p, rest);
+    fence_tmem_before();
+    __syncthreads();
+    fence_tmem_after();
+    const uint32_t tmem = rest.tmem, tmem_scores = tmem + 256;
+    int* abort = &rest.abort;
+    Walk w;
+    w.at = rest.from, w.to = rest.to;
+
+    if (warp < kSoftmaxWarps) {
+        // ------------------------------------------------------------------------------------------------ softmax, outputs
+        const float c = p.a.scale * kLog2e;
+        const int row_a = 16 * warp + (lane >> 2), quad = 2 * (lane & 3);
+        const uint32_t lanes = static_cast<uint32_t>(32 * warp) << 16;
+        int it = 0;
+        bool ok = true;
+        const int slot_of_head = 2 * blockIdx.x + 1, slot_of_rest = 2 * blockIdx.x;
+        if (threadIdx.x < 2 && p.pieces) p.pieces[2 * blockIdx.x + threadIdx.x] = make_int4(0, 0, 0, 0);
+        __syncwarp();
+        for (; ok && w.settle(p); w.step(p)) {
+            const Tile& t = w.tile;
+            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+            // positions of this thread's two rows
+            const int last = t.position + t.count - 1;
+            int position[2] = {t.position, t.position};
+            if (t.count > 1) position[0] += row_a / p.a.num_heads, position[1] += (row_a + 8) / p.a.num_heads;
+            for (int block = w.begin; block < w.end; ++block, ++it) {
+                const int buffer = it & 1;
+                const uint32_t parity = (it >> 1) & 1;
+                if (!warp_wait(&rest.s_full[buffer], parity, abort) || !warp_wait(&rest.kv_full[2 * buffer + 1], parity, abort)) {
+                    ok = false;
+                    break;
+                }
+                fence_tmem_after();
+                float s[32];
+                load_scores(s, tmem_scores + 64 * buffer + lanes);
+                const uint64_t valid = *reinterpret_cast<const uint64_t*>(rest.valid[buffer]);
+                const int k0 = block * kBlockKeys;
+                bool mixed = false;
+                if (t.count > 1) {
+                    const int k1 = min(k0 + kBlockKeys, t.keys) - 1;
+                    const int newest = k1 < t.first ? k1 : k1 - t.first + t.low;
+                    mixed = newest > t.position || (p.a.window > 0 && (k0 < t.first || k0 - t.first + t.low <= last - p.a.window));
+                }
+                wait_tmem_loads(s);
+                if (mixed) {
+                    const uint64_t bad = *reinterpret_cast<const uint64_t*>(rest.bad[buffer]);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int k = 8 * (i >> 2) + quad + (i & 1);
+                        const int at = k0 + k, where = at < t.first ? at : at - t.first + t.low;
+                        const int mine = position[(i >> 1) & 1];
+                        const bool seen = ((valid >> k) & 1) != 0 && where <= mine && (p.a.window <= 0 || mine - where < p.a.window || where < p.a.first);
+                        s[i] = !seen ? -INFINITY : ((bad >> k) & 1) != 0 ? NAN : s[i];
+                    }
+                } else if (valid != ~0ull) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (((valid >> (8 * (i >> 2) + quad + (i & 1))) & 1) == 0) s[i] = -INFINITY;
+                }
+                float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < 32; ++i) top[(i >> 1) & 1] = fmaxf(top[(i >> 1) & 1], s[i]);
+                float factor[2] = {1.0f, 1.0f};
+                bool grown = false;
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+                    if (m[r] == -INFINITY) {
+                        m[r] = top[r];  // (nothing but zeros so far)
+                    } else if ((top[r] - m[r]) * c > kMostGrowth) {
+                        factor[r] = exp2_approx((m[r] - top[r]) * c);
+                        l[r] *= factor[r];
+                        m[r] = top[r];
+                        grown = true;
+                    }
+                }
+                if (__any_sync(0xffffffffu, grown)) {
+                    // O has been written up to the block before this one
+                    if (!warp_wait(&rest.pv_done[buffer ^ 1], ((it - 1) >> 1) & 1, abort)) {
+                        ok = false;
+                        break;
+                    }
+                    fence_tmem_after();
+                    const int from = (lane & 7) << 2;
+                    const float fa = __shfl_sync(0xffffffffu, factor[0], from), fb = __shfl_sync(0xffffffffu, factor[1], from);
+                    const float f = (lane & 8) ? fb : fa;
+#pragma unroll 1
+                    for (int at = 0; at < 256; at += 32) {
+                        float o[32];
+                        load_columns(o, tmem + at + lanes);
+                        wait_tmem_loads(o);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] *= f;
+                        store_columns(o, tmem + at + lanes);
+                    }
+                    wait_tmem_stores();
+                }
+                const float mc[2] = {m[0] == -INFINITY ? 0.0f : m[0] * c, m[1] == -INFINITY ? 0.0f : m[1] * c};
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    s[i] = exp2_approx(fmaf(s[i], c, -mc[(i >> 1) & 1]));
+                    l[(i >> 1) & 1] += s[i];
+                }
+                // P of two blocks ago has been read
+                if (it >= 2 && !warp_wait(&rest.pv_done[buffer], ((it >> 1) - 1) & 1, abort)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t to = base + kOffsetP + buffer * kChunkBytes + row_a * 128 + 2 * quad;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t unit = (j ^ (row_a & 7)) << 4;  // (row_a + 8 has the same low bits)
+                    store_shared4(to + unit, pack_bf16x2(s[4 * j], s[4 * j + 1]));
+                    store_shared4(to + 8 * 128 + unit, pack_bf16x2(s[4 * j + 2], s[4 * j + 3]));
+                }
+                fence_to_async();
+                fence_tmem_before();
+                __syncwarp();
+                if (lane == 0) barrier_arrive(&rest.p_full[buffer]);
+            }
+            if (!ok) break;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            }
+            // from here on a lane's row is the one it has in TMEM: 16 * warp + lane % 16, dimensions 256 * (lane / 16) on
+            const int from = (lane & 7) << 2, row = 16 * warp + (lane & 15);
+            const float ma = __shfl_sync(0xffffffffu, m[0], from), mb = __shfl_sync(0xffffffffu, m[1], from);
+            const float la = __shfl_sync(0xffffffffu, l[0], from), lb = __shfl_sync(0xffffffffu, l[1], from);
+            const float row_m = (lane & 8) ? mb : ma, row_l = (lane & 8) ? lb : la;
+            const bool live = row < t.rows;
+            const int token = t.token + (t.count > 1 ? row / p.a.num_heads : 0);
+            const int head = t.count > 1 ? row % p.a.num_heads : t.head + row;
+            if (w.begin < w.end) {
+                if (!warp_wait(&rest.pv_done[(it - 1) & 1], ((it - 1) >> 1) & 1, abort)) {
+                    ok = false;
+                    break;
+                }
+                fence_tmem_after();
+            }
+            if (w.whole()) {
+                const bool some = row_l != 0.0f;
+                float total = row_l;
+                if (live && p.a.sink && some) total += exp2_approx(fmaf(__ldg(p.a.sink + head), kLog2e, -row_m * c));
+                const float inverse = some ? 1.0f / total : 0.0f;
+                uint8_t* out = p.a.out + token * p.a.out_stride_token + head * p.a.out_stride_head + 512 * (lane >> 4);
+                if (live && lane < 16 && p.a.lse)
+                    p.a.lse[token * p.a.lse_stride_token + head * p.a.lse_stride_head] = some ? (row_m * c + log2f(row_l)) * kLn2 : -INFINITY;
+#pragma unroll 1
+                for (int at = 0; at < 256; at += 32) {
+                    float o[32];
+                    if (w.begin < w.end) {
+                        load_columns(o, tmem + at + lanes);
+                        wait_tmem_loads(o);
+                    }
+                    if (live) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                            if (some)
+                                v = make_uint4(pack_bf16x2(o[i] * inverse, o[i + 1] * inverse), pack_bf16x2(o[i + 2] * inverse, o[i + 3] * inverse),
+                                               pack_bf16x2(o[i + 4] * inverse, o[i + 5] * inverse), pack_bf16x2(o[i + 6] * inverse, o[i + 7] * inverse));
+                            *reinterpret_cast<uint4*>(out + 2 * (at + i)) = v;
+                        }
+                    }
+                }
+            } else {
+                const int slot = w.begin == 0 ? slot_of_head : slot_of_rest;
+                float* out = p.sums + (static_cast<int64_t>(slot) * kRows + row) * kHeadDim + 256 * (lane >> 4);
+                if (lane < 16) p.rows[slot * kRows + row] = make_float2(row_m, row_l);
+                if (threadIdx.x == 0) p.pieces[slot] = make_int4(t.token, t.head, t.rows, w.end == t.blocks ? 2 : 1);
+#pragma unroll 1
+                for (int at = 0; at < 256; at += 32) {
+                    float o[32];
+                    load_columns(o, tmem + at + lanes);
+                    wait_tmem_loads(o);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(out + at + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                }
+            }
+            if (w.begin < w.end) {
+                fence_tmem_before();
+                __syncwarp();
+                if (lane == 0) barrier_arrive(&rest.o_empty);
+            }
+        }
+    } else if (warp < kIssuerWarp) {
+        // ------------------------------------------------------------------------------------------------ readers
+        const int reader = warp - kSoftmaxWarps, sub = lane >> 1, odd = lane & 1;
+        // keys 8 * reader + 2 i + odd of a block; of each, dimensions 16 sub .. of both halves (rotary ones: sub 12-15 of the second).  Two
+        // neighbouring keys and four subs, which are what eight lanes store at once, hit all eight 16-byte columns of the swizzle.
+        const int key_a = 8 * reader + odd;
+        const uint32_t store_at = base + kOffsetKeys + (sub >> 2) * kChunkBytes + key_a * 128;
+        const uint32_t unit = 2 * (sub & 3);
+        const bool rotary = sub >= 12;
+        Held h;
+        uint32_t valid = 0;     // of the block whose values are held
+        // pages (or slots) of the block whose values are asked for next
+        const auto find = [&](const Walk& w, int block, int (&page)[4]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int k = block * kBlockKeys + key_a + 2 * i;
+                page[i] = -1;
+                if (k < w.tile.keys) {
+                    if (p.a.indices) {
+                        page[i] = __ldg(p.a.indices + w.tile.token * p.a.indices_stride + k);
+                    } else {
+                        const int where = k < w.tile.first ? k : k - w.tile.first + w.tile.low;
+                        page[i] = __ldg(p.a.block_table + w.at.request * p.a.table_stride + fast_div(where, p.a.block_mul, p.a.block_shift));
+                    }
+                }
+            }
+        };
+        const uint8_t* data[4];
+        const auto ask_low = [&](const Walk& w, int block, const int (&page)[4]) {
+            uint32_t bits = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int k = block * kBlockKeys + key_a + 2 * i;
+                uint32_t at = p.a.indices ? static_cast<uint32_t>(max(page[i], 0)) : k < w.tile.first ? k : k - w.tile.first + w.tile.low;
+                const uint32_t quotient = fast_div(at, p.a.block_mul, p.a.block_shift);
+                const uint32_t in_block = at - quotient * p.a.block_size;
+                const int number = p.a.indices ? static_cast<int>(quotient) : page[i];
+                const bool there = page[i] >= 0 && number < p.a.num_blocks;
+                data[i] = nullptr;
+                h.low[i] = make_uint4(0u, 0u, 0u, 0u), h.codes[i] = make_uint2(0u, 0u);
+                if (there) {
+                    const uint8_t* block_at = p.a.k_cache + number * p.a.block_stride;
+                    data[i] = block_at + static_cast<int64_t>(in_block) * kTokenDataBytes;
+                    h.low[i] = ld_stream16(data[i] + 16 * sub);
+                    h.codes[i] = __ldg(reinterpret_cast<const uint2*>(block_at + static_cast<int64_t>(p.a.block_size) * kTokenDataBytes + static_cast<int64_t>(in_block) * kScaleBytes));
+                    bits |= 1u << (2 * i + odd);
+                }
+            }
+            return bits | __shfl_xor_sync(0xffffffffu, bits, 1);
+        };
+        const auto ask_high = [&] {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                h.high[i] = h.rotary[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (data[i]) {
+                    const uint8_t* at = rotary ? data[i] + kNopeDim + 32 * (sub - 12) : data[i] + 256 + 16 * sub;
+                    h.high[i] = ld_stream16(at);
+                    if (rotary) h.rotary[i] = ld_stream16(at + 16);
+                }
+            }
+        };
+        // 16 e4m3 values to two 16-byte columns
+        const auto convert = [&](const uint4& v, float scale, uint4& a, uint4& b) {
+            a = make_uint4(two_values<0>(v.x, scale), two_values<1>(v.x, scale), two_values<0>(v.y, scale), two_values<1>(v.y, scale));
+            b = make_uint4(two_values<0>(v.z, scale), two_values<1>(v.z, scale), two_values<0>(v.w, scale), two_values<1>(v.w, scale));
+        };
+        const auto store = [&](uint32_t half, int i, const uint4& a, const uint4& b) {
+            const uint32_t at = store_at + half * kHalfBytes + 2 * i * 128, twist = (key_a + 2 * i) & 7;
+            store_shared16(at + ((unit ^ twist) << 4), a);
+            store_shared16(at + (((unit + 1) ^ twist) << 4), b);
+        };
+        bool more = w.settle(p);
+        while (more && w.begin == w.end) w.step(p), more = w.settle(p);
+        int block = w.begin;
+        uint2 codes[4];
+        if (more) {
+            int page[4];
+            find(w, block, page);
+            valid = ask_low(w, block, page);
+            ask_high();
+        }
+        for (int it = 0; more; ++it) {
+            const uint32_t slot = 2 * (it & 1), parity = ((it >> 1) - 1) & 1;
+            // this block's mask, then on to the next block
+            bool mixed = false;
+            if (w.tile.count > 1) {
+                const int k0 = block * kBlockKeys, k1 = min(k0 + kBlockKeys, w.tile.keys) - 1;
+                const int newest = k1 < w.tile.first ? k1 : k1 - w.tile.first + w.tile.low;
+                mixed = newest > w.tile.position ||
+                        (p.a.window > 0 && (k0 < w.tile.first || k0 - w.tile.first + w.tile.low <= w.tile.position + w.tile.count - 1 - p.a.window));
+            }
+            const uint32_t valid_now = valid;
+            int page[4];
+            if (++block == w.end) {
+                do {
+                    w.step(p), more = w.settle(p);
+                } while (more && w.begin == w.end);
+                block = w.begin;
+            }
+            if (more) find(w, block, page);
+
+            if (it >= 2 && !warp_wait(&rest.kv_empty[slot], parity, abort)) break;
+            uint32_t bad = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint4 a, b;
+                convert(h.low[i], power_of_code((h.codes[i].x >> (8 * (sub >> 2))) & 0xffu), a, b);
+                store(slot, i, a, b);
+                if (mixed && (not_finite(a) || not_finite(b))) bad |= 1u << (2 * i + odd);
+                codes[i] = h.codes[i];
+            }
+            if (!mixed) {
+                fence_to_async();
+                __syncwarp();
+                if (lane == 0) barrier_arrive(&rest.kv_full[slot]);
+            }
+            if (more) valid = ask_low(w, block, page);
+            if (it >= 2 && !warp_wait(&rest.kv_empty[slot + 1], parity, abort)) break;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint4 a = h.high[i], b = h.rotary[i];
+                if (!rotary) convert(h.high[i], power_of_code((codes[i].y >> (8 * (sub >> 2))) & 0xffu), a, b);
+                store(slot + 1, i, a, b);
+                if (mixed && (not_finite(a) || not_finite(b))) bad |= 1u << (2 * i + odd);
+            }
+            if (more) ask_high();
+            if (mixed) {
+                // Keys that some rows of the tile do not see: those with a value that is not finite are stored as zeros, which the rows that do
+                // not see them multiply by zero; the others get NaN as their score.
+                bad = __reduce_or_sync(0xffffffffu, bad);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if ((bad >> (2 * i + odd)) & 1u) {
+                        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+                        store(slot, i, zero, zero), store(slot + 1, i, zero, zero);
+                    }
+                }
+            }
+            if (lane == 0) rest.valid[it & 1][reader] = static_cast<uint8_t>(valid_now), rest.bad[it & 1][reader] = static_cast<uint8_t>(bad);
+            fence_to_async();
+            __syncwarp();
+            if (lane == 0) {
+                if (mixed) barrier_arrive(&rest.kv_full[slot]);
+                barrier_arrive(&rest.kv_full[slot + 1]);
+            }
+        }
+    } else if (warp == kIssuerWarp) {
+        // ------------------------------------------------------------------------------------------------ products
+        if (lane == 0) {
+            bool ok = true;
+            int it = 0, tiles = 0;
+            const auto product_o = [&](int i, bool first, int tile) {  // O += P V of block i
+                const int buffer = i & 1;
+                if (!barrier_wait(&rest.p_full[buffer], (i >> 1) & 1, abort)) return false;
+                if (first && tile > 0 && !barrier_wait(&rest.o_empty, (tile - 1) & 1, abort)) return false;
+                fence_tmem_after();
+                for (int half = 0; half < 2; ++half) {
+                    const uint64_t a = operand(base + kOffsetP + buffer * kChunkBytes, 16);
+                    const uint64_t b = operand(base + kOffsetKeys + (2 * buffer + half) * kHalfBytes, kChunkBytes);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        multiply(tmem + (static_cast<uint32_t>(16 * half) << 16), a + k * (32 >> 4), b + k * (2048 >> 4), kKindO, !first || k > 0);
+                    commit_to(&rest.kv_empty[2 * buffer + half]);
+                }
+                commit_to(&rest.pv_done[buffer]);
+                return true;
+            };
+            bool pending = false, pending_first = false;
+            int pending_tile = 0;
+            for (; ok && w.settle(p); w.step(p)) {
+                if (w.begin == w.end) continue;
+                // (q of this tile is on its way while the last product of the one before runs)
+                if (pending && !product_o(it - 1, pending_first, pending_tile)) break;
+                pending = false;
+                if (!barrier_wait(&rest.q_full, tiles & 1, abort)) break;
+                for (int block = w.begin; block < w.end; ++block, ++it) {
+                    const int buffer = it & 1;
+                    for (int half = 0; half < 2 && ok; ++half) {
+                        ok = barrier_wait(&rest.kv_full[2 * buffer + half], (it >> 1) & 1, abort);
+                        if (!ok) break;
+                        fence_tmem_after();
+#pragma unroll
+                        for (int chunk = 0; chunk < 4; ++chunk) {
+                            const uint64_t a = operand(base + (4 * half + chunk) * kChunkBytes, 16);
+                            const uint64_t b = operand(base + kOffsetKeys + (2 * buffer + half) * kHalfBytes + chunk * kChunkBytes, 16);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                multiply(tmem_scores + 64 * buffer, a + k * (32 >> 4), b + k * (32 >> 4), kKindS, half + chunk + k > 0);
+                        }
+                    }
+                    if (!ok) break;
+                    commit_to(&rest.s_full[buffer]);
+                    if (block + 1 == w.end) commit_to(&rest.q_empty);
+                    if (pending) ok = product_o(it - 1, pending_first, pending_tile);
+                    if (!ok) break;
+                    pending = true, pending_first = block == w.begin, pending_tile = tiles;
+                }
+                ++tiles;
+            }
+            if (ok && pending) product_o(it - 1, pending_first, pending_tile);
+            // nothing of this CTA may be in flight when its memory is given back
+            commit_to(&rest.drained);
+            for (uint32_t i = 0; i < (1u << 24) && !barrier_try(&rest.drained, 0); ++i) {}
+        }
+        __syncwarp();
+    } else {
+        // ------------------------------------------------------------------------------------------------ queries
+        int tiles = 0;
+        for (; w.settle(p); w.step(p)) {
+            if (w.begin == w.end) continue;
+            const Tile& t = w.tile;
+            if (tiles > 0 && !warp_wait(&rest.q_empty, (tiles - 1) & 1, abort)) break;
+            // a row is 64 pieces of 16 bytes: two passes of the warp
+            for (int row = 0; row < kRows; ++row) {
+                const int token = t.token + (t.count > 1 ? row / p.a.num_heads : 0);
+                const int head = t.count > 1 ? row % p.a.num_heads : t.head + row;
+                const bool live = row < t.rows;
+                const uint8_t* from = live ? p.a.q + token * p.a.q_stride_token + head * p.a.q_stride_head : p.a.q;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int piece = lane + 32 * i;
+                    const uint32_t to = base + (piece >> 3) * kChunkBytes + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(live ? from + 16 * piece : from), "r"(live ? 16 : 0) : "memory");
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_to_async();
+            __syncwarp();
+            if (lane == 0) barrier_arrive(&rest.q_full);
+            ++tiles;
+        }
+    }
+    fence_tmem_before();
+    __syncthreads();
+    if (warp == kIssuerWarp) {
+        fence_tmem_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+}
+
+// Joins the pieces of tiles that were cut: the CTAs (c, .) those of the tile whose first piece CTA c had, a few rows each.
+constexpr int kJoinedRows = 4;
+__global__ void __launch_bounds__(128) join_pieces_kernel(const Launched<Tiles> p) {
+    begin_dependent_kernel();
+    const int4 head = p.pieces[2 * blockIdx.x + 1];
+    if (head.w == 0) return;
+    const float c = p.a.scale * kLog2e;
+    for (int r = 0; r < kJoinedRows; ++r) {
+        const int row = blockIdx.y * kJoinedRows + r;
+        if (row >= head.z) return;
+        float m = -INFINITY;
+        const auto for_pieces = [&](auto&& f) {
+            f(2 * blockIdx.x + 1);
+            for (unsigned cta = blockIdx.x + 1; cta < gridDim.x; ++cta) {
+                const int kind = p.pieces[2 * cta].w;
+                if (kind != 0) f(2 * cta);
+                if (kind == 2) break;
+            }
+        };
+        for_pieces([&](int slot) { m = fmaxf(m, p.rows[slot * kRows + row].x); });
+        float l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for_pieces([&](int slot) {
+            const float2 s = p.rows[slot * kRows + row];
+            const float f = s.x == -INFINITY ? (s.y == 0.0f ? 0.0f : 1.0f) : exp2_approx((s.x - m) * c);
+            const float4 v = *reinterpret_cast<const float4*>(p.sums + (static_cast<int64_t>(slot) * kRows + row) * kHeadDim + 4 * threadIdx.x);
+            l = fmaf(s.y, f, l);
+            if (f != 0.0f) o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
+        });
+        const int token = head.x + (p.head_groups == 1 ? row / p.a.num_heads : 0), at = p.head_groups == 1 ? row % p.a.num_heads : head.y + row;
+        const bool some = l != 0.0f;
+        float total = l;
+        if (p.a.sink && some) total += exp2_approx(fmaf(__ldg(p.a.sink + at), kLog2e, -m * c));
+        const float inverse = some ? 1.0f / total : 0.0f;
+        uint8_t* out = p.a.out + token * p.a.out_stride_token + at * p.a.out_stride_head + 8 * threadIdx.x;
+        *reinterpret_cast<uint2*>(out) = some ? make_uint2(pack_bf16x2(o.x * inverse, o.y * inverse), pack_bf16x2(o.z * inverse, o.w * inverse)) : make_uint2(0u, 0u);
+        if (threadIdx.x == 0 && p.a.lse)
+            p.a.lse[token * p.a.lse_stride_token + at * p.a.lse_stride_head] = some ? (m * c + log2f(l)) * kLn2 : -INFINITY;
+    }
+}
+
+constexpr size_t kSumBytes = sizeof(float) * 2 * kMaxCtas * kRows * kHeadDim, kRowBytes2 = sizeof(float2) * 2 * kMaxCtas * kRows;
 
 }  // namespace
 
-size_t latent_attention_workspace(int64_t num_tokens, int64_t num_heads) { return 0; }
+size_t latent_attention_workspace(int64_t, int64_t) { return kSumBytes + kRowBytes2 + sizeof(int4) * 2 * kMaxCtas; }
 
-cudaError_t launch_latent_attention(const LatentAttention& p, void* workspace, cudaStream_t stream) {
-    const int64_t rows = static_cast<int64_t>(p.num_tokens) * p.num_heads;
-    launch_dependent(latent_attention_kernel, static_cast<unsigned>((rows + 3) / 4), 128, stream, p);
+cudaError_t launch_latent_attention(const LatentAttention& a, void* workspace, cudaStream_t stream) {
+    Tiles p{};
+    p.a = a;
+    p.tokens_per_tile = a.indices || a.num_heads >= kRows ? 1 : kRows / a.num_heads;
+    p.head_groups = (a.num_heads + kRows - 1) / kRows;
+    auto* at = static_cast<uint8_t*>(workspace);
+    p.sums = reinterpret_cast<float*>(at), p.rows = reinterpret_cast<float2*>(at + kSumBytes), p.pieces = reinterpret_cast<int4*>(at + kSumBytes + kRowBytes2);
+    // Set for the current device each time: cheaper than to remember for which ones it was.
+    cudaError_t rc = cudaFuncSetAttribute(latent_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedBytes);
+    if (rc != cudaSuccess) return rc;
+    rc = launch_dependent_cluster(latent_attention_kernel, dim3(kMaxCtas), dim3(kThreads), 1, kSharedBytes, stream, p);
+    if (rc != cudaSuccess) return rc;
+    count_launch();
+    rc = launch_dependent(join_pieces_kernel, dim3(kMaxCtas, kRows / kJoinedRows), dim3(128), stream, p);
+    if (rc != cudaSuccess) return rc;
     count_launch();
     return cudaGetLastError();
+}
+
+cudaError_t read_attention_error(int* value) {
+    int zero = 0;
+    const cudaError_t rc = cudaMemcpyFromSymbol(value, g_attention_error, sizeof(int));
+    return rc != cudaSuccess || *value == 0 ? rc : cudaMemcpyToSymbol(g_attention_error, &zero, sizeof(int));
 }
 
 }  // namespace dsv4

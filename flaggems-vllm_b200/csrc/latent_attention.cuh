@@ -32,5 +32,6 @@ struct LatentAttention {
 
 size_t latent_attention_workspace(int64_t num_tokens, int64_t num_heads);
 cudaError_t launch_latent_attention(const LatentAttention& p, void* workspace, cudaStream_t stream);
+cudaError_t read_attention_error(int* value);
 
 }  // namespace dsv4

@@ -375,8 +375,8 @@ int dsv4_sparse_latent_attention(const void* q, int64_t q_stride_token, int64_t 
 
 /*
  * Reads into *value_host, and clears, the error word the kernels of the current device keep:
- * bit 0 = a bounded wait inside the DSV4_VARIANT_BULK kernel ran out (its result is then
- * incomplete).  Synchronises the device.  0 after every healthy run.  No counterpart in the reference.
+ * bit 0 = a bounded wait inside the DSV4_VARIANT_BULK kernel ran out, bit 1 = one inside the latent attention (the
+ * result of that launch is then incomplete).  Synchronises the device.  0 after every healthy run.  No counterpart in the reference.
  */
 int dsv4_device_error(int32_t* value_host);
 
