@@ -20,6 +20,8 @@
 // Rows of work are few in decoding and of any length, so the blocks of all tiles are dealt out evenly: every CTA computes the same prefix sum
 // over the tiles' numbers of blocks and takes its share, which may begin and end inside a tile.  Pieces of a tile go to a workspace as
 // unnormalised sums and are joined, in a fixed order, by a second small kernel.
+#include <algorithm>
+
 #include "dsv4_common.cuh"
 #include "latent_attention.cuh"
 
@@ -75,20 +77,17 @@ __device__ __forceinline__ bool barrier_try(uint64_t* bar, uint32_t parity) {
                  : "memory");
     return done != 0;
 }
-// Bounded: false, and the CTA's other roles told to leave, where the phase does not complete within about a second.
-__device__ __noinline__ bool barrier_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort) {
-    const long long start = clock64();
-    for (uint32_t i = 0; i < (1u << 24); ++i) {
+// Bounded: false, and the CTA's other roles told to leave, where the phase does not complete within 2^22 tries, each of which the hardware
+// suspends for up to about a microsecond (a second or more in all; a phase takes a few microseconds).
+constexpr uint32_t kTries = 1u << 22;
+__device__ __forceinline__ bool barrier_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    for (uint32_t i = 0; i < kTries; ++i) {
         if (barrier_try(bar, parity)) return true;
         if (*abort) return false;
-        if (clock64() - start > 2000000000LL) break;
     }
     *abort = 1;
     atomicOr(&g_attention_error, 1);
     return false;
-}
-__device__ __forceinline__ bool barrier_wait(uint64_t* bar, uint32_t parity, int* abort) {
-    return barrier_try(bar, parity) || barrier_wait_long(bar, parity, abort);
 }
 // The same by a whole warp, with one answer.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* abort) {
@@ -105,6 +104,13 @@ __device__ __forceinline__ void multiply(uint32_t d, uint64_t a, uint64_t b, uin
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
                  "l"(b), "r"(kind), "r"(static_cast<uint32_t>(accumulate))
                  : "memory");
+}
+// One lane of a converged warp.  A branch on it, unlike one on a lane's number, lets the compiler keep descriptors in uniform registers: a
+// product of 64 x 64 x 16 is issued every 33 cycles (its rate) instead of every 45.
+__device__ __forceinline__ bool elected() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
 }
 #define DSV4_R8(v, i) "=f"(v[i]), "=f"(v[i + 1]), "=f"(v[i + 2]), "=f"(v[i + 3]), "=f"(v[i + 4]), "=f"(v[i + 5]), "=f"(v[i + 6]), "=f"(v[i + 7])
 #define DSV4_W8(v, i) "f"(v[i]), "f"(v[i + 1]), "f"(v[i + 2]), "f"(v[i + 3]), "f"(v[i + 4]), "f"(v[i + 5]), "f"(v[i + 6]), "f"(v[i + 7])
@@ -307,21 +313,21 @@ __device__ __forceinline__ void make_plan(const Tiles& p, Rest& rest) {
 
 // ---- the kernel -------------------------------------------------------------------------------------------------------------------
 
-// Two e4m3 bytes of `word` (the low ones, or the high ones) times a scale, as a bf16 pair.
+// Two e4m3 bytes of `word` (the low ones, or the high ones) times a power of two, given as a pair of equal bf16: the values are exact in bf16,
+// and their product is rounded once.
 template <int HIGH>
-__device__ __forceinline__ uint32_t two_values(uint32_t word, float scale) {
+__device__ __forceinline__ uint32_t two_values(uint32_t word, uint32_t scale) {
     uint32_t halves, out;
     const auto pair = static_cast<uint16_t>(HIGH ? word >> 16 : word);
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(halves) : "h"(pair));
     float lo, hi;
     asm("{.reg .f16 l, h; mov.b32 {l, h}, %2; cvt.f32.f16 %0, l; cvt.f32.f16 %1, h;}" : "=f"(lo), "=f"(hi) : "r"(halves));
-    out = pack_bf16x2(__fmul_rn(lo, scale), __fmul_rn(hi, scale));
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(out) : "r"(pack_bf16x2(lo, hi)), "r"(scale));
     return out;
 }
 
-__device__ __forceinline__ float power_of_code(uint32_t code) {
-    return code == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(code << 23);  // (255: infinity)
-}
+// 2^(code - 127) as a pair of bf16; 0: subnormal, 255: infinity.
+__device__ __forceinline__ uint32_t power_of_code(uint32_t code) { return (code == 0u ? 0x40u : code << 7) * 0x10001u; }
 
 // Whether one of a bf16 pair is infinite or NaN.
 __device__ __forceinline__ bool not_finite(uint32_t pair) { return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u; }
@@ -551,60 +557,56 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
         const uint32_t store_at = base + kOffsetKeys + (sub >> 2) * kChunkBytes + key_a * 128;
         const uint32_t unit = 2 * (sub & 3);
         const bool rotary = sub >= 12;
+        const int low_at = 16 * sub, high_at = rotary ? kNopeDim + 32 * (sub - 12) : 256 + 16 * sub, code_shift = 8 * (sub >> 2);
+        const int64_t codes_from = static_cast<int64_t>(p.a.block_size) * kTokenDataBytes;
         Held h;
-        uint32_t valid = 0;     // of the block whose values are held
-        // pages (or slots) of the block whose values are asked for next
-        const auto find = [&](const Walk& w, int block, int (&page)[4]) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int k = block * kBlockKeys + key_a + 2 * i;
-                page[i] = -1;
-                if (k < w.tile.keys) {
-                    if (p.a.indices) {
-                        page[i] = __ldg(p.a.indices + w.tile.token * p.a.indices_stride + k);
-                    } else {
-                        const int where = k < w.tile.first ? k : k - w.tile.first + w.tile.low;
-                        page[i] = __ldg(p.a.block_table + w.at.request * p.a.table_stride + fast_div(where, p.a.block_mul, p.a.block_shift));
-                    }
+        uint32_t valid = 0;  // of the block whose values are held
+        // Each lane looks up one of the warp's eight keys (lane % 8): its place in its block and its page, or its slot.
+        const auto find = [&](const Walk& w, int block, int& in_block) {
+            const int k = block * kBlockKeys + 8 * reader + (lane & 7);
+            int number = -1;
+            in_block = 0;
+            if (k < w.tile.keys) {
+                if (p.a.indices) {
+                    number = __ldg(p.a.indices + w.tile.token * p.a.indices_stride + k);
+                } else {
+                    const uint32_t where = k < w.tile.first ? k : k - w.tile.first + w.tile.low;
+                    const uint32_t page = fast_div(where, p.a.block_mul, p.a.block_shift);
+                    in_block = where - page * p.a.block_size;
+                    number = __ldg(p.a.block_table + w.at.request * p.a.table_stride + page);
                 }
             }
+            return number;
         };
         const uint8_t* data[4];
-        const auto ask_low = [&](const Walk& w, int block, const int (&page)[4]) {
-            uint32_t bits = 0;
+        // Asks for the first half's values and the scale codes.  Keys that do not exist are read from q instead, and zeroed when they arrive.
+        const auto ask_low = [&](int number, int in_block) {
+            if (p.a.indices) {
+                const uint32_t block = fast_div(static_cast<uint32_t>(max(number, 0)), p.a.block_mul, p.a.block_shift);
+                in_block = static_cast<uint32_t>(max(number, 0)) - block * p.a.block_size;
+                number = number < 0 ? -1 : static_cast<int>(block);
+            }
+            const bool there = number >= 0 && number < p.a.num_blocks;
+            const uint8_t* mine = there ? p.a.k_cache + number * p.a.block_stride + static_cast<int64_t>(in_block) * kTokenDataBytes : p.a.q;
+            const int64_t codes = there ? codes_from - static_cast<int64_t>(in_block) * (kTokenDataBytes - kScaleBytes) : 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int k = block * kBlockKeys + key_a + 2 * i;
-                uint32_t at = p.a.indices ? static_cast<uint32_t>(max(page[i], 0)) : k < w.tile.first ? k : k - w.tile.first + w.tile.low;
-                const uint32_t quotient = fast_div(at, p.a.block_mul, p.a.block_shift);
-                const uint32_t in_block = at - quotient * p.a.block_size;
-                const int number = p.a.indices ? static_cast<int>(quotient) : page[i];
-                const bool there = page[i] >= 0 && number < p.a.num_blocks;
-                data[i] = nullptr;
-                h.low[i] = make_uint4(0u, 0u, 0u, 0u), h.codes[i] = make_uint2(0u, 0u);
-                if (there) {
-                    const uint8_t* block_at = p.a.k_cache + number * p.a.block_stride;
-                    data[i] = block_at + static_cast<int64_t>(in_block) * kTokenDataBytes;
-                    h.low[i] = ld_stream16(data[i] + 16 * sub);
-                    h.codes[i] = __ldg(reinterpret_cast<const uint2*>(block_at + static_cast<int64_t>(p.a.block_size) * kTokenDataBytes + static_cast<int64_t>(in_block) * kScaleBytes));
-                    bits |= 1u << (2 * i + odd);
-                }
+                data[i] = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(mine), 2 * i + odd));
+                h.low[i] = ld_stream16(data[i] + low_at);
+                h.codes[i] = __ldg(reinterpret_cast<const uint2*>(data[i] + __shfl_sync(0xffffffffu, codes, 2 * i + odd)));
             }
-            return bits | __shfl_xor_sync(0xffffffffu, bits, 1);
+            return __ballot_sync(0xffffffffu, there) & 0xffu;
         };
         const auto ask_high = [&] {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                h.high[i] = h.rotary[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (data[i]) {
-                    const uint8_t* at = rotary ? data[i] + kNopeDim + 32 * (sub - 12) : data[i] + 256 + 16 * sub;
-                    h.high[i] = ld_stream16(at);
-                    if (rotary) h.rotary[i] = ld_stream16(at + 16);
-                }
+                h.high[i] = ld_stream16(data[i] + high_at);
+                if (rotary) h.rotary[i] = ld_stream16(data[i] + high_at + 16);
             }
         };
         // 16 e4m3 values to two 16-byte columns
-        const auto convert = [&](const uint4& v, float scale, uint4& a, uint4& b) {
+        const auto convert = [&](const uint4& v, uint32_t code_word, uint4& a, uint4& b) {
+            const uint32_t scale = power_of_code((code_word >> code_shift) & 0xffu);
             a = make_uint4(two_values<0>(v.x, scale), two_values<1>(v.x, scale), two_values<0>(v.y, scale), two_values<1>(v.y, scale));
             b = make_uint4(two_values<0>(v.z, scale), two_values<1>(v.z, scale), two_values<0>(v.w, scale), two_values<1>(v.w, scale));
         };
@@ -616,11 +618,11 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
         bool more = w.settle(p);
         while (more && w.begin == w.end) w.step(p), more = w.settle(p);
         int block = w.begin;
-        uint2 codes[4];
+        uint32_t codes[4];
         if (more) {
-            int page[4];
-            find(w, block, page);
-            valid = ask_low(w, block, page);
+            int in_block;
+            const int number = find(w, block, in_block);
+            valid = ask_low(number, in_block);
             ask_high();
         }
         for (int it = 0; more; ++it) {
@@ -634,36 +636,38 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                         (p.a.window > 0 && (k0 < w.tile.first || k0 - w.tile.first + w.tile.low <= w.tile.position + w.tile.count - 1 - p.a.window));
             }
             const uint32_t valid_now = valid;
-            int page[4];
             if (++block == w.end) {
                 do {
                     w.step(p), more = w.settle(p);
                 } while (more && w.begin == w.end);
                 block = w.begin;
             }
-            if (more) find(w, block, page);
+            int in_block = 0, number = -1;
+            if (more) number = find(w, block, in_block);
 
             if (it >= 2 && !warp_wait(&rest.kv_empty[slot], parity, abort)) break;
             uint32_t bad = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 uint4 a, b;
-                convert(h.low[i], power_of_code((h.codes[i].x >> (8 * (sub >> 2))) & 0xffu), a, b);
+                convert(h.low[i], h.codes[i].x, a, b);
+                if (valid_now != 0xffu && ((valid_now >> (2 * i + odd)) & 1u) == 0) a = b = make_uint4(0u, 0u, 0u, 0u);
                 store(slot, i, a, b);
                 if (mixed && (not_finite(a) || not_finite(b))) bad |= 1u << (2 * i + odd);
-                codes[i] = h.codes[i];
+                codes[i] = h.codes[i].y;
             }
             if (!mixed) {
                 fence_to_async();
                 __syncwarp();
                 if (lane == 0) barrier_arrive(&rest.kv_full[slot]);
             }
-            if (more) valid = ask_low(w, block, page);
+            if (more) valid = ask_low(number, in_block);
             if (it >= 2 && !warp_wait(&rest.kv_empty[slot + 1], parity, abort)) break;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 uint4 a = h.high[i], b = h.rotary[i];
-                if (!rotary) convert(h.high[i], power_of_code((codes[i].y >> (8 * (sub >> 2))) & 0xffu), a, b);
+                if (!rotary) convert(h.high[i], codes[i], a, b);
+                if (valid_now != 0xffu && ((valid_now >> (2 * i + odd)) & 1u) == 0) a = b = make_uint4(0u, 0u, 0u, 0u);
                 store(slot + 1, i, a, b);
                 if (mixed && (not_finite(a) || not_finite(b))) bad |= 1u << (2 * i + odd);
             }
@@ -690,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
         }
     } else if (warp == kIssuerWarp) {
         // ------------------------------------------------------------------------------------------------ products
-        if (lane == 0) {
+        if (elected()) {
             bool ok = true;
             int it = 0, tiles = 0;
             const auto product_o = [&](int i, bool first, int tile) {  // O += P V of block i
@@ -744,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
             if (ok && pending) product_o(it - 1, pending_first, pending_tile);
             // nothing of this CTA may be in flight when its memory is given back
             commit_to(&rest.drained);
-            for (uint32_t i = 0; i < (1u << 24) && !barrier_try(&rest.drained, 0); ++i) {}
+            for (uint32_t i = 0; i < kTries && !barrier_try(&rest.drained, 0); ++i) {}
         }
         __syncwarp();
     } else {
@@ -782,45 +786,66 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
     }
 }
 
-// Joins the pieces of tiles that were cut: the CTAs (c, .) those of the tile whose first piece CTA c had, a few rows each.
-constexpr int kJoinedRows = 4;
-__global__ void __launch_bounds__(128) join_pieces_kernel(const Launched<Tiles> p) {
+// Joins the pieces of tiles that were cut: CTA (c, row) one row of the tile whose first piece CTA c of the kernel above had.  Its warps take
+// the pieces in turn, all 512 sums of a piece's row in one go.
+constexpr int kJoinWarps = 8;
+__global__ void __launch_bounds__(kJoinWarps * 32) join_pieces_kernel(const Launched<Tiles> p) {
     begin_dependent_kernel();
-    const int4 head = p.pieces[2 * blockIdx.x + 1];
-    if (head.w == 0) return;
-    const float c = p.a.scale * kLog2e;
-    for (int r = 0; r < kJoinedRows; ++r) {
-        const int row = blockIdx.y * kJoinedRows + r;
-        if (row >= head.z) return;
-        float m = -INFINITY;
-        const auto for_pieces = [&](auto&& f) {
-            f(2 * blockIdx.x + 1);
-            for (unsigned cta = blockIdx.x + 1; cta < gridDim.x; ++cta) {
-                const int kind = p.pieces[2 * cta].w;
-                if (kind != 0) f(2 * cta);
-                if (kind == 2) break;
-            }
-        };
-        for_pieces([&](int slot) { m = fmaxf(m, p.rows[slot * kRows + row].x); });
-        float l = 0.0f;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for_pieces([&](int slot) {
-            const float2 s = p.rows[slot * kRows + row];
-            const float f = s.x == -INFINITY ? (s.y == 0.0f ? 0.0f : 1.0f) : exp2_approx((s.x - m) * c);
-            const float4 v = *reinterpret_cast<const float4*>(p.sums + (static_cast<int64_t>(slot) * kRows + row) * kHeadDim + 4 * threadIdx.x);
-            l = fmaf(s.y, f, l);
-            if (f != 0.0f) o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
-        });
-        const int token = head.x + (p.head_groups == 1 ? row / p.a.num_heads : 0), at = p.head_groups == 1 ? row % p.a.num_heads : head.y + row;
-        const bool some = l != 0.0f;
-        float total = l;
-        if (p.a.sink && some) total += exp2_approx(fmaf(__ldg(p.a.sink + at), kLog2e, -m * c));
-        const float inverse = some ? 1.0f / total : 0.0f;
-        uint8_t* out = p.a.out + token * p.a.out_stride_token + at * p.a.out_stride_head + 8 * threadIdx.x;
-        *reinterpret_cast<uint2*>(out) = some ? make_uint2(pack_bf16x2(o.x * inverse, o.y * inverse), pack_bf16x2(o.z * inverse, o.w * inverse)) : make_uint2(0u, 0u);
-        if (threadIdx.x == 0 && p.a.lse)
-            p.a.lse[token * p.a.lse_stride_token + at * p.a.lse_stride_head] = some ? (m * c + log2f(l)) * kLn2 : -INFINITY;
+    __shared__ float2 state[kMaxCtas];
+    __shared__ int slots[kMaxCtas], last_cta;
+    __shared__ float4 part[kJoinWarps][kHeadDim / 4];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.y, first = blockIdx.x;
+    const int4 head = p.pieces[2 * first + 1];
+    if (head.w == 0 || row >= head.z) return;
+    if (tid == 0) last_cta = kMaxCtas;
+    __syncthreads();
+    // piece i: that of CTA first + i, where it has one
+    const int cta = first + tid, slot = tid == 0 ? 2 * first + 1 : 2 * cta;
+    const int kind = cta < kMaxCtas ? p.pieces[slot].w : 0;
+    if (kind == 2) atomicMin(&last_cta, cta);
+    __syncthreads();
+    const int count = last_cta - first + 1;  // (the piece that ends the tile is always there)
+    if (tid < count && cta < kMaxCtas) {
+        slots[tid] = kind != 0 ? slot : -1;
+        state[tid] = kind != 0 ? p.rows[slot * kRows + row] : make_float2(-INFINITY, 0.0f);
     }
+    __syncthreads();
+    const float c = p.a.scale * kLog2e;
+    float m = -INFINITY, l = 0.0f;
+    for (int i = 0; i < count; ++i) m = fmaxf(m, state[i].x);
+    const auto factor = [&](float of) { return of == -INFINITY ? 0.0f : exp2_approx((of - m) * c); };
+    // (a sum that is NaN stays NaN, also that of a row without a finite maximum)
+    for (int i = 0; i < count; ++i) l += state[i].x == -INFINITY ? state[i].y : state[i].y * factor(state[i].x);
+    float4 o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int i = warp; i < count; i += kJoinWarps) {
+        if (slots[i] < 0) continue;
+        const float f = factor(state[i].x);
+        const float4* from = reinterpret_cast<const float4*>(p.sums + (static_cast<int64_t>(slots[i]) * kRows + row) * kHeadDim) + lane;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float4 v = __ldg(from + 32 * k);
+            o[k].x = fmaf(v.x, f, o[k].x), o[k].y = fmaf(v.y, f, o[k].y), o[k].z = fmaf(v.z, f, o[k].z), o[k].w = fmaf(v.w, f, o[k].w);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) part[warp][lane + 32 * k] = o[k];
+    __syncthreads();
+    const int token = head.x + (p.head_groups == 1 ? row / p.a.num_heads : 0), at = p.head_groups == 1 ? row % p.a.num_heads : head.y + row;
+    const bool some = l != 0.0f;
+    float total = l;
+    if (p.a.sink && some) total += exp2_approx(fmaf(__ldg(p.a.sink + at), kLog2e, -m * c));
+    const float inverse = some ? 1.0f / total : 0.0f;
+    float2 sum = make_float2(0.0f, 0.0f);
+    for (int w = 0; w < kJoinWarps; ++w) {
+        const float2 v = reinterpret_cast<const float2*>(part[w])[tid];
+        sum.x += v.x, sum.y += v.y;
+    }
+    *reinterpret_cast<uint32_t*>(p.a.out + token * p.a.out_stride_token + at * p.a.out_stride_head + 4 * tid) =
+        some ? pack_bf16x2(sum.x * inverse, sum.y * inverse) : 0u;
+    if (tid == 0 && p.a.lse) p.a.lse[token * p.a.lse_stride_token + at * p.a.lse_stride_head] = some ? (m * c + log2f(l)) * kLn2 : -INFINITY;
 }
 
 constexpr size_t kSumBytes = sizeof(float) * 2 * kMaxCtas * kRows * kHeadDim, kRowBytes2 = sizeof(float2) * 2 * kMaxCtas * kRows;
@@ -834,6 +859,9 @@ cudaError_t launch_latent_attention(const LatentAttention& a, void* workspace, c
     p.a = a;
     p.tokens_per_tile = a.indices || a.num_heads >= kRows ? 1 : kRows / a.num_heads;
     p.head_groups = (a.num_heads + kRows - 1) / kRows;
+    // Where no tile can have enough keys to be cut, there are no pieces to join.
+    const int64_t most_keys = a.indices ? a.topk : a.window > 0 ? static_cast<int64_t>(a.window) + a.first + p.tokens_per_tile : a.capacity;
+    const bool may_split = std::min<int64_t>(most_keys, a.indices ? a.topk : a.capacity) > (kLeastSplit - 1) * kBlockKeys;
     auto* at = static_cast<uint8_t*>(workspace);
     p.sums = reinterpret_cast<float*>(at), p.rows = reinterpret_cast<float2*>(at + kSumBytes), p.pieces = reinterpret_cast<int4*>(at + kSumBytes + kRowBytes2);
     // Set for the current device each time: cheaper than to remember for which ones it was.
@@ -842,7 +870,8 @@ cudaError_t launch_latent_attention(const LatentAttention& a, void* workspace, c
     rc = launch_dependent_cluster(latent_attention_kernel, dim3(kMaxCtas), dim3(kThreads), 1, kSharedBytes, stream, p);
     if (rc != cudaSuccess) return rc;
     count_launch();
-    rc = launch_dependent(join_pieces_kernel, dim3(kMaxCtas, kRows / kJoinedRows), dim3(128), stream, p);
+    if (!may_split) return cudaGetLastError();
+    rc = launch_dependent(join_pieces_kernel, dim3(kMaxCtas, kRows), dim3(kJoinWarps * 32), stream, p);
     if (rc != cudaSuccess) return rc;
     count_launch();
     return cudaGetLastError();
