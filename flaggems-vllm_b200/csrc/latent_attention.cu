@@ -32,8 +32,12 @@ __device__ int g_attention_error = 0;
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kRows = 64, kBlockKeys = 64;
-constexpr int kSoftmaxWarps = 4, kReaderWarps = 8, kIssuerWarp = 12, kThreads = 14 * 32;
+constexpr int kRows = 64, kBlockKeys = 48, kStages = 3;
+constexpr int kSoftmaxWarps = 4, kReaderWarps = 12, kIssuerWarp = kSoftmaxWarps + kReaderWarps, kQueryWarps = 3;
+constexpr int kThreads = 32 * (kIssuerWarp + 1 + kQueryWarps), kWarpKeys = kBlockKeys / kReaderWarps;
+// Registers a thread: 96 at launch (65536 / 640 threads, in steps of 8), then other shares of the same sum.
+constexpr int kSoftmaxRegisters = 128, kReaderRegisters = 80, kOtherRegisters = 96;
+static_assert(kThreads == 640 && kWarpKeys == 4 && 4 * kSoftmaxRegisters + 12 * kReaderRegisters + 4 * kOtherRegisters <= 20 * 96, "");
 constexpr float kMostGrowth = 8.0f;  // log2 of the factor that a row's maximum may have grown by before O is corrected
 constexpr int kMaxCtas = 148;        // a B200's SMs: one CTA on each (its shared memory allows no second)
 // Cuts between CTAs are moved to a tile's border where a piece would be short of this many blocks, and fewer CTAs take part where each
@@ -42,23 +46,24 @@ constexpr int kLeastPiece = 2, kLeastShare = 4, kLeastSplit = 8;
 
 // ---- shared memory -----------------------------------------------------------------------------------------------------------
 
-constexpr int kChunkBytes = kRows * 128;           // 64 rows of 64 dimensions: eight 8-row, 128-byte swizzle atoms
-constexpr int kHalfBytes = 4 * kChunkBytes;        // 64 keys x 256 dimensions
-constexpr int kQueryBytes = 8 * kChunkBytes;
-constexpr int kOffsetKeys = kQueryBytes, kOffsetP = kOffsetKeys + 4 * kHalfBytes, kOffsetRest = kOffsetP + 2 * kChunkBytes;
+constexpr int kQueryChunk = kRows * 128, kKeyChunk = kBlockKeys * 128;  // rows of 64 dimensions: 8-row, 128-byte swizzle atoms
+constexpr int kQueryBytes = 8 * kQueryChunk, kKeyBytes = 8 * kKeyChunk;   // 64 KiB and 48 KiB
+constexpr int kOffsetKeys = kQueryBytes, kOffsetP = kOffsetKeys + kStages * kKeyBytes, kOffsetRest = kOffsetP + 2 * kQueryChunk;
 
 struct Cut {
     int request, token, group, block;
 };
 struct Rest {
-    uint64_t kv_full[4], kv_empty[4], s_full[2], p_full[2], pv_done[2], q_full, q_empty, o_empty, drained;
-    uint64_t sums[16];
-    uint8_t valid[2][8], bad[2][8];  // a bit per key of a block: it exists, it has a value that is not finite
+    uint64_t kv_full[kStages], kv_empty[kStages], s_full[2], p_full[2], pv_done[2], q_full, q_empty, o_empty, drained;
+    uint64_t sums[kThreads / 32];
+    alignas(4) uint8_t valid[kStages][kReaderWarps], bad[kStages][kReaderWarps];  // a bit per key of a reader warp's four: it exists, it has a value that is not finite
     Cut from, to;
+    alignas(8) uint32_t walks[kReaderWarps][20];  // of each reader warp (struct Walk): read where it is needed instead of held in registers
     uint32_t tmem;
     int abort;
 };
-constexpr int kSharedBytes = kOffsetRest + static_cast<int>(sizeof(Rest)) + 1024;  // (the base is moved up to a multiple of 1024)
+constexpr int kSharedBytes = kOffsetRest + static_cast<int>(sizeof(Rest));
+static_assert(kSharedBytes <= 232448, "227 KiB a CTA");
 
 // ---- PTX ----------------------------------------------------------------------------------------------------------------------
 
@@ -93,6 +98,7 @@ __device__ __forceinline__ bool barrier_wait(uint64_t* bar, uint32_t parity, vol
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* abort) {
     return __all_sync(0xffffffffu, barrier_wait(bar, parity, abort));
 }
+// Between a thread's ordinary writes of shared memory and the products that read them.  It waits for the thread's loads that are under way, too.
 __device__ __forceinline__ void fence_to_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void fence_tmem_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_tmem_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -116,12 +122,13 @@ __device__ __forceinline__ bool elected() {
 #define DSV4_W8(v, i) "f"(v[i]), "f"(v[i + 1]), "f"(v[i + 2]), "f"(v[i + 3]), "f"(v[i + 4]), "f"(v[i + 5]), "f"(v[i + 6]), "f"(v[i + 7])
 #define DSV4_LIST32                                                                                                                       \
     "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}"
-// 16 lanes x 64 columns: lane l of the warp gets, of columns 8j + 2(l % 4) + {0, 1}, row l / 4 in v[4j], v[4j + 1] and row l / 4 + 8 in the
+// 16 lanes x 48 columns: lane l of the warp gets, of columns 8j + 2(l % 4) + {0, 1}, row l / 4 in v[4j], v[4j + 1] and row l / 4 + 8 in the
 // next two.
-__device__ __forceinline__ void load_scores(float (&v)[32], uint32_t at) {
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x8.b32 " DSV4_LIST32 ", [%32];"
-                 : DSV4_R8(v, 0), DSV4_R8(v, 8), DSV4_R8(v, 16), DSV4_R8(v, 24)
+__device__ __forceinline__ void load_scores(float (&v)[24], uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : DSV4_R8(v, 0), DSV4_R8(v, 8)
                  : "r"(at));
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : DSV4_R8(v, 16) : "r"(at + 32));
 }
 // 32 lanes x 32 columns, one lane a thread.
 __device__ __forceinline__ void load_columns(float (&v)[32], uint32_t at) {
@@ -133,6 +140,9 @@ __device__ __forceinline__ void load_columns(float (&v)[32], uint32_t at) {
 #define DSV4_U8(v, i) "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]), "+f"(v[i + 6]), "+f"(v[i + 7])
 __device__ __forceinline__ void wait_tmem_loads(float (&v)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" : DSV4_U8(v, 0), DSV4_U8(v, 8), DSV4_U8(v, 16), DSV4_U8(v, 24)::"memory");
+}
+__device__ __forceinline__ void wait_tmem_loads(float (&v)[24]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : DSV4_U8(v, 0), DSV4_U8(v, 8), DSV4_U8(v, 16)::"memory");
 }
 __device__ __forceinline__ void store_columns(const float (&v)[32], uint32_t at) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], " DSV4_LIST32 ";" ::DSV4_W8(v, 0), DSV4_W8(v, 8), DSV4_W8(v, 16), DSV4_W8(v, 24),
@@ -175,6 +185,13 @@ struct Tiles {
 // The keys of a tile as one list: `first` first tokens, then the positions from `low` on.
 struct Tile {
     int token, count, head, rows, position, first, low, keys, blocks;
+    // Whether some rows of the tile see a key of the block that others do not.
+    __device__ __forceinline__ bool mixed(const Tiles& p, int block) const {
+        if (count == 1) return false;
+        const int k0 = block * kBlockKeys, k1 = min(k0 + kBlockKeys, keys) - 1;
+        const int oldest = k0 < first ? k0 : k0 - first + low, newest = k1 < first ? k1 : k1 - first + low;
+        return newest > position || (p.a.window > 0 && (k0 < first || oldest <= position + count - 1 - p.a.window));
+    }
 };
 
 __device__ __forceinline__ Tile tile_at(const Tiles& p, int request, int token, int group) {
@@ -212,7 +229,8 @@ __device__ __forceinline__ int request_of(const Tiles& p, int& token) {
 
 // A CTA's share: pieces of tiles, in order.
 struct Walk {
-    Cut at, to;
+    Cut at;
+    const Cut* end_of_share;  // in shared memory
     Tile tile;
     int begin, end;  // blocks of the tile
     __device__ __forceinline__ void step(const Tiles& p) {
@@ -228,6 +246,7 @@ struct Walk {
     // Makes `tile`, `begin` and `end` those of the piece at `at`, or of the first one behind it that is none of nothing; false at the end.
     __device__ __forceinline__ bool settle(const Tiles& p) {
         for (;;) {
+            const volatile Cut& to = *end_of_share;
             if (at.token >= p.a.num_tokens || at.token > to.token || (at.token == to.token && at.group > to.group)) return false;
             const bool last = at.token == to.token && at.group == to.group;
             if (last && to.block == 0) return false;
@@ -333,23 +352,31 @@ __device__ __forceinline__ uint32_t power_of_code(uint32_t code) { return (code 
 __device__ __forceinline__ bool not_finite(uint32_t pair) { return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u; }
 __device__ __forceinline__ bool not_finite(const uint4& v) { return not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w); }
 
-// What a reader lane holds of its four keys of a block: 16 bytes of each half's values (32 of the rotary ones), scale codes.
-struct Held {
-    uint4 low[4], high[4], rotary[4];
-    uint2 codes[4];
-};
+// Twelve bytes of four bits each as one number.
+__device__ __forceinline__ uint64_t key_bits(const uint32_t* v) {
+    const auto four = [](uint32_t x) {
+        x = (x | (x >> 4)) & 0x00ff00ffu;
+        return (x | (x >> 8)) & 0xffffu;
+    };
+    return static_cast<uint64_t>(four(v[0]) | (four(v[1]) << 16)) | (static_cast<uint64_t>(four(v[2])) << 32);
+}
+
+template <int COUNT, bool MORE>
+__device__ __forceinline__ void set_registers() {
+    if (MORE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(COUNT));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(COUNT));
+}
 
 __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Launched<Tiles> p) {
-    extern __shared__ uint8_t raw[];
-    uint8_t* shared = raw + ((1024u - (shared_address(raw) & 1023u)) & 1023u);
+    extern __shared__ __align__(1024) uint8_t shared[];
     Rest& rest = *reinterpret_cast<Rest*>(shared + kOffsetRest);
     const uint32_t base = shared_address(shared);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 4; ++i) barrier_init(&rest.kv_full[i], kReaderWarps), barrier_init(&rest.kv_empty[i], 1);
+        for (int i = 0; i < kStages; ++i) barrier_init(&rest.kv_full[i], kReaderWarps), barrier_init(&rest.kv_empty[i], 1);
         for (int i = 0; i < 2; ++i) barrier_init(&rest.s_full[i], 1), barrier_init(&rest.p_full[i], kSoftmaxWarps), barrier_init(&rest.pv_done[i], 1);
-        barrier_init(&rest.q_full, 1), barrier_init(&rest.q_empty, 1), barrier_init(&rest.o_empty, kSoftmaxWarps), barrier_init(&rest.drained, 1);
+        barrier_init(&rest.q_full, kQueryWarps), barrier_init(&rest.q_empty, 1), barrier_init(&rest.o_empty, kSoftmaxWarps), barrier_init(&rest.drained, 1);
         rest.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_to_async();
@@ -366,14 +393,16 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
     const uint32_t tmem = rest.tmem, tmem_scores = tmem + 256;
     int* abort = &rest.abort;
     Walk w;
-    w.at = rest.from, w.to = rest.to;
+    w.at = rest.from, w.end_of_share = &rest.to;
 
     if (warp < kSoftmaxWarps) {
         // ------------------------------------------------------------------------------------------------ softmax, outputs
+        set_registers<kSoftmaxRegisters, true>();
         const float c = p.a.scale * kLog2e;
         const int row_a = 16 * warp + (lane >> 2), quad = 2 * (lane & 3);
         const uint32_t lanes = static_cast<uint32_t>(32 * warp) << 16;
-        int it = 0;
+        int it = 0, stage = 0;  // blocks so far, and that number modulo kStages
+        uint32_t stage_phase = 0;
         bool ok = true;
         const int slot_of_head = 2 * blockIdx.x + 1, slot_of_rest = 2 * blockIdx.x;
         if (threadIdx.x < 2 && p.pieces) p.pieces[2 * blockIdx.x + threadIdx.x] = make_int4(0, 0, 0, 0);
@@ -382,46 +411,42 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
             const Tile& t = w.tile;
             float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
             // positions of this thread's two rows
-            const int last = t.position + t.count - 1;
             int position[2] = {t.position, t.position};
             if (t.count > 1) position[0] += row_a / p.a.num_heads, position[1] += (row_a + 8) / p.a.num_heads;
             for (int block = w.begin; block < w.end; ++block, ++it) {
                 const int buffer = it & 1;
                 const uint32_t parity = (it >> 1) & 1;
-                if (!warp_wait(&rest.s_full[buffer], parity, abort) || !warp_wait(&rest.kv_full[2 * buffer + 1], parity, abort)) {
+                if (!warp_wait(&rest.s_full[buffer], parity, abort) || !warp_wait(&rest.kv_full[stage], stage_phase, abort)) {
                     ok = false;
                     break;
                 }
                 fence_tmem_after();
-                float s[32];
+                float s[24];
                 load_scores(s, tmem_scores + 64 * buffer + lanes);
-                const uint64_t valid = *reinterpret_cast<const uint64_t*>(rest.valid[buffer]);
+                const uint32_t* exist = reinterpret_cast<const uint32_t*>(rest.valid[stage]);
+                const bool all = (exist[0] & exist[1] & exist[2]) == 0x0f0f0f0fu;
+                const bool mixed = t.mixed(p, block);
                 const int k0 = block * kBlockKeys;
-                bool mixed = false;
-                if (t.count > 1) {
-                    const int k1 = min(k0 + kBlockKeys, t.keys) - 1;
-                    const int newest = k1 < t.first ? k1 : k1 - t.first + t.low;
-                    mixed = newest > t.position || (p.a.window > 0 && (k0 < t.first || k0 - t.first + t.low <= last - p.a.window));
-                }
                 wait_tmem_loads(s);
                 if (mixed) {
-                    const uint64_t bad = *reinterpret_cast<const uint64_t*>(rest.bad[buffer]);
+                    const uint64_t valid = key_bits(exist), bad = key_bits(reinterpret_cast<const uint32_t*>(rest.bad[stage]));
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
+                    for (int i = 0; i < 24; ++i) {
                         const int k = 8 * (i >> 2) + quad + (i & 1);
                         const int at = k0 + k, where = at < t.first ? at : at - t.first + t.low;
                         const int mine = position[(i >> 1) & 1];
                         const bool seen = ((valid >> k) & 1) != 0 && where <= mine && (p.a.window <= 0 || mine - where < p.a.window || where < p.a.first);
                         s[i] = !seen ? -INFINITY : ((bad >> k) & 1) != 0 ? NAN : s[i];
                     }
-                } else if (valid != ~0ull) {
+                } else if (!all) {
+                    const uint64_t valid = key_bits(exist);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
+                    for (int i = 0; i < 24; ++i)
                         if (((valid >> (8 * (i >> 2) + quad + (i & 1))) & 1) == 0) s[i] = -INFINITY;
                 }
                 float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < 32; ++i) top[(i >> 1) & 1] = fmaxf(top[(i >> 1) & 1], s[i]);
+                for (int i = 0; i < 24; ++i) top[(i >> 1) & 1] = fmaxf(top[(i >> 1) & 1], s[i]);
                 float factor[2] = {1.0f, 1.0f};
                 bool grown = false;
 #pragma unroll
@@ -460,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                 }
                 const float mc[2] = {m[0] == -INFINITY ? 0.0f : m[0] * c, m[1] == -INFINITY ? 0.0f : m[1] * c};
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
+                for (int i = 0; i < 24; ++i) {
                     s[i] = exp2_approx(fmaf(s[i], c, -mc[(i >> 1) & 1]));
                     l[(i >> 1) & 1] += s[i];
                 }
@@ -469,9 +494,9 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                     ok = false;
                     break;
                 }
-                const uint32_t to = base + kOffsetP + buffer * kChunkBytes + row_a * 128 + 2 * quad;
+                const uint32_t to = base + kOffsetP + buffer * kQueryChunk + row_a * 128 + 2 * quad;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
+                for (int j = 0; j < kBlockKeys / 8; ++j) {
                     const uint32_t unit = (j ^ (row_a & 7)) << 4;  // (row_a + 8 has the same low bits)
                     store_shared4(to + unit, pack_bf16x2(s[4 * j], s[4 * j + 1]));
                     store_shared4(to + 8 * 128 + unit, pack_bf16x2(s[4 * j + 2], s[4 * j + 3]));
@@ -480,6 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                 fence_tmem_before();
                 __syncwarp();
                 if (lane == 0) barrier_arrive(&rest.p_full[buffer]);
+                if (++stage == kStages) stage = 0, stage_phase ^= 1;
             }
             if (!ok) break;
 #pragma unroll
@@ -550,59 +576,58 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
         }
     } else if (warp < kIssuerWarp) {
         // ------------------------------------------------------------------------------------------------ readers
+        set_registers<kReaderRegisters, false>();
+        // A warp has four keys of each block.  It asks for its values of the next block when it has handed over this one's, not before: the fence
+        // and the arrival wait for a warp's loads that are under way.
         const int reader = warp - kSoftmaxWarps, sub = lane >> 1, odd = lane & 1;
-        // keys 8 * reader + 2 i + odd of a block; of each, dimensions 16 sub .. of both halves (rotary ones: sub 12-15 of the second).  Two
-        // neighbouring keys and four subs, which are what eight lanes store at once, hit all eight 16-byte columns of the swizzle.
-        const int key_a = 8 * reader + odd;
-        const uint32_t store_at = base + kOffsetKeys + (sub >> 2) * kChunkBytes + key_a * 128;
-        const uint32_t unit = 2 * (sub & 3);
-        const bool rotary = sub >= 12;
-        const int low_at = 16 * sub, high_at = rotary ? kNopeDim + 32 * (sub - 12) : 256 + 16 * sub, code_shift = 8 * (sub >> 2);
-        const int64_t codes_from = static_cast<int64_t>(p.a.block_size) * kTokenDataBytes;
-        Held h;
-        uint32_t valid = 0;  // of the block whose values are held
-        // Each lane looks up one of the warp's eight keys (lane % 8): its place in its block and its page, or its slot.
-        const auto find = [&](const Walk& w, int block, int& in_block) {
-            const int k = block * kBlockKeys + 8 * reader + (lane & 7);
-            int number = -1;
-            in_block = 0;
-            if (k < w.tile.keys) {
+        // Keys 4 * reader + 2 i + odd of a block; of each, dimensions 16 sub .. of the first half, the same of the second where they are e4m3
+        // (sub 0-11), and four rotary ones.  Two neighbouring keys and four subs, which are what eight lanes store at once, hit all eight 16-byte
+        // columns of the swizzle.
+        const int key_a = kWarpKeys * reader + odd;
+        const uint32_t store_row = base + kOffsetKeys + key_a * 128, unit = 2 * (sub & 3);
+        const bool coded = sub < 12;
+        const int code_shift = 8 * (sub >> 2);
+        uint4 low[2], high[2];
+        uint2 rotary[2], codes[2];
+        // Each lane looks up one of the warp's keys (lane % 4): its place in its block and its page, or its slot.
+        int number = -1, in_block = 0, block, end;
+        Walk& walk = reinterpret_cast<Walk&>(rest.walks[reader]);
+        static_assert(sizeof(Walk) <= sizeof(rest.walks[0]) && alignof(Walk) <= 8, "");
+        const auto find = [&] {
+            const int k = block * kBlockKeys + kWarpKeys * reader + (lane & 3);
+            number = -1, in_block = 0;
+            if (k < walk.tile.keys) {
                 if (p.a.indices) {
-                    number = __ldg(p.a.indices + w.tile.token * p.a.indices_stride + k);
+                    number = __ldg(p.a.indices + walk.tile.token * p.a.indices_stride + k);
                 } else {
-                    const uint32_t where = k < w.tile.first ? k : k - w.tile.first + w.tile.low;
+                    const uint32_t where = k < walk.tile.first ? k : k - walk.tile.first + walk.tile.low;
                     const uint32_t page = fast_div(where, p.a.block_mul, p.a.block_shift);
                     in_block = where - page * p.a.block_size;
-                    number = __ldg(p.a.block_table + w.at.request * p.a.table_stride + page);
+                    number = __ldg(p.a.block_table + walk.at.request * p.a.table_stride + page);
                 }
             }
-            return number;
         };
-        const uint8_t* data[4];
-        // Asks for the first half's values and the scale codes.  Keys that do not exist are read from q instead, and zeroed when they arrive.
-        const auto ask_low = [&](int number, int in_block) {
+        // Asks for the values and scale codes of the keys that were looked up; a bit for each that exists.  Those that do not are read from q
+        // instead, and zeroed when they arrive.
+        const auto ask = [&] {
             if (p.a.indices) {
-                const uint32_t block = fast_div(static_cast<uint32_t>(max(number, 0)), p.a.block_mul, p.a.block_shift);
-                in_block = static_cast<uint32_t>(max(number, 0)) - block * p.a.block_size;
-                number = number < 0 ? -1 : static_cast<int>(block);
+                const uint32_t of = static_cast<uint32_t>(max(number, 0)), page = fast_div(of, p.a.block_mul, p.a.block_shift);
+                in_block = of - page * p.a.block_size;
+                number = number < 0 ? -1 : static_cast<int>(page);
             }
             const bool there = number >= 0 && number < p.a.num_blocks;
             const uint8_t* mine = there ? p.a.k_cache + number * p.a.block_stride + static_cast<int64_t>(in_block) * kTokenDataBytes : p.a.q;
-            const int64_t codes = there ? codes_from - static_cast<int64_t>(in_block) * (kTokenDataBytes - kScaleBytes) : 0;
+            const int64_t codes_on =
+                there ? static_cast<int64_t>(p.a.block_size) * kTokenDataBytes - static_cast<int64_t>(in_block) * (kTokenDataBytes - kScaleBytes) : 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                data[i] = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(mine), 2 * i + odd));
-                h.low[i] = ld_stream16(data[i] + low_at);
-                h.codes[i] = __ldg(reinterpret_cast<const uint2*>(data[i] + __shfl_sync(0xffffffffu, codes, 2 * i + odd)));
+            for (int i = 0; i < 2; ++i) {
+                const uint8_t* data = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(mine), 2 * i + odd));
+                codes[i] = __ldg(reinterpret_cast<const uint2*>(data + __shfl_sync(0xffffffffu, codes_on, 2 * i + odd)));
+                low[i] = ld_stream16(data + 16 * sub);
+                if (coded) high[i] = ld_stream16(data + 256 + 16 * sub);
+                rotary[i] = __ldg(reinterpret_cast<const uint2*>(data + kNopeDim + 8 * sub));
             }
-            return __ballot_sync(0xffffffffu, there) & 0xffu;
-        };
-        const auto ask_high = [&] {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                h.high[i] = ld_stream16(data[i] + high_at);
-                if (rotary) h.rotary[i] = ld_stream16(data[i] + high_at + 16);
-            }
+            return __ballot_sync(0xffffffffu, there) & 0xfu;
         };
         // 16 e4m3 values to two 16-byte columns
         const auto convert = [&](const uint4& v, uint32_t code_word, uint4& a, uint4& b) {
@@ -610,106 +635,100 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
             a = make_uint4(two_values<0>(v.x, scale), two_values<1>(v.x, scale), two_values<0>(v.y, scale), two_values<1>(v.y, scale));
             b = make_uint4(two_values<0>(v.z, scale), two_values<1>(v.z, scale), two_values<0>(v.w, scale), two_values<1>(v.w, scale));
         };
-        const auto store = [&](uint32_t half, int i, const uint4& a, const uint4& b) {
-            const uint32_t at = store_at + half * kHalfBytes + 2 * i * 128, twist = (key_a + 2 * i) & 7;
+        int stage = 0;
+        const auto store = [&](int half, int i, const uint4& a, const uint4& b) {
+            const uint32_t at = store_row + stage * kKeyBytes + (4 * half + (sub >> 2)) * kKeyChunk + 2 * i * 128, twist = (key_a + 2 * i) & 7;
             store_shared16(at + ((unit ^ twist) << 4), a);
             store_shared16(at + (((unit + 1) ^ twist) << 4), b);
         };
-        bool more = w.settle(p);
-        while (more && w.begin == w.end) w.step(p), more = w.settle(p);
-        int block = w.begin;
-        uint32_t codes[4];
-        if (more) {
-            int in_block;
-            const int number = find(w, block, in_block);
-            valid = ask_low(number, in_block);
-            ask_high();
-        }
-        for (int it = 0; more; ++it) {
-            const uint32_t slot = 2 * (it & 1), parity = ((it >> 1) - 1) & 1;
-            // this block's mask, then on to the next block
-            bool mixed = false;
-            if (w.tile.count > 1) {
-                const int k0 = block * kBlockKeys, k1 = min(k0 + kBlockKeys, w.tile.keys) - 1;
-                const int newest = k1 < w.tile.first ? k1 : k1 - w.tile.first + w.tile.low;
-                mixed = newest > w.tile.position ||
-                        (p.a.window > 0 && (k0 < w.tile.first || k0 - w.tile.first + w.tile.low <= w.tile.position + w.tile.count - 1 - p.a.window));
-            }
-            const uint32_t valid_now = valid;
-            if (++block == w.end) {
-                do {
-                    w.step(p), more = w.settle(p);
-                } while (more && w.begin == w.end);
-                block = w.begin;
-            }
-            int in_block = 0, number = -1;
-            if (more) number = find(w, block, in_block);
+        const auto store_rotary = [&](int i, uint2 v) {
+            const uint32_t at = store_row + stage * kKeyBytes + 7 * kKeyChunk + 2 * i * 128 + (((sub >> 1) ^ ((key_a + 2 * i) & 7)) << 4) + 8 * (sub & 1);
+            asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(at), "r"(v.x), "r"(v.y) : "memory");
+        };
+        bool more = true;
+        const auto next_tile = [&](bool first) {
+            Walk next = first ? w : walk;
+            do {
+                if (!first) next.step(p);
+                first = false;
+                more = next.settle(p);
+            } while (more && next.begin == next.end);
+            block = next.begin, end = next.end;
+            __syncwarp();
+            if (lane == 0) walk = next;
+            __syncwarp();
+        };
+        next_tile(true);
+        if (more) find();
+        uint32_t phase = 1;  // of kv_empty[stage]: the first round finds it "complete"
+        while (more) {
+            const uint32_t valid = ask();
+            const bool mixed = walk.tile.mixed(p, block);
+            if (++block == end) next_tile(false);
+            if (more) find();
 
-            if (it >= 2 && !warp_wait(&rest.kv_empty[slot], parity, abort)) break;
+            if (!warp_wait(&rest.kv_empty[stage], phase, abort)) break;
+            const bool all = valid == 0xfu;
             uint32_t bad = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 2; ++i) {
+                const bool absent = !all && ((valid >> (2 * i + odd)) & 1u) == 0;
                 uint4 a, b;
-                convert(h.low[i], h.codes[i].x, a, b);
-                if (valid_now != 0xffu && ((valid_now >> (2 * i + odd)) & 1u) == 0) a = b = make_uint4(0u, 0u, 0u, 0u);
-                store(slot, i, a, b);
+                convert(low[i], codes[i].x, a, b);
+                if (absent) a = b = make_uint4(0u, 0u, 0u, 0u);
+                store(0, i, a, b);
                 if (mixed && (not_finite(a) || not_finite(b))) bad |= 1u << (2 * i + odd);
-                codes[i] = h.codes[i].y;
+                if (coded) {
+                    convert(high[i], codes[i].y, a, b);
+                    if (absent) a = b = make_uint4(0u, 0u, 0u, 0u);
+                    store(1, i, a, b);
+                    if (mixed && (not_finite(a) || not_finite(b))) bad |= 1u << (2 * i + odd);
+                }
+                if (absent) rotary[i] = make_uint2(0u, 0u);
+                store_rotary(i, rotary[i]);
+                if (mixed && (not_finite(rotary[i].x) || not_finite(rotary[i].y))) bad |= 1u << (2 * i + odd);
             }
-            if (!mixed) {
-                fence_to_async();
-                __syncwarp();
-                if (lane == 0) barrier_arrive(&rest.kv_full[slot]);
-            }
-            if (more) valid = ask_low(number, in_block);
-            if (it >= 2 && !warp_wait(&rest.kv_empty[slot + 1], parity, abort)) break;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint4 a = h.high[i], b = h.rotary[i];
-                if (!rotary) convert(h.high[i], codes[i], a, b);
-                if (valid_now != 0xffu && ((valid_now >> (2 * i + odd)) & 1u) == 0) a = b = make_uint4(0u, 0u, 0u, 0u);
-                store(slot + 1, i, a, b);
-                if (mixed && (not_finite(a) || not_finite(b))) bad |= 1u << (2 * i + odd);
-            }
-            if (more) ask_high();
             if (mixed) {
                 // Keys that some rows of the tile do not see: those with a value that is not finite are stored as zeros, which the rows that do
                 // not see them multiply by zero; the others get NaN as their score.
                 bad = __reduce_or_sync(0xffffffffu, bad);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < 2; ++i) {
                     if ((bad >> (2 * i + odd)) & 1u) {
                         const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-                        store(slot, i, zero, zero), store(slot + 1, i, zero, zero);
+                        store(0, i, zero, zero);
+                        if (coded) store(1, i, zero, zero);
+                        store_rotary(i, make_uint2(0u, 0u));
                     }
                 }
             }
-            if (lane == 0) rest.valid[it & 1][reader] = static_cast<uint8_t>(valid_now), rest.bad[it & 1][reader] = static_cast<uint8_t>(bad);
+            if (lane == 0) rest.valid[stage][reader] = static_cast<uint8_t>(valid), rest.bad[stage][reader] = static_cast<uint8_t>(bad);
             fence_to_async();
             __syncwarp();
-            if (lane == 0) {
-                if (mixed) barrier_arrive(&rest.kv_full[slot]);
-                barrier_arrive(&rest.kv_full[slot + 1]);
-            }
+            if (lane == 0) barrier_arrive(&rest.kv_full[stage]);
+            if (++stage == kStages) stage = 0, phase ^= 1;
         }
     } else if (warp == kIssuerWarp) {
         // ------------------------------------------------------------------------------------------------ products
+        set_registers<kOtherRegisters, false>();
         if (elected()) {
             bool ok = true;
-            int it = 0, tiles = 0;
-            const auto product_o = [&](int i, bool first, int tile) {  // O += P V of block i
+            int it = 0, tiles = 0, stage = 0, stage_before = 0;
+            uint32_t phase = 0;
+            const auto product_o = [&](int i, bool first, int tile) {  // O += P V of block i, the one before the last
                 const int buffer = i & 1;
                 if (!barrier_wait(&rest.p_full[buffer], (i >> 1) & 1, abort)) return false;
                 if (first && tile > 0 && !barrier_wait(&rest.o_empty, (tile - 1) & 1, abort)) return false;
                 fence_tmem_after();
-                for (int half = 0; half < 2; ++half) {
-                    const uint64_t a = operand(base + kOffsetP + buffer * kChunkBytes, 16);
-                    const uint64_t b = operand(base + kOffsetKeys + (2 * buffer + half) * kHalfBytes, kChunkBytes);
+                const uint64_t a = operand(base + kOffsetP + buffer * kQueryChunk, 16);
+                const uint64_t b = operand(base + kOffsetKeys + stage_before * kKeyBytes, kKeyChunk);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        multiply(tmem + (static_cast<uint32_t>(16 * half) << 16), a + k * (32 >> 4), b + k * (2048 >> 4), kKindO, !first || k > 0);
-                    commit_to(&rest.kv_empty[2 * buffer + half]);
-                }
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int k = 0; k < kBlockKeys / 16; ++k)
+                        multiply(tmem + (static_cast<uint32_t>(16 * half) << 16), a + k * (32 >> 4), b + (half * 4 * kKeyChunk + k * 2048) / 16, kKindO,
+                                 !first || k > 0);
+                commit_to(&rest.kv_empty[stage_before]);
                 commit_to(&rest.pv_done[buffer]);
                 return true;
             };
@@ -723,25 +742,23 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                 if (!barrier_wait(&rest.q_full, tiles & 1, abort)) break;
                 for (int block = w.begin; block < w.end; ++block, ++it) {
                     const int buffer = it & 1;
-                    for (int half = 0; half < 2 && ok; ++half) {
-                        ok = barrier_wait(&rest.kv_full[2 * buffer + half], (it >> 1) & 1, abort);
-                        if (!ok) break;
-                        fence_tmem_after();
-#pragma unroll
-                        for (int chunk = 0; chunk < 4; ++chunk) {
-                            const uint64_t a = operand(base + (4 * half + chunk) * kChunkBytes, 16);
-                            const uint64_t b = operand(base + kOffsetKeys + (2 * buffer + half) * kHalfBytes + chunk * kChunkBytes, 16);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                multiply(tmem_scores + 64 * buffer, a + k * (32 >> 4), b + k * (32 >> 4), kKindS, half + chunk + k > 0);
-                        }
-                    }
+                    ok = barrier_wait(&rest.kv_full[stage], phase, abort);
                     if (!ok) break;
+                    fence_tmem_after();
+                    const uint64_t a = operand(base, 16), b = operand(base + kOffsetKeys + stage * kKeyBytes, 16);
+#pragma unroll
+                    for (int chunk = 0; chunk < 8; ++chunk)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            multiply(tmem_scores + 64 * buffer, a + (chunk * kQueryChunk + 32 * k) / 16, b + (chunk * kKeyChunk + 32 * k) / 16, kKindS,
+                                     chunk + k > 0);
                     commit_to(&rest.s_full[buffer]);
                     if (block + 1 == w.end) commit_to(&rest.q_empty);
                     if (pending) ok = product_o(it - 1, pending_first, pending_tile);
                     if (!ok) break;
                     pending = true, pending_first = block == w.begin, pending_tile = tiles;
+                    stage_before = stage;
+                    if (++stage == kStages) stage = 0, phase ^= 1;
                 }
                 ++tiles;
             }
@@ -753,13 +770,14 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
         __syncwarp();
     } else {
         // ------------------------------------------------------------------------------------------------ queries
+        set_registers<kOtherRegisters, false>();
         int tiles = 0;
         for (; w.settle(p); w.step(p)) {
             if (w.begin == w.end) continue;
             const Tile& t = w.tile;
             if (tiles > 0 && !warp_wait(&rest.q_empty, (tiles - 1) & 1, abort)) break;
             // a row is 64 pieces of 16 bytes: two passes of the warp
-            for (int row = 0; row < kRows; ++row) {
+            for (int row = warp - kIssuerWarp - 1; row < kRows; row += kQueryWarps) {
                 const int token = t.token + (t.count > 1 ? row / p.a.num_heads : 0);
                 const int head = t.count > 1 ? row % p.a.num_heads : t.head + row;
                 const bool live = row < t.rows;
@@ -767,7 +785,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int piece = lane + 32 * i;
-                    const uint32_t to = base + (piece >> 3) * kChunkBytes + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
+                    const uint32_t to = base + (piece >> 3) * kQueryChunk + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(live ? from + 16 * piece : from), "r"(live ? 16 : 0) : "memory");
                 }
             }
