@@ -64,6 +64,7 @@ struct Rest {
 };
 constexpr int kSharedBytes = kOffsetRest + static_cast<int>(sizeof(Rest));
 static_assert(kSharedBytes <= 232448, "227 KiB a CTA");
+constexpr int kScratchInts = kOffsetRest / 4;  // all that is not in use while the plan is made
 
 // ---- PTX ----------------------------------------------------------------------------------------------------------------------
 
@@ -174,8 +175,13 @@ constexpr uint32_t kKindS = kind_of(kBlockKeys, false), kKindO = kind_of(256, tr
 
 // ---- tiles and their order ------------------------------------------------------------------------------------------------------
 
+// The lists of starts and lengths, in global memory or, while the plan is made, copied to shared memory.
+struct Lists {
+    const int32_t *starts, *lens;
+};
 struct Tiles {
     LatentAttention a;
+    Lists lists;
     int32_t tokens_per_tile, heads_per_tile, head_groups;
     float* sums;      // workspace: [2 * kMaxCtas][64][512] unnormalised outputs,
     float2* rows;     // [2 * kMaxCtas][64] their maximum and sum,
@@ -194,17 +200,17 @@ struct Tile {
     }
 };
 
-__device__ __forceinline__ Tile tile_at(const Tiles& p, int request, int token, int group) {
+__device__ __forceinline__ Tile tile_at(const Tiles& p, const Lists& lists, int request, int token, int group) {
     Tile t;
     t.token = token, t.head = group * kRows;
     t.position = t.first = t.low = 0;
     if (p.a.indices) {
         t.count = 1;
-        t.keys = min(max(__ldg(p.a.lens + token), 0), p.a.topk);
+        t.keys = min(max(lists.lens[token], 0), p.a.topk);
     } else {
-        const int end = min(__ldg(p.a.query_start_loc + request + 1), p.a.num_tokens);
+        const int end = min(lists.starts[request + 1], p.a.num_tokens);
         t.count = min(p.tokens_per_tile, end - token);
-        t.position = max(__ldg(p.a.seq_lens + request), 0) - end + token;
+        t.position = max(lists.lens[request], 0) - end + token;
         t.low = p.a.window > 0 && t.position >= p.a.window ? t.position - p.a.window + 1 : 0;
         t.first = min(min(t.low, p.a.first), p.a.capacity);
         t.keys = max(0, min(t.position + t.count, p.a.capacity) - t.low) + t.first;
@@ -215,13 +221,13 @@ __device__ __forceinline__ Tile tile_at(const Tiles& p, int request, int token, 
 }
 
 // Request of the first token at or behind `token` that belongs to one (num_reqs if none does), and that token.
-__device__ __forceinline__ int request_of(const Tiles& p, int& token) {
+__device__ __forceinline__ int request_of(const Tiles& p, const Lists& lists, int& token) {
     if (p.a.indices) return 0;
-    token = max(token, __ldg(p.a.query_start_loc));
+    token = max(token, lists.starts[0]);
     int low = 0, high = p.a.num_reqs;  // the first request that ends behind the token
     while (low < high) {
         const int mid = (low + high) >> 1;
-        if (__ldg(p.a.query_start_loc + mid + 1) > token) high = mid;
+        if (lists.starts[mid + 1] > token) high = mid;
         else low = mid + 1;
     }
     return low;
@@ -238,7 +244,7 @@ struct Walk {
             at.group = 0;
             at.token += tile.count;
             if (!p.a.indices)
-                while (at.request < p.a.num_reqs && __ldg(p.a.query_start_loc + at.request + 1) <= at.token) ++at.request;
+                while (at.request < p.a.num_reqs && __ldg(p.lists.starts + at.request + 1) <= at.token) ++at.request;
             if (at.request >= p.a.num_reqs && !p.a.indices) at.token = p.a.num_tokens;
         }
         at.block = 0;
@@ -250,7 +256,7 @@ struct Walk {
             if (at.token >= p.a.num_tokens || at.token > to.token || (at.token == to.token && at.group > to.group)) return false;
             const bool last = at.token == to.token && at.group == to.group;
             if (last && to.block == 0) return false;
-            tile = tile_at(p, at.request, at.token, at.group);
+            tile = tile_at(p, p.lists, at.request, at.token, at.group);
             begin = at.block, end = last ? min(to.block, tile.blocks) : tile.blocks;
             if (begin < end || tile.blocks == 0) return true;
             step(p);
@@ -261,26 +267,35 @@ struct Walk {
 
 // Every CTA's share has the same number of blocks, a tile counting one more for its own cost.  All threads take part; thread-uniform results in
 // rest.from and rest.to.
-__device__ __forceinline__ void make_plan(const Tiles& p, Rest& rest) {
+__device__ __forceinline__ void make_plan(const Tiles& p, Rest& rest, int32_t* scratch) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // The starts and lengths of all requests (lengths of all tokens) are read at once, where they fit, instead of in a chain of dependent loads.
+    Lists lists = p.lists;
+    const int starts = p.a.indices ? 0 : p.a.num_reqs + 1, lens = p.a.indices ? p.a.num_tokens : p.a.num_reqs;
+    if (starts + lens <= kScratchInts) {
+        for (int i = tid; i < starts; i += kThreads) scratch[i] = __ldg(p.lists.starts + i);
+        for (int i = tid; i < lens; i += kThreads) scratch[starts + i] = __ldg(p.lists.lens + i);
+        lists.starts = scratch, lists.lens = scratch + starts;
+        __syncthreads();
+    }
     const int each = (p.a.num_tokens + kThreads - 1) / kThreads;
     const int begin = min(tid * each, p.a.num_tokens), end = min(begin + each, p.a.num_tokens);
     // f(request, token, blocks) for the tiles' first tokens in [begin, end)
     const auto for_tiles = [&](auto&& f) {
-        int token = begin, request = begin < end ? request_of(p, token) : 0;
+        int token = begin, request = begin < end ? request_of(p, lists, token) : 0;
         while (token < end) {
             if (!p.a.indices) {
-                while (request < p.a.num_reqs && __ldg(p.a.query_start_loc + request + 1) <= token) ++request;
+                while (request < p.a.num_reqs && lists.starts[request + 1] <= token) ++request;
                 if (request >= p.a.num_reqs) break;
-                const int start = __ldg(p.a.query_start_loc + request);
+                const int start = lists.starts[request];
                 const int behind = (token - start) % p.tokens_per_tile;
                 if (behind != 0) {
                     token += p.tokens_per_tile - behind;
-                    token = min(token, __ldg(p.a.query_start_loc + request + 1));
+                    token = min(token, lists.starts[request + 1]);
                     continue;
                 }
             }
-            const Tile t = tile_at(p, request, token, 0);
+            const Tile t = tile_at(p, lists, request, token, 0);
             if (f(request, token, t.blocks)) break;
             token += t.count;
         }
@@ -386,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     begin_dependent_kernel();
-    make_plan(p, rest);
+    make_plan(p, rest, reinterpret_cast<int32_t*>(shared));
     fence_tmem_before();
     __syncthreads();
     fence_tmem_after();
@@ -804,66 +819,109 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
     }
 }
 
-// Joins the pieces of tiles that were cut: CTA (c, row) one row of the tile whose first piece CTA c of the kernel above had.  Its warps take
-// the pieces in turn, all 512 sums of a piece's row in one go.
-constexpr int kJoinWarps = 8;
+// Joins the pieces of tiles that were cut, which the CTAs of the kernel above have left in order: the head of a tile in one CTA, the rest in the
+// CTAs behind it.  A CTA takes rows in turn, one warp a row, or 4 or 16 warps that share out the pieces of a row where there are many.  (A CTA for
+// every row that might need it took 15 to 28 us, most of it for those that did not.)
+constexpr int kJoinWarps = 16, kJoinCtas = 2 * kMaxCtas;
 __global__ void __launch_bounds__(kJoinWarps * 32) join_pieces_kernel(const Launched<Tiles> p) {
     begin_dependent_kernel();
-    __shared__ float2 state[kMaxCtas];
-    __shared__ int slots[kMaxCtas], last_cta;
+    __shared__ int4 pieces[2 * kMaxCtas];
+    __shared__ int heads[kMaxCtas], ends[kMaxCtas], counts[2][kJoinWarps], most;
     __shared__ float4 part[kJoinWarps][kHeadDim / 4];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.y, first = blockIdx.x;
-    const int4 head = p.pieces[2 * first + 1];
-    if (head.w == 0 || row >= head.z) return;
-    if (tid == 0) last_cta = kMaxCtas;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    for (int i = tid; i < 2 * kMaxCtas; i += kJoinWarps * 32) pieces[i] = p.pieces[i];
+    if (tid == 0) most = 0;
     __syncthreads();
-    // piece i: that of CTA first + i, where it has one
-    const int cta = first + tid, slot = tid == 0 ? 2 * first + 1 : 2 * cta;
-    const int kind = cta < kMaxCtas ? p.pieces[slot].w : 0;
-    if (kind == 2) atomicMin(&last_cta, cta);
+    // The tiles: the CTA with the head and the one with the end of each, which follow one another.
+    const bool head = tid < kMaxCtas && pieces[2 * tid + 1].w != 0, end = tid < kMaxCtas && pieces[2 * tid].w == 2;
+    const uint32_t head_votes = __ballot_sync(0xffffffffu, head), end_votes = __ballot_sync(0xffffffffu, end);
+    if (lane == 0) counts[0][warp] = __popc(head_votes), counts[1][warp] = __popc(end_votes);
     __syncthreads();
-    const int count = last_cta - first + 1;  // (the piece that ends the tile is always there)
-    if (tid < count && cta < kMaxCtas) {
-        slots[tid] = kind != 0 ? slot : -1;
-        state[tid] = kind != 0 ? p.rows[slot * kRows + row] : make_float2(-INFINITY, 0.0f);
+    int tiles = 0, heads_before = __popc(head_votes & ((1u << lane) - 1u)), ends_before = __popc(end_votes & ((1u << lane) - 1u));
+    for (int w = 0; w < kJoinWarps; ++w) {
+        if (w < warp) heads_before += counts[0][w], ends_before += counts[1][w];
+        tiles += counts[0][w];
     }
+    if (head) heads[heads_before] = tid;
+    if (end) ends[ends_before] = tid;
     __syncthreads();
+    if (tid < tiles) atomicMax(&most, ends[tid] - heads[tid] + 1);
+    __syncthreads();
+    const int each = most <= 4 ? 1 : most <= 16 ? 4 : 16, rows = kJoinWarps / each, turn = warp % each;  // warps for a row, rows at once
     const float c = p.a.scale * kLog2e;
-    float m = -INFINITY, l = 0.0f;
-    for (int i = 0; i < count; ++i) m = fmaxf(m, state[i].x);
-    const auto factor = [&](float of) { return of == -INFINITY ? 0.0f : exp2_approx((of - m) * c); };
-    // (a sum that is NaN stays NaN, also that of a row without a finite maximum)
-    for (int i = 0; i < count; ++i) l += state[i].x == -INFINITY ? state[i].y : state[i].y * factor(state[i].x);
-    float4 o[4];
+    constexpr int kPerLane = (kMaxCtas + 31) / 32;
+    for (int item = blockIdx.x; item < tiles * (kRows / rows); item += kJoinCtas) {
+        const int tile = item / (kRows / rows), row = item % (kRows / rows) * rows + warp / each;
+        const int first = heads[tile], count = ends[tile] - first + 1;
+        const int4 of = pieces[2 * first + 1];
+        const bool live = row < of.z;
+        // piece i: that of CTA first + i, where it has one
+        const auto slot_of = [&](int i) { return i == 0 ? 2 * first + 1 : pieces[2 * (first + i)].w != 0 ? 2 * (first + i) : -1; };
+        float2 state[kPerLane];
+        float m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int i = warp; i < count; i += kJoinWarps) {
-        if (slots[i] < 0) continue;
-        const float f = factor(state[i].x);
-        const float4* from = reinterpret_cast<const float4*>(p.sums + (static_cast<int64_t>(slots[i]) * kRows + row) * kHeadDim) + lane;
+        for (int k = 0; k < kPerLane; ++k) {
+            const int i = lane + 32 * k, slot = live && i < count ? slot_of(i) : -1;
+            state[k] = slot >= 0 ? p.rows[slot * kRows + row] : make_float2(-INFINITY, 0.0f);
+            m = fmaxf(m, state[k].x);
+        }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float4 v = __ldg(from + 32 * k);
-            o[k].x = fmaf(v.x, f, o[k].x), o[k].y = fmaf(v.y, f, o[k].y), o[k].z = fmaf(v.z, f, o[k].z), o[k].w = fmaf(v.w, f, o[k].w);
+        for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+#pragma unroll
+        for (int k = 0; k < kPerLane; ++k) {
+            const bool some = state[k].x != -INFINITY;
+            state[k].x = some ? exp2_approx((state[k].x - m) * c) : 0.0f;
+            l += some ? state[k].y * state[k].x : state[k].y;  // (a sum that is NaN stays NaN, also that of a row without a finite maximum)
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+        float4 o[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < kPerLane; ++k) {
+#pragma unroll 2
+            for (int i = 32 * k + turn; i < min(count, 32 * k + 32); i += each) {
+                const float f = __shfl_sync(0xffffffffu, state[k].x, i & 31);
+                const int slot = slot_of(i);
+                if (slot < 0 || !live) continue;
+                const float4* from = reinterpret_cast<const float4*>(p.sums + (static_cast<int64_t>(slot) * kRows + row) * kHeadDim) + lane;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float4 v = __ldg(from + 32 * q);
+                    o[q].x = fmaf(v.x, f, o[q].x), o[q].y = fmaf(v.y, f, o[q].y), o[q].z = fmaf(v.z, f, o[q].z), o[q].w = fmaf(v.w, f, o[q].w);
+                }
+            }
+        }
+        const int token = of.x + (p.head_groups == 1 ? row / p.a.num_heads : 0), at = p.head_groups == 1 ? row % p.a.num_heads : of.y + row;
+        const bool some = l != 0.0f;
+        float total = l;
+        if (live && p.a.sink && some) total += exp2_approx(fmaf(__ldg(p.a.sink + at), kLog2e, -m * c));
+        const float inverse = some ? 1.0f / total : 0.0f;
+        const auto store = [&](int dim, const float4& v) {  // of four dimensions
+            *reinterpret_cast<uint2*>(p.a.out + token * p.a.out_stride_token + at * p.a.out_stride_head + 8 * dim) =
+                some ? make_uint2(pack_bf16x2(v.x * inverse, v.y * inverse), pack_bf16x2(v.z * inverse, v.w * inverse)) : make_uint2(0u, 0u);
+        };
+        if (live && turn == 0 && lane == 0 && p.a.lse)
+            p.a.lse[token * p.a.lse_stride_token + at * p.a.lse_stride_head] = some ? (m * c + log2f(l)) * kLn2 : -INFINITY;
+        if (each == 1) {
+            if (live)
+                for (int q = 0; q < 4; ++q) store(lane + 32 * q, o[q]);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) part[warp][lane + 32 * q] = o[q];
+            __syncthreads();
+            for (int dim = 32 * turn + lane; live && dim < kHeadDim / 4; dim += 32 * each) {
+                float4 sum = part[warp - turn][dim];
+                for (int w = 1; w < each; ++w) {
+                    const float4 v = part[warp - turn + w][dim];
+                    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+                }
+                store(dim, sum);
+            }
+            __syncthreads();
         }
     }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) part[warp][lane + 32 * k] = o[k];
-    __syncthreads();
-    const int token = head.x + (p.head_groups == 1 ? row / p.a.num_heads : 0), at = p.head_groups == 1 ? row % p.a.num_heads : head.y + row;
-    const bool some = l != 0.0f;
-    float total = l;
-    if (p.a.sink && some) total += exp2_approx(fmaf(__ldg(p.a.sink + at), kLog2e, -m * c));
-    const float inverse = some ? 1.0f / total : 0.0f;
-    float2 sum = make_float2(0.0f, 0.0f);
-    for (int w = 0; w < kJoinWarps; ++w) {
-        const float2 v = reinterpret_cast<const float2*>(part[w])[tid];
-        sum.x += v.x, sum.y += v.y;
-    }
-    *reinterpret_cast<uint32_t*>(p.a.out + token * p.a.out_stride_token + at * p.a.out_stride_head + 4 * tid) =
-        some ? pack_bf16x2(sum.x * inverse, sum.y * inverse) : 0u;
-    if (tid == 0 && p.a.lse) p.a.lse[token * p.a.lse_stride_token + at * p.a.lse_stride_head] = some ? (m * c + log2f(l)) * kLn2 : -INFINITY;
 }
 
 constexpr size_t kSumBytes = sizeof(float) * 2 * kMaxCtas * kRows * kHeadDim, kRowBytes2 = sizeof(float2) * 2 * kMaxCtas * kRows;
@@ -875,6 +933,7 @@ size_t latent_attention_workspace(int64_t, int64_t) { return kSumBytes + kRowByt
 cudaError_t launch_latent_attention(const LatentAttention& a, void* workspace, cudaStream_t stream) {
     Tiles p{};
     p.a = a;
+    p.lists = Lists{a.query_start_loc, a.indices ? a.lens : a.seq_lens};
     p.tokens_per_tile = a.indices || a.num_heads >= kRows ? 1 : kRows / a.num_heads;
     p.head_groups = (a.num_heads + kRows - 1) / kRows;
     // Where no tile can have enough keys to be cut, there are no pieces to join.
@@ -889,7 +948,7 @@ cudaError_t launch_latent_attention(const LatentAttention& a, void* workspace, c
     if (rc != cudaSuccess) return rc;
     count_launch();
     if (!may_split) return cudaGetLastError();
-    rc = launch_dependent(join_pieces_kernel, dim3(kMaxCtas, kRows), dim3(kJoinWarps * 32), stream, p);
+    rc = launch_dependent(join_pieces_kernel, dim3(kJoinCtas), dim3(kJoinWarps * 32), stream, p);
     if (rc != cudaSuccess) return rc;
     count_launch();
     return cudaGetLastError();
