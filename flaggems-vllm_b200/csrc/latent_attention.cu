@@ -33,11 +33,12 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kRows = 64, kBlockKeys = 48, kStages = 3;
-constexpr int kSoftmaxWarps = 4, kReaderWarps = 12, kIssuerWarp = kSoftmaxWarps + kReaderWarps, kQueryWarps = 3;
-constexpr int kThreads = 32 * (kIssuerWarp + 1 + kQueryWarps), kWarpKeys = kBlockKeys / kReaderWarps;
+constexpr int kSoftmaxWarps = 4, kReaderWarps = 12, kIssuerWarp = kSoftmaxWarps + kReaderWarps, kLookupWarp = kIssuerWarp + 1, kQueryWarps = 2;
+constexpr int kThreads = 32 * (kLookupWarp + 1 + kQueryWarps), kWarpKeys = kBlockKeys / kReaderWarps;
 // Registers a thread: 96 at launch (65536 / 640 threads, in steps of 8), then other shares of the same sum.
 constexpr int kSoftmaxRegisters = 128, kReaderRegisters = 80, kOtherRegisters = 96;
 static_assert(kThreads == 640 && kWarpKeys == 4 && 4 * kSoftmaxRegisters + 12 * kReaderRegisters + 4 * kOtherRegisters <= 20 * 96, "");
+constexpr uint64_t kAllKeys = (1ull << kBlockKeys) - 1;
 constexpr float kMostGrowth = 8.0f;  // log2 of the factor that a row's maximum may have grown by before O is corrected
 constexpr int kMaxCtas = 148;        // a B200's SMs: one CTA on each (its shared memory allows no second)
 // Cuts between CTAs are moved to a tile's border where a piece would be short of this many blocks, and fewer CTAs take part where each
@@ -54,11 +55,16 @@ struct Cut {
     int request, token, group, block;
 };
 struct Rest {
-    uint64_t kv_full[kStages], kv_empty[kStages], s_full[2], p_full[2], pv_done[2], q_full, q_empty, o_empty, drained;
+    uint64_t kv_full[kStages], kv_empty[kStages], s_full[2], p_full[2], pv_done[2], look_full[2], look_empty[2], q_full, q_empty, o_empty, drained;
     uint64_t sums[kThreads / 32];
-    alignas(4) uint8_t valid[kStages][kReaderWarps], bad[kStages][kReaderWarps];  // a bit per key of a reader warp's four: it exists, it has a value that is not finite
+    uint64_t valid[kStages];                        // a bit per key of a block: it exists,
+    alignas(4) uint8_t bad[kStages][kReaderWarps];  // it has a value that is not finite: four keys a reader warp (mixed blocks only)
+    // What the look-up warp tells the readers of the next two blocks: where the values and the scale codes of every key are, which exist (bit 63:
+    // there is no such block), and whether the block is mixed.
+    alignas(16) ulonglong2 keys[2][kBlockKeys];
+    uint64_t exist[2];
+    uint32_t mixed[2];
     Cut from, to;
-    alignas(8) uint32_t walks[kReaderWarps][20];  // of each reader warp (struct Walk): read where it is needed instead of held in registers
     uint32_t tmem;
     int abort;
 };
@@ -75,11 +81,12 @@ __device__ __forceinline__ void barrier_init(uint64_t* bar, uint32_t count) {
 __device__ __forceinline__ void barrier_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_address(bar)) : "memory");
 }
+constexpr uint32_t kTryNs = 2000;  // how long the hardware may suspend the thread in one try
 __device__ __forceinline__ bool barrier_try(uint64_t* bar, uint32_t parity) {
     uint32_t done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                  : "=r"(done)
-                 : "r"(shared_address(bar)), "r"(parity)
+                 : "r"(shared_address(bar)), "r"(parity), "r"(kTryNs)
                  : "memory");
     return done != 0;
 }
@@ -391,6 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) barrier_init(&rest.kv_full[i], kReaderWarps), barrier_init(&rest.kv_empty[i], 1);
         for (int i = 0; i < 2; ++i) barrier_init(&rest.s_full[i], 1), barrier_init(&rest.p_full[i], kSoftmaxWarps), barrier_init(&rest.pv_done[i], 1);
+        for (int i = 0; i < 2; ++i) barrier_init(&rest.look_full[i], 1), barrier_init(&rest.look_empty[i], kReaderWarps);
         barrier_init(&rest.q_full, kQueryWarps), barrier_init(&rest.q_empty, 1), barrier_init(&rest.o_empty, kSoftmaxWarps), barrier_init(&rest.drained, 1);
         rest.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -438,13 +446,12 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                 fence_tmem_after();
                 float s[24];
                 load_scores(s, tmem_scores + 64 * buffer + lanes);
-                const uint32_t* exist = reinterpret_cast<const uint32_t*>(rest.valid[stage]);
-                const bool all = (exist[0] & exist[1] & exist[2]) == 0x0f0f0f0fu;
+                const uint64_t valid = rest.valid[stage];
                 const bool mixed = t.mixed(p, block);
                 const int k0 = block * kBlockKeys;
                 wait_tmem_loads(s);
                 if (mixed) {
-                    const uint64_t valid = key_bits(exist), bad = key_bits(reinterpret_cast<const uint32_t*>(rest.bad[stage]));
+                    const uint64_t bad = key_bits(reinterpret_cast<const uint32_t*>(rest.bad[stage]));
 #pragma unroll
                     for (int i = 0; i < 24; ++i) {
                         const int k = 8 * (i >> 2) + quad + (i & 1);
@@ -453,8 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                         const bool seen = ((valid >> k) & 1) != 0 && where <= mine && (p.a.window <= 0 || mine - where < p.a.window || where < p.a.first);
                         s[i] = !seen ? -INFINITY : ((bad >> k) & 1) != 0 ? NAN : s[i];
                     }
-                } else if (!all) {
-                    const uint64_t valid = key_bits(exist);
+                } else if (valid != kAllKeys) {
 #pragma unroll
                     for (int i = 0; i < 24; ++i)
                         if (((valid >> (8 * (i >> 2) + quad + (i & 1))) & 1) == 0) s[i] = -INFINITY;
@@ -462,41 +468,47 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                 float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                 for (int i = 0; i < 24; ++i) top[(i >> 1) & 1] = fmaxf(top[(i >> 1) & 1], s[i]);
-                float factor[2] = {1.0f, 1.0f};
+                // The common case is that no row's maximum has grown by so much that it matters: every lane sees that of its own columns.
                 bool grown = false;
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-                    if (m[r] == -INFINITY) {
-                        m[r] = top[r];  // (nothing but zeros so far)
-                    } else if ((top[r] - m[r]) * c > kMostGrowth) {
-                        factor[r] = exp2_approx((m[r] - top[r]) * c);
-                        l[r] *= factor[r];
-                        m[r] = top[r];
-                        grown = true;
-                    }
-                }
+                for (int r = 0; r < 2; ++r) grown |= m[r] == -INFINITY ? top[r] != -INFINITY : (top[r] - m[r]) * c > kMostGrowth;
                 if (__any_sync(0xffffffffu, grown)) {
-                    // O has been written up to the block before this one
-                    if (!warp_wait(&rest.pv_done[buffer ^ 1], ((it - 1) >> 1) & 1, abort)) {
-                        ok = false;
-                        break;
-                    }
-                    fence_tmem_after();
-                    const int from = (lane & 7) << 2;
-                    const float fa = __shfl_sync(0xffffffffu, factor[0], from), fb = __shfl_sync(0xffffffffu, factor[1], from);
-                    const float f = (lane & 8) ? fb : fa;
-#pragma unroll 1
-                    for (int at = 0; at < 256; at += 32) {
-                        float o[32];
-                        load_columns(o, tmem + at + lanes);
-                        wait_tmem_loads(o);
+                    float factor[2] = {1.0f, 1.0f};
+                    bool correct = false;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] *= f;
-                        store_columns(o, tmem + at + lanes);
+                    for (int r = 0; r < 2; ++r) {
+                        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+                        if (m[r] == -INFINITY) {
+                            m[r] = top[r];  // (O is zero so far)
+                        } else if (top[r] > m[r]) {
+                            factor[r] = exp2_approx((m[r] - top[r]) * c);
+                            l[r] *= factor[r];
+                            m[r] = top[r];
+                            correct = true;
+                        }
                     }
-                    wait_tmem_stores();
+                    if (__any_sync(0xffffffffu, correct)) {
+                        // O has been written up to the block before this one
+                        if (!warp_wait(&rest.pv_done[buffer ^ 1], ((it - 1) >> 1) & 1, abort)) {
+                            ok = false;
+                            break;
+                        }
+                        fence_tmem_after();
+                        const int from = (lane & 7) << 2;
+                        const float fa = __shfl_sync(0xffffffffu, factor[0], from), fb = __shfl_sync(0xffffffffu, factor[1], from);
+                        const float f = (lane & 8) ? fb : fa;
+#pragma unroll 1
+                        for (int at = 0; at < 256; at += 32) {
+                            float o[32];
+                            load_columns(o, tmem + at + lanes);
+                            wait_tmem_loads(o);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] *= f;
+                            store_columns(o, tmem + at + lanes);
+                        }
+                        wait_tmem_stores();
+                    }
                 }
                 const float mc[2] = {m[0] == -INFINITY ? 0.0f : m[0] * c, m[1] == -INFINITY ? 0.0f : m[1] * c};
 #pragma unroll
@@ -601,49 +613,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
         const int key_a = kWarpKeys * reader + odd;
         const uint32_t store_row = base + kOffsetKeys + key_a * 128, unit = 2 * (sub & 3);
         const bool coded = sub < 12;
+        const int rotary_sub = sub ^ (8 * odd);  // (the two keys' halves, so that their stores use different banks)
         const int code_shift = 8 * (sub >> 2);
-        uint4 low[2], high[2];
-        uint2 rotary[2], codes[2];
-        // Each lane looks up one of the warp's keys (lane % 4): its place in its block and its page, or its slot.
-        int number = -1, in_block = 0, block, end;
-        Walk& walk = reinterpret_cast<Walk&>(rest.walks[reader]);
-        static_assert(sizeof(Walk) <= sizeof(rest.walks[0]) && alignof(Walk) <= 8, "");
-        const auto find = [&] {
-            const int k = block * kBlockKeys + kWarpKeys * reader + (lane & 3);
-            number = -1, in_block = 0;
-            if (k < walk.tile.keys) {
-                if (p.a.indices) {
-                    number = __ldg(p.a.indices + walk.tile.token * p.a.indices_stride + k);
-                } else {
-                    const uint32_t where = k < walk.tile.first ? k : k - walk.tile.first + walk.tile.low;
-                    const uint32_t page = fast_div(where, p.a.block_mul, p.a.block_shift);
-                    in_block = where - page * p.a.block_size;
-                    number = __ldg(p.a.block_table + walk.at.request * p.a.table_stride + page);
-                }
-            }
-        };
-        // Asks for the values and scale codes of the keys that were looked up; a bit for each that exists.  Those that do not are read from q
-        // instead, and zeroed when they arrive.
-        const auto ask = [&] {
-            if (p.a.indices) {
-                const uint32_t of = static_cast<uint32_t>(max(number, 0)), page = fast_div(of, p.a.block_mul, p.a.block_shift);
-                in_block = of - page * p.a.block_size;
-                number = number < 0 ? -1 : static_cast<int>(page);
-            }
-            const bool there = number >= 0 && number < p.a.num_blocks;
-            const uint8_t* mine = there ? p.a.k_cache + number * p.a.block_stride + static_cast<int64_t>(in_block) * kTokenDataBytes : p.a.q;
-            const int64_t codes_on =
-                there ? static_cast<int64_t>(p.a.block_size) * kTokenDataBytes - static_cast<int64_t>(in_block) * (kTokenDataBytes - kScaleBytes) : 0;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint8_t* data = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(mine), 2 * i + odd));
-                codes[i] = __ldg(reinterpret_cast<const uint2*>(data + __shfl_sync(0xffffffffu, codes_on, 2 * i + odd)));
-                low[i] = ld_stream16(data + 16 * sub);
-                if (coded) high[i] = ld_stream16(data + 256 + 16 * sub);
-                rotary[i] = __ldg(reinterpret_cast<const uint2*>(data + kNopeDim + 8 * sub));
-            }
-            return __ballot_sync(0xffffffffu, there) & 0xfu;
-        };
         // 16 e4m3 values to two 16-byte columns
         const auto convert = [&](const uint4& v, uint32_t code_word, uint4& a, uint4& b) {
             const uint32_t scale = power_of_code((code_word >> code_shift) & 0xffu);
@@ -657,31 +628,32 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
             store_shared16(at + (((unit + 1) ^ twist) << 4), b);
         };
         const auto store_rotary = [&](int i, uint2 v) {
-            const uint32_t at = store_row + stage * kKeyBytes + 7 * kKeyChunk + 2 * i * 128 + (((sub >> 1) ^ ((key_a + 2 * i) & 7)) << 4) + 8 * (sub & 1);
+            const uint32_t at = store_row + stage * kKeyBytes + 7 * kKeyChunk + 2 * i * 128 + (((rotary_sub >> 1) ^ ((key_a + 2 * i) & 7)) << 4) + 8 * (sub & 1);
             asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(at), "r"(v.x), "r"(v.y) : "memory");
         };
-        bool more = true;
-        const auto next_tile = [&](bool first) {
-            Walk next = first ? w : walk;
-            do {
-                if (!first) next.step(p);
-                first = false;
-                more = next.settle(p);
-            } while (more && next.begin == next.end);
-            block = next.begin, end = next.end;
-            __syncwarp();
-            if (lane == 0) walk = next;
-            __syncwarp();
-        };
-        next_tile(true);
-        if (more) find();
         uint32_t phase = 1;  // of kv_empty[stage]: the first round finds it "complete"
-        while (more) {
-            const uint32_t valid = ask();
-            const bool mixed = walk.tile.mixed(p, block);
-            if (++block == end) next_tile(false);
-            if (more) find();
-
+        for (int it = 0;; ++it) {
+            const int entry = it & 1;
+            if (!warp_wait(&rest.look_full[entry], (it >> 1) & 1, abort)) break;
+            const uint64_t exist = rest.exist[entry];
+            if (exist >> 63) break;
+            const uint32_t valid = static_cast<uint32_t>(exist >> (kWarpKeys * reader)) & 0xfu;
+            const bool mixed = rest.mixed[entry] != 0;
+            ulonglong2 at[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) at[i] = rest.keys[entry][key_a + 2 * i];
+            __syncwarp();
+            if (lane == 0) barrier_arrive(&rest.look_empty[entry]);
+            uint4 low[2], high[2];
+            uint2 rotary[2], codes[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint8_t* data = reinterpret_cast<const uint8_t*>(at[i].x);
+                codes[i] = __ldg(reinterpret_cast<const uint2*>(at[i].y));
+                low[i] = ld_stream16(data + 16 * sub);
+                if (coded) high[i] = ld_stream16(data + 256 + 16 * sub);
+                rotary[i] = __ldg(reinterpret_cast<const uint2*>(data + kNopeDim + 8 * rotary_sub));
+            }
             if (!warp_wait(&rest.kv_empty[stage], phase, abort)) break;
             const bool all = valid == 0xfu;
             uint32_t bad = 0;
@@ -707,6 +679,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                 // Keys that some rows of the tile do not see: those with a value that is not finite are stored as zeros, which the rows that do
                 // not see them multiply by zero; the others get NaN as their score.
                 bad = __reduce_or_sync(0xffffffffu, bad);
+                if (lane == 0) rest.bad[stage][reader] = static_cast<uint8_t>(bad);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     if ((bad >> (2 * i + odd)) & 1u) {
@@ -717,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                     }
                 }
             }
-            if (lane == 0) rest.valid[stage][reader] = static_cast<uint8_t>(valid), rest.bad[stage][reader] = static_cast<uint8_t>(bad);
+            if (reader == 0 && lane == 0) rest.valid[stage] = exist;
             fence_to_async();
             __syncwarp();
             if (lane == 0) barrier_arrive(&rest.kv_full[stage]);
@@ -783,6 +756,55 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
             for (uint32_t i = 0; i < kTries && !barrier_try(&rest.drained, 0); ++i) {}
         }
         __syncwarp();
+    } else if (warp == kLookupWarp) {
+        // ------------------------------------------------------------------------------------------------ look-ups
+        set_registers<kOtherRegisters, false>();
+        // Keys lane and lane + 32 of each block.  Keys that do not exist are given q as their place, and zeroed when they have been read.
+        bool ok = true;
+        int it = 0;
+        const int64_t codes_from = static_cast<int64_t>(p.a.block_size) * kTokenDataBytes;
+        for (; ok && w.settle(p); w.step(p)) {
+            const Tile& t = w.tile;
+            for (int block = w.begin; block < w.end; ++block, ++it) {
+                const int entry = it & 1;
+                uint64_t exist = 0;
+                ulonglong2 at[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int n = lane + 32 * i, k = block * kBlockKeys + n;
+                    int number = -1;
+                    uint32_t in_block = 0;
+                    if (n < kBlockKeys && k < t.keys) {
+                        if (p.a.indices) {
+                            const int slot = __ldg(p.a.indices + t.token * p.a.indices_stride + k);
+                            if (slot >= 0) {
+                                number = fast_div(slot, p.a.block_mul, p.a.block_shift);
+                                in_block = slot - static_cast<uint32_t>(number) * p.a.block_size;
+                            }
+                        } else {
+                            const uint32_t where = k < t.first ? k : k - t.first + t.low, page = fast_div(where, p.a.block_mul, p.a.block_shift);
+                            in_block = where - page * p.a.block_size;
+                            number = __ldg(p.a.block_table + w.at.request * p.a.table_stride + page);
+                        }
+                    }
+                    const bool there = number >= 0 && number < p.a.num_blocks;
+                    const uint8_t* block_at = p.a.k_cache + number * p.a.block_stride;
+                    at[i].x = reinterpret_cast<uint64_t>(there ? block_at + static_cast<int64_t>(in_block) * kTokenDataBytes : p.a.q);
+                    at[i].y = reinterpret_cast<uint64_t>(there ? block_at + codes_from + static_cast<int64_t>(in_block) * kScaleBytes : p.a.q);
+                    exist |= static_cast<uint64_t>(__ballot_sync(0xffffffffu, there)) << (32 * i);
+                }
+                ok = warp_wait(&rest.look_empty[entry], ((it >> 1) - 1) & 1, abort);
+                if (!ok) break;
+                rest.keys[entry][lane] = at[0];
+                if (lane + 32 < kBlockKeys) rest.keys[entry][lane + 32] = at[1];
+                if (lane == 0) rest.exist[entry] = exist, rest.mixed[entry] = t.mixed(p, block);
+                __syncwarp();
+                if (lane == 0) barrier_arrive(&rest.look_full[entry]);
+            }
+        }
+        // the end
+        ok = ok && warp_wait(&rest.look_empty[it & 1], ((it >> 1) - 1) & 1, abort);
+        if (ok && lane == 0) rest.exist[it & 1] = 1ull << 63, barrier_arrive(&rest.look_full[it & 1]);
     } else {
         // ------------------------------------------------------------------------------------------------ queries
         set_registers<kOtherRegisters, false>();
@@ -792,7 +814,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
             const Tile& t = w.tile;
             if (tiles > 0 && !warp_wait(&rest.q_empty, (tiles - 1) & 1, abort)) break;
             // a row is 64 pieces of 16 bytes: two passes of the warp
-            for (int row = warp - kIssuerWarp - 1; row < kRows; row += kQueryWarps) {
+            for (int row = warp - kLookupWarp - 1; row < kRows; row += kQueryWarps) {
                 const int token = t.token + (t.count > 1 ? row / p.a.num_heads : 0);
                 const int head = t.count > 1 ? row % p.a.num_heads : t.head + row;
                 const bool live = row < t.rows;
