@@ -189,7 +189,8 @@ struct Lists {
 struct Tiles {
     LatentAttention a;
     Lists lists;
-    int32_t tokens_per_tile, heads_per_tile, head_groups;
+    int32_t tokens_per_tile, head_groups;
+    int32_t one_each;  // every CTA has the tile of its number, if there is one: no tile is long enough to be cut, and no more tokens than CTAs
     float* sums;      // workspace: [2 * kMaxCtas][64][512] unnormalised outputs,
     float2* rows;     // [2 * kMaxCtas][64] their maximum and sum,
     int4* pieces;     // [2 * kMaxCtas] what they belong to: token, first head, rows, and 0: nothing, 1: more follow, 2: the last
@@ -307,6 +308,22 @@ __device__ __forceinline__ void make_plan(const Tiles& p, Rest& rest, int32_t* s
             token += t.count;
         }
     };
+    if (tid == 0) rest.from = rest.to = Cut{p.a.num_reqs, p.a.num_tokens, 0, 0};
+    if (p.one_each) {
+        __syncthreads();
+        if (tid == 0) {
+            const int group = blockIdx.x % p.head_groups, mine = blockIdx.x / p.head_groups;
+            int token = mine;
+            const int request = mine < p.a.num_tokens ? request_of(p, lists, token) : p.a.num_reqs;
+            // (a token in front of the first request's, or behind the last one's, has none; nor has one in the middle of a tile)
+            if (mine < p.a.num_tokens && token == mine && (p.a.indices || (request < p.a.num_reqs && (token - lists.starts[request]) % p.tokens_per_tile == 0))) {
+                rest.from = Cut{request, token, group, 0};
+                rest.to = Cut{request, token, group + 1, 0};
+            }
+        }
+        __syncthreads();
+        return;
+    }
     uint64_t mine = 0;
     for_tiles([&](int, int, int blocks) {
         mine += static_cast<uint64_t>(blocks + 1) * p.head_groups;
@@ -326,8 +343,6 @@ __device__ __forceinline__ void make_plan(const Tiles& p, Rest& rest, int32_t* s
         total += rest.sums[w];
     }
     const uint64_t ctas = min(static_cast<uint64_t>(gridDim.x), max(total / kLeastShare, static_cast<uint64_t>(1)));
-    if (tid == 0) rest.from = rest.to = Cut{p.a.num_reqs, p.a.num_tokens, 0, 0};
-    __syncthreads();
     for (int side = 0; side < 2; ++side) {
         const uint64_t cta = blockIdx.x + side;
         if (cta >= ctas) continue;
@@ -340,7 +355,9 @@ __device__ __forceinline__ void make_plan(const Tiles& p, Rest& rest, int32_t* s
                 at = next;
                 return false;
             }
-            const int group = static_cast<int>((cut - at) / (blocks + 1)), offset = static_cast<int>((cut - at) % (blocks + 1));
+            const uint64_t behind = cut - at;  // (below 2^32 but for tiles of 2^25 blocks in hundreds of groups)
+            const uint32_t each = blocks + 1, whole = p.head_groups == 1 ? 0 : behind >> 32 ? static_cast<uint32_t>(behind / each) : static_cast<uint32_t>(behind) / each;
+            const int group = static_cast<int>(whole), offset = static_cast<int>(behind - static_cast<uint64_t>(whole) * each);
             int block = min(offset, blocks);
             if (blocks < kLeastSplit) block = 2 * offset <= blocks ? 0 : blocks;
             else if (block < kLeastPiece) block = 0;
@@ -540,66 +557,97 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                 l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
                 l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
             }
-            // from here on a lane's row is the one it has in TMEM: 16 * warp + lane % 16, dimensions 256 * (lane / 16) on
+            // From here on a lane's row is the one it has in TMEM: 16 * warp + lane % 16, dimensions 256 * (lane / 16) on.
             const int from = (lane & 7) << 2, row = 16 * warp + (lane & 15);
             const float ma = __shfl_sync(0xffffffffu, m[0], from), mb = __shfl_sync(0xffffffffu, m[1], from);
             const float la = __shfl_sync(0xffffffffu, l[0], from), lb = __shfl_sync(0xffffffffu, l[1], from);
             const float row_m = (lane & 8) ? mb : ma, row_l = (lane & 8) ? lb : la;
-            const bool live = row < t.rows;
-            const int token = t.token + (t.count > 1 ? row / p.a.num_heads : 0);
-            const int head = t.count > 1 ? row % p.a.num_heads : t.head + row;
-            if (w.begin < w.end) {
-                if (!warp_wait(&rest.pv_done[(it - 1) & 1], ((it - 1) >> 1) & 1, abort)) {
-                    ok = false;
-                    break;
-                }
-                fence_tmem_after();
-            }
-            if (w.whole()) {
-                const bool some = row_l != 0.0f;
-                float total = row_l;
-                if (live && p.a.sink && some) total += exp2_approx(fmaf(__ldg(p.a.sink + head), kLog2e, -row_m * c));
-                const float inverse = some ? 1.0f / total : 0.0f;
-                uint8_t* out = p.a.out + token * p.a.out_stride_token + head * p.a.out_stride_head + 512 * (lane >> 4);
-                if (live && lane < 16 && p.a.lse)
-                    p.a.lse[token * p.a.lse_stride_token + head * p.a.lse_stride_head] = some ? (row_m * c + log2f(row_l)) * kLn2 : -INFINITY;
-#pragma unroll 1
-                for (int at = 0; at < 256; at += 32) {
-                    float o[32];
-                    if (w.begin < w.end) {
-                        load_columns(o, tmem + at + lanes);
-                        wait_tmem_loads(o);
-                    }
-                    if (live) {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                            if (some)
-                                v = make_uint4(pack_bf16x2(o[i] * inverse, o[i + 1] * inverse), pack_bf16x2(o[i + 2] * inverse, o[i + 3] * inverse),
-                                               pack_bf16x2(o[i + 4] * inverse, o[i + 5] * inverse), pack_bf16x2(o[i + 6] * inverse, o[i + 7] * inverse));
-                            *reinterpret_cast<uint4*>(out + 2 * (at + i)) = v;
-                        }
-                    }
-                }
-            } else {
-                const int slot = w.begin == 0 ? slot_of_head : slot_of_rest;
-                float* out = p.sums + (static_cast<int64_t>(slot) * kRows + row) * kHeadDim + 256 * (lane >> 4);
+            const auto out_of = [&](int of) {
+                const int token = t.token + (t.count > 1 ? of / p.a.num_heads : 0), head = t.count > 1 ? of % p.a.num_heads : t.head + of;
+                return p.a.out + token * p.a.out_stride_token + head * p.a.out_stride_head;
+            };
+            float inverse = 0.0f;
+            const bool some = row_l != 0.0f, whole = w.whole();
+            const int slot = w.begin == 0 ? slot_of_head : slot_of_rest;
+            if (!whole) {
                 if (lane < 16) p.rows[slot * kRows + row] = make_float2(row_m, row_l);
                 if (threadIdx.x == 0) p.pieces[slot] = make_int4(t.token, t.head, t.rows, w.end == t.blocks ? 2 : 1);
+            } else if (row < t.rows) {
+                const int token = t.token + (t.count > 1 ? row / p.a.num_heads : 0), head = t.count > 1 ? row % p.a.num_heads : t.head + row;
+                float total = row_l;
+                if (p.a.sink && some) total += exp2_approx(fmaf(__ldg(p.a.sink + head), kLog2e, -row_m * c));
+                inverse = some ? 1.0f / total : 0.0f;
+                if (lane < 16 && p.a.lse)
+                    p.a.lse[token * p.a.lse_stride_token + head * p.a.lse_stride_head] = some ? (row_m * c + log2f(row_l)) * kLn2 : -INFINITY;
+            }
+            if (w.begin == w.end) {
+                if (row < t.rows) {
+                    uint8_t* out = out_of(row) + 512 * (lane >> 4);
 #pragma unroll 1
-                for (int at = 0; at < 256; at += 32) {
-                    float o[32];
-                    load_columns(o, tmem + at + lanes);
-                    wait_tmem_loads(o);
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(out + at + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    for (int i = 0; i < 512; i += 16) *reinterpret_cast<uint4*>(out + i) = make_uint4(0u, 0u, 0u, 0u);
                 }
+                continue;
             }
-            if (w.begin < w.end) {
-                fence_tmem_before();
+            if (!warp_wait(&rest.pv_done[(it - 1) & 1], ((it - 1) >> 1) & 1, abort)) {
+                ok = false;
+                break;
+            }
+            fence_tmem_after();
+            // 128 bytes of every row at a time, of both halves of its dimensions, go through this warp's rows of the two P buffers, which have been read:
+            // a store then writes four rows' 128 bytes, where a lane's own would touch 32 lines each.
+            const uint32_t stage_at = base + kOffsetP + 16 * warp * 128;
+            const uint32_t put = stage_at + (lane >> 4) * kQueryChunk + (lane & 15) * 128, get = stage_at + (lane >> 3) * 128;
+            const int unit = lane & 7;
+            uint8_t* to[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int of = 16 * warp + 4 * i + (lane >> 3);
+                to[i] = of >= t.rows ? nullptr : whole ? out_of(of) + 16 * unit : reinterpret_cast<uint8_t*>(p.sums + (static_cast<int64_t>(slot) * kRows + of) * kHeadDim) + 16 * unit;
+            }
+            const int half_bytes = whole ? 512 : 1024;
+#pragma unroll 1
+            for (int at = 0, bytes = 0; at < 256; bytes += 128) {
+                float o[32];
+                load_columns(o, tmem + at + lanes);
+                wait_tmem_loads(o);
+                if (whole) {
+#pragma unroll
+                    for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                            if (some)
+                                v = make_uint4(pack_bf16x2(o[8 * i] * inverse, o[8 * i + 1] * inverse), pack_bf16x2(o[8 * i + 2] * inverse, o[8 * i + 3] * inverse),
+                                               pack_bf16x2(o[8 * i + 4] * inverse, o[8 * i + 5] * inverse), pack_bf16x2(o[8 * i + 6] * inverse, o[8 * i + 7] * inverse));
+                            store_shared16(put + (((4 * pass + i) ^ (lane & 7)) << 4), v);
+                        }
+                        at += 32;
+                        if (pass == 0) {
+                            load_columns(o, tmem + at + lanes);
+                            wait_tmem_loads(o);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        store_shared16(put + ((i ^ (lane & 7)) << 4), make_uint4(__float_as_uint(o[4 * i]), __float_as_uint(o[4 * i + 1]), __float_as_uint(o[4 * i + 2]), __float_as_uint(o[4 * i + 3])));
+                    at += 32;
+                }
                 __syncwarp();
-                if (lane == 0) barrier_arrive(&rest.o_empty);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    uint4 v;
+                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                 : "r"(get + (i >> 2) * kQueryChunk + 4 * (i & 3) * 128 + ((unit ^ ((4 * i + (lane >> 3)) & 7)) << 4))
+                                 : "memory");
+                    if (to[i & 3]) *reinterpret_cast<uint4*>(to[i & 3] + (i >> 2) * half_bytes + bytes) = v;
+                }
+                __syncwarp();
             }
+            fence_tmem_before();
+            __syncwarp();
+            if (lane == 0) barrier_arrive(&rest.o_empty);
         }
     } else if (warp < kIssuerWarp) {
         // ------------------------------------------------------------------------------------------------ readers
@@ -814,17 +862,16 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
             const Tile& t = w.tile;
             if (tiles > 0 && !warp_wait(&rest.q_empty, (tiles - 1) & 1, abort)) break;
             // a row is 64 pieces of 16 bytes: two passes of the warp
-            for (int row = warp - kLookupWarp - 1; row < kRows; row += kQueryWarps) {
-                const int token = t.token + (t.count > 1 ? row / p.a.num_heads : 0);
-                const int head = t.count > 1 ? row % p.a.num_heads : t.head + row;
+            const uint32_t to = base + (lane >> 3) * kQueryChunk;
+            int token = t.token, head = t.head + warp - kLookupWarp - 1;
+#pragma unroll 4
+            for (int row = warp - kLookupWarp - 1; row < kRows; row += kQueryWarps, head += kQueryWarps) {
+                while (t.count > 1 && head >= p.a.num_heads) head -= p.a.num_heads, ++token;
                 const bool live = row < t.rows;
                 const uint8_t* from = live ? p.a.q + token * p.a.q_stride_token + head * p.a.q_stride_head : p.a.q;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int piece = lane + 32 * i;
-                    const uint32_t to = base + (piece >> 3) * kQueryChunk + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(live ? from + 16 * piece : from), "r"(live ? 16 : 0) : "memory");
-                }
+                const uint32_t at = to + row * 128 + (((lane & 7) ^ (row & 7)) << 4);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from + 16 * lane), "r"(live ? 16 : 0) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + 4 * kQueryChunk), "l"(from + 512 + 16 * lane), "r"(live ? 16 : 0) : "memory");
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             fence_to_async();
@@ -961,6 +1008,7 @@ cudaError_t launch_latent_attention(const LatentAttention& a, void* workspace, c
     // Where no tile can have enough keys to be cut, there are no pieces to join.
     const int64_t most_keys = a.indices ? a.topk : a.window > 0 ? static_cast<int64_t>(a.window) + a.first + p.tokens_per_tile : a.capacity;
     const bool may_split = std::min<int64_t>(most_keys, a.indices ? a.topk : a.capacity) > (kLeastSplit - 1) * kBlockKeys;
+    p.one_each = !may_split && static_cast<int64_t>(a.num_tokens) * p.head_groups <= kMaxCtas;
     auto* at = static_cast<uint8_t*>(workspace);
     p.sums = reinterpret_cast<float*>(at), p.rows = reinterpret_cast<float2*>(at + kSumBytes), p.pieces = reinterpret_cast<int4*>(at + kSumBytes + kRowBytes2);
     // Set for the current device each time: cheaper than to remember for which ones it was.
