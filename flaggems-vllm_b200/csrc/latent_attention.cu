@@ -605,45 +605,53 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                 to[i] = of >= t.rows ? nullptr : whole ? out_of(of) + 16 * unit : reinterpret_cast<uint8_t*>(p.sums + (static_cast<int64_t>(slot) * kRows + of) * kHeadDim) + 16 * unit;
             }
             const int half_bytes = whole ? 512 : 1024;
-#pragma unroll 1
-            for (int at = 0, bytes = 0; at < 256; bytes += 128) {
-                float o[32];
-                load_columns(o, tmem + at + lanes);
-                wait_tmem_loads(o);
-                if (whole) {
+            const auto pass_on = [&] {
+                __syncwarp();
+                uint4 v[8];
 #pragma unroll
-                    for (int pass = 0; pass < 2; ++pass) {
+                for (int i = 0; i < 8; ++i)
+                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(v[i].x), "=r"(v[i].y), "=r"(v[i].z), "=r"(v[i].w)
+                                 : "r"(get + (i >> 2) * kQueryChunk + 4 * (i & 3) * 128 + ((unit ^ ((4 * i + (lane >> 3)) & 7)) << 4))
+                                 : "memory");
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                            if (some)
-                                v = make_uint4(pack_bf16x2(o[8 * i] * inverse, o[8 * i + 1] * inverse), pack_bf16x2(o[8 * i + 2] * inverse, o[8 * i + 3] * inverse),
-                                               pack_bf16x2(o[8 * i + 4] * inverse, o[8 * i + 5] * inverse), pack_bf16x2(o[8 * i + 6] * inverse, o[8 * i + 7] * inverse));
-                            store_shared16(put + (((4 * pass + i) ^ (lane & 7)) << 4), v);
-                        }
-                        at += 32;
-                        if (pass == 0) {
-                            load_columns(o, tmem + at + lanes);
-                            wait_tmem_loads(o);
-                        }
+                for (int i = 0; i < 4; ++i)
+                    if (to[i]) {
+                        *reinterpret_cast<uint4*>(to[i]) = v[i];
+                        *reinterpret_cast<uint4*>(to[i] + half_bytes) = v[i + 4];
+                        to[i] += 128;
                     }
-                } else {
+                __syncwarp();
+            };
+            if (whole) {
+                const uint32_t keep = some ? 0xffffffffu : 0u;
+#pragma unroll 1
+                for (int at = 0; at < 256; at += 64) {
+                    float o[2][32];
+                    load_columns(o[0], tmem + at + lanes);
+                    load_columns(o[1], tmem + at + 32 + lanes);
+                    wait_tmem_loads(o[0]), wait_tmem_loads(o[1]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float* from = o[i >> 2] + 8 * (i & 3);
+                        uint32_t v[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) v[k] = pack_bf16x2(from[2 * k] * inverse, from[2 * k + 1] * inverse) & keep;
+                        store_shared16(put + ((i ^ (lane & 7)) << 4), make_uint4(v[0], v[1], v[2], v[3]));
+                    }
+                    pass_on();
+                }
+            } else {
+#pragma unroll 1
+                for (int at = 0; at < 256; at += 32) {
+                    float o[32];
+                    load_columns(o, tmem + at + lanes);
+                    wait_tmem_loads(o);
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         store_shared16(put + ((i ^ (lane & 7)) << 4), make_uint4(__float_as_uint(o[4 * i]), __float_as_uint(o[4 * i + 1]), __float_as_uint(o[4 * i + 2]), __float_as_uint(o[4 * i + 3])));
-                    at += 32;
+                    pass_on();
                 }
-                __syncwarp();
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    uint4 v;
-                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                                 : "r"(get + (i >> 2) * kQueryChunk + 4 * (i & 3) * 128 + ((unit ^ ((4 * i + (lane >> 3)) & 7)) << 4))
-                                 : "memory");
-                    if (to[i & 3]) *reinterpret_cast<uint4*>(to[i & 3] + (i >> 2) * half_bytes + bytes) = v;
-                }
-                __syncwarp();
             }
             fence_tmem_before();
             __syncwarp();
@@ -861,17 +869,25 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
             if (w.begin == w.end) continue;
             const Tile& t = w.tile;
             if (tiles > 0 && !warp_wait(&rest.q_empty, (tiles - 1) & 1, abort)) break;
-            // a row is 64 pieces of 16 bytes: two passes of the warp
-            const uint32_t to = base + (lane >> 3) * kQueryChunk;
-            int token = t.token, head = t.head + warp - kLookupWarp - 1;
-#pragma unroll 4
-            for (int row = warp - kLookupWarp - 1; row < kRows; row += kQueryWarps, head += kQueryWarps) {
-                while (t.count > 1 && head >= p.a.num_heads) head -= p.a.num_heads, ++token;
-                const bool live = row < t.rows;
-                const uint8_t* from = live ? p.a.q + token * p.a.q_stride_token + head * p.a.q_stride_head : p.a.q;
-                const uint32_t at = to + row * 128 + (((lane & 7) ^ (row & 7)) << 4);
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from + 16 * lane), "r"(live ? 16 : 0) : "memory");
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + 4 * kQueryChunk), "l"(from + 512 + 16 * lane), "r"(live ? 16 : 0) : "memory");
+            // Atoms of eight rows in turn; a row is 64 pieces of 16 bytes, two passes of the warp.  (These warps share their schedulers with the
+            // readers: the time that a tile's queries take is that of the instructions for them.)
+            const int own = warp - kLookupWarp - 1;
+            int row = 8 * own, token = t.token, head = t.head + row;
+#pragma unroll 1
+            for (; row < kRows; row += 8 * (kQueryWarps - 1), head += 8 * (kQueryWarps - 1)) {
+                if (t.count > 1) token = t.token + row / p.a.num_heads, head = row % p.a.num_heads;
+                const uint8_t* from = p.a.q + token * p.a.q_stride_token + head * p.a.q_stride_head + 16 * lane;
+                const uint32_t to = base + (lane >> 3) * kQueryChunk + row * 128;
+#pragma unroll
+                for (int i = 0; i < 8; ++i, ++row) {
+                    const uint32_t at = to + i * 128 + (((lane & 7) ^ i) << 4);
+                    const bool live = row < t.rows;
+                    const uint8_t* safe = live ? from : p.a.q;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(safe), "r"(live ? 16 : 0) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + 4 * kQueryChunk), "l"(safe + 512), "r"(live ? 16 : 0) : "memory");
+                    from += p.a.q_stride_head;
+                    if (++head == p.a.num_heads && t.count > 1) head = 0, from += p.a.q_stride_token - p.a.num_heads * p.a.q_stride_head;
+                }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             fence_to_async();
