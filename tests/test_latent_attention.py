@@ -156,6 +156,29 @@ def test_requests_without_tokens_or_keys_and_rows_behind_the_last():
 
 
 @gpu
+@pytest.mark.parametrize("heads,new", [(64, [150, 40]), (128, [70, 4]), (128, [71, 4]), (16, [139, 5]), (16, [146, 5])])
+def test_short_lists_with_and_without_a_cta_for_each(heads, new):
+    """No tile is long enough to be cut: fewer or as many tokens (times groups of heads) as CTAs, or more."""
+    b = Batch([200, 60], new, heads, 64, seed=14)
+    out, lse = b.run(16, 2)
+    check(out, lse, b.want(16, 2))
+
+
+@gpu
+@pytest.mark.parametrize("window", [16, None])
+def test_rows_in_front_of_the_first_request(window):
+    """Rows that belong to no request lie in front of the first one and behind the last, and stay as they are."""
+    b = Batch([80, 30], [3, 6], 16, 64, seed=15, extra_rows=6)
+    want = b.want(window)
+    b.q = b.q.roll(4, 0)
+    b.starts += 4
+    out, lse = b.run(window)
+    check(out[4:13], lse[4:13], want)
+    for rows in (slice(0, 4), slice(13, None)):
+        assert (out[rows] == 7).all() and (lse[rows] == 7).all()
+
+
+@gpu
 @pytest.mark.parametrize("heads", [16, 64, 128])
 def test_long_contexts(heads):
     """Work split over the keys of few rows; ragged."""
