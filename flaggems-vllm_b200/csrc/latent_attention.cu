@@ -167,6 +167,27 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
+// max(a, b, c), two products and sums at once: one instruction each
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 y;
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(y.x), "=f"(y.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return y;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 y;
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(y.x), "=f"(y.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return y;
+}
+
 // Shared-memory operand with 128-byte swizzle: atoms of 8 rows x 128 bytes, the next 8 rows 1024 bytes on.  `leading`: bytes between chunks of
 // 64 dimensions, used where the dimensions are the operand's outer direction.
 __device__ __forceinline__ uint64_t operand(uint32_t address, uint32_t leading) {
@@ -385,7 +406,8 @@ __device__ __forceinline__ uint32_t two_values(uint32_t word, uint32_t scale) {
 }
 
 // 2^(code - 127) as a pair of bf16; 0: subnormal, 255: infinity.
-__device__ __forceinline__ uint32_t power_of_code(uint32_t code) { return (code == 0u ? 0x40u : code << 7) * 0x10001u; }
+// `codes` has the code twice, one in each half.
+__device__ __forceinline__ uint32_t power_of_codes(uint32_t codes) { return __vmaxu2(codes << 7, 0x400040u); }
 
 // Whether one of a bf16 pair is infinite or NaN.
 __device__ __forceinline__ bool not_finite(uint32_t pair) { return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u; }
@@ -449,7 +471,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
         __syncwarp();
         for (; ok && w.settle(p); w.step(p)) {
             const Tile& t = w.tile;
-            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+            float m[2] = {-INFINITY, -INFINITY};
+            float2 l[2] = {};  // (sums of even and of odd columns)
             // positions of this thread's two rows
             int position[2] = {t.position, t.position};
             if (t.count > 1) position[0] += row_a / p.a.num_heads, position[1] += (row_a + 8) / p.a.num_heads;
@@ -484,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                 }
                 float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < 24; ++i) top[(i >> 1) & 1] = fmaxf(top[(i >> 1) & 1], s[i]);
+                for (int i = 0; i < 24; i += 2) top[(i >> 1) & 1] = max3(top[(i >> 1) & 1], s[i], s[i + 1]);
                 // The common case is that no row's maximum has grown by so much that it matters: every lane sees that of its own columns.
                 bool grown = false;
 #pragma unroll
@@ -500,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                             m[r] = top[r];  // (O is zero so far)
                         } else if (top[r] > m[r]) {
                             factor[r] = exp2_approx((m[r] - top[r]) * c);
-                            l[r] *= factor[r];
+                            l[r].x *= factor[r], l[r].y *= factor[r];
                             m[r] = top[r];
                             correct = true;
                         }
@@ -529,9 +552,11 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                 }
                 const float mc[2] = {m[0] == -INFINITY ? 0.0f : m[0] * c, m[1] == -INFINITY ? 0.0f : m[1] * c};
 #pragma unroll
-                for (int i = 0; i < 24; ++i) {
-                    s[i] = exp2_approx(fmaf(s[i], c, -mc[(i >> 1) & 1]));
-                    l[(i >> 1) & 1] += s[i];
+                for (int i = 0; i < 24; i += 2) {
+                    const int r = (i >> 1) & 1;
+                    const float2 x = fma2(make_float2(s[i], s[i + 1]), make_float2(c, c), make_float2(-mc[r], -mc[r]));
+                    s[i] = exp2_approx(x.x), s[i + 1] = exp2_approx(x.y);
+                    l[r] = add2(l[r], make_float2(s[i], s[i + 1]));
                 }
                 // P of two blocks ago has been read
                 if (it >= 2 && !warp_wait(&rest.pv_done[buffer], ((it >> 1) - 1) & 1, abort)) {
@@ -554,13 +579,14 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
             if (!ok) break;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+                l[r].x += l[r].y;
+                l[r].x += __shfl_xor_sync(0xffffffffu, l[r].x, 1);
+                l[r].x += __shfl_xor_sync(0xffffffffu, l[r].x, 2);
             }
             // From here on a lane's row is the one it has in TMEM: 16 * warp + lane % 16, dimensions 256 * (lane / 16) on.
             const int from = (lane & 7) << 2, row = 16 * warp + (lane & 15);
             const float ma = __shfl_sync(0xffffffffu, m[0], from), mb = __shfl_sync(0xffffffffu, m[1], from);
-            const float la = __shfl_sync(0xffffffffu, l[0], from), lb = __shfl_sync(0xffffffffu, l[1], from);
+            const float la = __shfl_sync(0xffffffffu, l[0].x, from), lb = __shfl_sync(0xffffffffu, l[1].x, from);
             const float row_m = (lane & 8) ? mb : ma, row_l = (lane & 8) ? lb : la;
             const auto out_of = [&](int of) {
                 const int token = t.token + (t.count > 1 ? of / p.a.num_heads : 0), head = t.count > 1 ? of % p.a.num_heads : t.head + of;
@@ -670,23 +696,22 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
         const uint32_t store_row = base + kOffsetKeys + key_a * 128, unit = 2 * (sub & 3);
         const bool coded = sub < 12;
         const int rotary_sub = sub ^ (8 * odd);  // (the two keys' halves, so that their stores use different banks)
-        const int code_shift = 8 * (sub >> 2);
+        const uint32_t code_select = 0x4040u + 0x0101u * (sub >> 2);  // of a byte and of zeros: the byte in both halves
         // 16 e4m3 values to two 16-byte columns
         const auto convert = [&](const uint4& v, uint32_t code_word, uint4& a, uint4& b) {
-            const uint32_t scale = power_of_code((code_word >> code_shift) & 0xffu);
+            const uint32_t scale = power_of_codes(__byte_perm(code_word, 0u, code_select));
             a = make_uint4(two_values<0>(v.x, scale), two_values<1>(v.x, scale), two_values<0>(v.y, scale), two_values<1>(v.y, scale));
             b = make_uint4(two_values<0>(v.z, scale), two_values<1>(v.z, scale), two_values<0>(v.w, scale), two_values<1>(v.w, scale));
         };
+        uint32_t to[2][2], to_rotary[2];  // where this lane's values of the two keys go: 16-byte columns of the first half's chunk, and the rotary ones
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t twist = (key_a + 2 * i) & 7, row = store_row + 2 * i * 128;
+            to[i][0] = row + (sub >> 2) * kKeyChunk + ((unit ^ twist) << 4), to[i][1] = row + (sub >> 2) * kKeyChunk + (((unit + 1) ^ twist) << 4);
+            to_rotary[i] = row + 7 * kKeyChunk + (((rotary_sub >> 1) ^ twist) << 4) + 8 * (sub & 1);
+        }
         int stage = 0;
-        const auto store = [&](int half, int i, const uint4& a, const uint4& b) {
-            const uint32_t at = store_row + stage * kKeyBytes + (4 * half + (sub >> 2)) * kKeyChunk + 2 * i * 128, twist = (key_a + 2 * i) & 7;
-            store_shared16(at + ((unit ^ twist) << 4), a);
-            store_shared16(at + (((unit + 1) ^ twist) << 4), b);
-        };
-        const auto store_rotary = [&](int i, uint2 v) {
-            const uint32_t at = store_row + stage * kKeyBytes + 7 * kKeyChunk + 2 * i * 128 + (((rotary_sub >> 1) ^ ((key_a + 2 * i) & 7)) << 4) + 8 * (sub & 1);
-            asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(at), "r"(v.x), "r"(v.y) : "memory");
-        };
+        uint32_t stage_at = 0;
         uint32_t phase = 1;  // of kv_empty[stage]: the first round finds it "complete"
         for (int it = 0;; ++it) {
             const int entry = it & 1;
@@ -711,46 +736,50 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                 rotary[i] = __ldg(reinterpret_cast<const uint2*>(data + kNopeDim + 8 * rotary_sub));
             }
             if (!warp_wait(&rest.kv_empty[stage], phase, abort)) break;
-            const bool all = valid == 0xfu;
-            uint32_t bad = 0;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const bool absent = !all && ((valid >> (2 * i + odd)) & 1u) == 0;
-                uint4 a, b;
-                convert(low[i], codes[i].x, a, b);
-                if (absent) a = b = make_uint4(0u, 0u, 0u, 0u);
-                store(0, i, a, b);
-                if (mixed && (not_finite(a) || not_finite(b))) bad |= 1u << (2 * i + odd);
-                if (coded) {
-                    convert(high[i], codes[i].y, a, b);
-                    if (absent) a = b = make_uint4(0u, 0u, 0u, 0u);
-                    store(1, i, a, b);
-                    if (mixed && (not_finite(a) || not_finite(b))) bad |= 1u << (2 * i + odd);
-                }
-                if (absent) rotary[i] = make_uint2(0u, 0u);
-                store_rotary(i, rotary[i]);
-                if (mixed && (not_finite(rotary[i].x) || not_finite(rotary[i].y))) bad |= 1u << (2 * i + odd);
-            }
+            uint32_t none = ~valid;  // keys of this warp that are stored as zeros
             if (mixed) {
                 // Keys that some rows of the tile do not see: those with a value that is not finite are stored as zeros, which the rows that do
                 // not see them multiply by zero; the others get NaN as their score.
-                bad = __reduce_or_sync(0xffffffffu, bad);
-                if (lane == 0) rest.bad[stage][reader] = static_cast<uint8_t>(bad);
+                uint32_t bad = 0;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    if ((bad >> (2 * i + odd)) & 1u) {
-                        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-                        store(0, i, zero, zero);
-                        if (coded) store(1, i, zero, zero);
-                        store_rotary(i, make_uint2(0u, 0u));
+                    uint4 a, b;
+                    convert(low[i], codes[i].x, a, b);
+                    bool any = not_finite(a) || not_finite(b) || not_finite(rotary[i].x) || not_finite(rotary[i].y);
+                    if (coded) {
+                        convert(high[i], codes[i].y, a, b);
+                        any = any || not_finite(a) || not_finite(b);
                     }
+                    if (any) bad |= 1u << (2 * i + odd);
                 }
+                bad = __reduce_or_sync(0xffffffffu, bad) & valid;
+                if (lane == 0) rest.bad[stage][reader] = static_cast<uint8_t>(bad);
+                none |= bad;
+            }
+            if ((none & 0xfu) != 0) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if ((none >> (2 * i + odd)) & 1u) low[i] = high[i] = make_uint4(0u, 0u, 0u, 0u), rotary[i] = codes[i] = make_uint2(0u, 0u);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint4 a, b;
+                convert(low[i], codes[i].x, a, b);
+                store_shared16(to[i][0] + stage_at, a);
+                store_shared16(to[i][1] + stage_at, b);
+                if (coded) {
+                    convert(high[i], codes[i].y, a, b);
+                    store_shared16(to[i][0] + stage_at + 4 * kKeyChunk, a);
+                    store_shared16(to[i][1] + stage_at + 4 * kKeyChunk, b);
+                }
+                asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(to_rotary[i] + stage_at), "r"(rotary[i].x), "r"(rotary[i].y) : "memory");
             }
             if (reader == 0 && lane == 0) rest.valid[stage] = exist;
             fence_to_async();
             __syncwarp();
             if (lane == 0) barrier_arrive(&rest.kv_full[stage]);
-            if (++stage == kStages) stage = 0, phase ^= 1;
+            stage_at += kKeyBytes;
+            if (++stage == kStages) stage = 0, stage_at = 0, phase ^= 1;
         }
     } else if (warp == kIssuerWarp) {
         // ------------------------------------------------------------------------------------------------ products
