@@ -8,8 +8,11 @@
 // definition bit for bit; a power-of-two scale would otherwise move by a factor of two where the last bit of a 32-bit sum carries it
 // across.
 //
-// One CTA per row, the row's sum in registers: thread i holds the 16-byte pieces i, i + blockDim, ..., so every access of a warp is 512
-// contiguous bytes and a group of 64 / 128 / 256 values is 8 / 16 / 32 neighbouring lanes.  Bound by HBM: 7 bytes a value.
+// As many CTAs as fit take rows in turn, the row's sum in registers: thread i holds the 16-byte pieces i, i + blockDim, ..., so every access of a
+// warp is 512 contiguous bytes and a group of 64 / 128 / 256 values is 8 / 16 / 32 neighbouring lanes.  The next row is copied to shared memory
+// while this one is worked on (with a CTA for each row instead, 4097 x 7168 took 47.7 us).  Bound by HBM, 7 bytes a value, for many long rows: 4097 x 7168
+// bf16 38.3 us (82% of the time that a copy of as many bytes takes), 8192 x 4096 fp16, a scale a row, 45.8; the rest is the arithmetic, about 60
+// instructions a piece.  One to 148 rows: 2.9 us, the latency of one row's loads, two reductions and stores.
 #include <algorithm>
 
 #include "dsv4_common.cuh"
@@ -320,9 +323,11 @@ cudaError_t launch_add_rmsnorm_quant(const void* x, int64_t x_stride, void* resi
     p.pieces = static_cast<int32_t>(cols / 8), p.group_lanes = group_size == cols ? 0 : static_cast<int32_t>(group_size / 8);
     while ((1 << p.group_shift) < p.group_lanes) ++p.group_shift;
     p.eps = eps, p.inv_cols = 1.0 / static_cast<double>(cols);
-    // Threads for a row: four pieces each, and no more threads than that takes; one piece each where there are few rows.
+    // Pieces a thread.  Few rows: one, for the shortest way (148 x 7168: one 3.0 us, four 3.6; 149: 4.5 | 4.2).  Many: more, so that a row's fixed cost, its
+    // reductions and barriers, falls on fewer warps (4097 x 7168: one 49 us, four 39, eight 57; 8192 x 2048: one 26.1, two 20.2, four 27.8; 8192 x 1024: one
+    // 15.3, two 12.3; 8192 x 768: 14.9 | 12.6; 8192 x 512: 8.7 | 9.9), as far as the registers hold them.
     const auto threads_for = [&](int each) { return ((p.pieces + each - 1) / each + 31) / 32 * 32; };
-    const int pieces = p.pieces <= 128 || (rows <= 148 && p.pieces <= 1024) ? 1 : p.pieces <= 256 ? 2 : p.pieces <= 1024 ? 4 : 8;
+    const int pieces = p.pieces <= 64 || (rows <= 148 && p.pieces <= 1024) ? 1 : p.pieces <= 256 ? 2 : p.pieces <= 1024 ? 4 : 8;
     const int threads = threads_for(pieces);
     if (fp16) return weight_f32 ? launch_pieces<Fp16, true>(pieces, rows, threads, stream, p, pow2) : launch_pieces<Fp16, false>(pieces, rows, threads, stream, p, pow2);
     return weight_f32 ? launch_pieces<Bf16, true>(pieces, rows, threads, stream, p, pow2) : launch_pieces<Bf16, false>(pieces, rows, threads, stream, p, pow2);

@@ -6,20 +6,29 @@
 // in one pass over the keys with a running maximum m and sum.  Both products run on the tensor cores with fp32 accumulators in TMEM.
 //
 // A tile is 64 rows of q that share a list of keys: the heads of one token (64 of them at a time), or of several neighbouring tokens of a
-// request where there are fewer heads.  A CTA holds a tile's q (64 KiB) and streams its keys in blocks of 64:
-//   warps 4-11  "readers": find the 64 cached rows, convert them to bf16 and store them swizzled, once; the same bytes are the K-major
-//               operand of S = Q K^T and the MN-major operand of O += P V.  A block is two halves of 256 dimensions, four halves in all
-//               in a ring, so that a half is refilled as soon as the product that reads it last is done with it.
-//   warp 12     one thread issues the products: S of the next block before O of this one, so that they run while the softmax does.
-//   warps 0-3   "softmax": S from TMEM, masks, running maximum and sum, P as bf16 to shared memory; O is multiplied by a correction only where
-//               a row's maximum has grown by more than a factor of 2^8 (P and the sum may exceed one by that factor; fp32 holds them).
-//   warp 13     copies q of the next tile as soon as the last S of this one is done.
+// request where there are fewer heads.  A CTA of 20 warps holds a tile's q (64 KiB) and streams its keys in blocks of 48, three of them in flight:
+//   warps 0-3    "softmax": S from TMEM, masks, running maximum and sum, P as bf16 to shared memory; O is multiplied by a correction only where a row's
+//                maximum has grown by more than a factor of 2^8 (P and the sum may exceed one by that factor; fp32 holds them).  At a tile's end: O to the
+//                output, or to the workspace as a piece.
+//   warps 4-15   "readers": four keys of each block a warp.  They convert the cached rows to bf16 and store them swizzled, once; the same bytes are the
+//                K-major operand of S = Q K^T and the MN-major operand of O += P V.
+//   warp 16      one elected lane issues the products: S of the next block before O of this one, so that they run while the softmax does.
+//   warp 17      looks the next two blocks' keys up (block table or list of slots) and tells the readers where they are.
+//   warps 18-19  copy q of the next tile as soon as the last S of this one is done.
 // O takes 64 x 512 accumulators: 256 columns, dimensions 0-255 in lanes 0-15 of each 32 and 256-511 in lanes 16-31 (a product of 64 rows uses
 // 16 lanes of each 32).
 //
 // Rows of work are few in decoding and of any length, so the blocks of all tiles are dealt out evenly: every CTA computes the same prefix sum
 // over the tiles' numbers of blocks and takes its share, which may begin and end inside a tile.  Pieces of a tile go to a workspace as
-// unnormalised sums and are joined, in a fixed order, by a second small kernel.
+// unnormalised sums and are joined, in a fixed order, by a second small kernel.  Where lists are short, tiles are not cut (see kLeastSplit).
+//
+// What bounds it.  A block takes about 2400 cycles, over all 148 SMs: the products 1700 (a product of 64 rows runs at half the rate of one of 128, which
+// would need 128 KiB for q and 512 columns for O, and leave nothing for S); the readers 2100 and the softmax 1650, which with 20 warps on four
+// schedulers is close to what these can issue (an e4m3 pair takes five instructions to become bf16).  Large chunks also run at about 1.6 GHz for power.
+// 1024 tokens x 128 heads over 8192 keys: 3.4 ms (690 TFLOP/s); 61 requests of up to 16384 keys, 64 heads: 158 us; one of 65536 keys, 128 heads: 46 us;
+// a window of 128 tokens, one request: 11.6 us, of which two thirds are the way in (plan, look-up, keys, q: each waits for memory that the one before names) and out.
+// Other forms that were built: blocks of 64 keys in two stages, 6.9 ms; two groups of readers in turn, 4.5; eight softmax warps, 4.1 (this form then 3.9);
+// two CTAs that share out keys and exchange S and P, 128 rows a product: 5.0, since each exchange takes 400 cycles one way.
 #include <algorithm>
 
 #include "dsv4_common.cuh"
@@ -39,11 +48,16 @@ constexpr int kThreads = 32 * (kLookupWarp + 1 + kQueryWarps), kWarpKeys = kBloc
 constexpr int kSoftmaxRegisters = 128, kReaderRegisters = 80, kOtherRegisters = 96;
 static_assert(kThreads == 640 && kWarpKeys == 4 && 4 * kSoftmaxRegisters + 12 * kReaderRegisters + 4 * kOtherRegisters <= 20 * 96, "");
 constexpr uint64_t kAllKeys = (1ull << kBlockKeys) - 1;
-constexpr float kMostGrowth = 8.0f;  // log2 of the factor that a row's maximum may have grown by before O is corrected
+constexpr float kMostGrowth = 8.0f;  // log2 of the factor that a row's maximum may have grown by before O is corrected (with 0: 61 requests 209 us, not 155)
 constexpr int kMaxCtas = 148;        // a B200's SMs: one CTA on each (its shared memory allows no second)
-// Cuts between CTAs are moved to a tile's border where a piece would be short of this many blocks, and fewer CTAs take part where each
-// would have less than kLeastShare of them: a piece costs 128 KiB of fp32 sums out and in.
-constexpr int kLeastPiece = 2, kLeastShare = 4, kLeastSplit = 8;
+// Splitting.  A piece costs 128 KiB of fp32 sums out and in, and the kernel that joins them 6 to 10 us, so no tile shorter than kLeastSplit blocks is cut
+// (with 8: 61 tokens x 128 heads of up to 512 listed keys 38 us, with 16: 24; a chunk with a window of 512: 515 | 462; one request of 700 keys: 24.7 | 26.6);
+// no piece is shorter than kLeastPiece (61 requests of up to 16384 keys: with 2 154.5 us, with 4 152.6); and a CTA has at least kLeastShare blocks (with 3, 4, 5
+// and 6, one request of 700 keys: 26.3, 27.4, 25.4, 27.7 us).
+// Where every tile can have a CTA and none is longer than kMostWhole blocks, they stay whole if that costs the longest no more than kSplitCost blocks over an even
+// share (61 x 128 heads of up to 1000 keys: 36 us, cut 49; 8 x 128 heads of up to 700: 26.8, cut 26.5).  The CTA of each is then its number, which saves the
+// plan (one request, a window of 128: 12.1 us, with a plan 13.8).  Beyond kMostWhole a batch of one long and many short lists would lose too much.
+constexpr int kLeastPiece = 4, kLeastShare = 5, kLeastSplit = 16, kSplitCost = 12, kMostWhole = 24;
 
 // ---- shared memory -----------------------------------------------------------------------------------------------------------
 
@@ -91,7 +105,7 @@ __device__ __forceinline__ bool barrier_try(uint64_t* bar, uint32_t parity) {
     return done != 0;
 }
 // Bounded: false, and the CTA's other roles told to leave, where the phase does not complete within 2^22 tries, each of which the hardware
-// suspends for up to about a microsecond (a second or more in all; a phase takes a few microseconds).
+// suspends for up to two microseconds (some seconds in all; a phase takes a few microseconds).
 constexpr uint32_t kTries = 1u << 22;
 __device__ __forceinline__ bool barrier_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
     for (uint32_t i = 0; i < kTries; ++i) {
@@ -211,7 +225,7 @@ struct Tiles {
     LatentAttention a;
     Lists lists;
     int32_t tokens_per_tile, head_groups;
-    int32_t one_each;  // every CTA has the tile of its number, if there is one: no tile is long enough to be cut, and no more tokens than CTAs
+    int32_t one_each;  // every CTA has the whole tile of its number, if there is one
     float* sums;      // workspace: [2 * kMaxCtas][64][512] unnormalised outputs,
     float2* rows;     // [2 * kMaxCtas][64] their maximum and sum,
     int4* pieces;     // [2 * kMaxCtas] what they belong to: token, first head, rows, and 0: nothing, 1: more follow, 2: the last
@@ -1050,10 +1064,11 @@ cudaError_t launch_latent_attention(const LatentAttention& a, void* workspace, c
     p.lists = Lists{a.query_start_loc, a.indices ? a.lens : a.seq_lens};
     p.tokens_per_tile = a.indices || a.num_heads >= kRows ? 1 : kRows / a.num_heads;
     p.head_groups = (a.num_heads + kRows - 1) / kRows;
-    // Where no tile can have enough keys to be cut, there are no pieces to join.
-    const int64_t most_keys = a.indices ? a.topk : a.window > 0 ? static_cast<int64_t>(a.window) + a.first + p.tokens_per_tile : a.capacity;
-    const bool may_split = std::min<int64_t>(most_keys, a.indices ? a.topk : a.capacity) > (kLeastSplit - 1) * kBlockKeys;
-    p.one_each = !may_split && static_cast<int64_t>(a.num_tokens) * p.head_groups <= kMaxCtas;
+    const int64_t most_keys = a.indices ? a.topk : std::min<int64_t>(a.capacity, a.window > 0 ? static_cast<int64_t>(a.window) + a.first + p.tokens_per_tile : a.capacity);
+    const int64_t most_blocks = (most_keys + kBlockKeys - 1) / kBlockKeys, tiles = static_cast<int64_t>(a.num_tokens) * p.head_groups;
+    const int64_t fewest_tiles = (static_cast<int64_t>(a.num_tokens) + p.tokens_per_tile - 1) / p.tokens_per_tile * p.head_groups;
+    p.one_each = tiles <= kMaxCtas && (most_blocks < kLeastSplit || (most_blocks <= kMostWhole && most_blocks * (kMaxCtas - fewest_tiles) <= kSplitCost * kMaxCtas));
+    const bool may_split = !p.one_each && most_blocks >= kLeastSplit;
     auto* at = static_cast<uint8_t*>(workspace);
     p.sums = reinterpret_cast<float*>(at), p.rows = reinterpret_cast<float2*>(at + kSumBytes), p.pieces = reinterpret_cast<int4*>(at + kSumBytes + kRowBytes2);
     // Set for the current device each time: cheaper than to remember for which ones it was.

@@ -338,6 +338,17 @@ def test_sparse(tokens, heads, topk):
 
 
 @gpu
+@pytest.mark.parametrize("tokens,topk", [(74, 1100), (75, 1100), (74, 1200), (3, 700), (3, 800), (150, 700)])
+def test_sparse_lists_that_may_be_cut_or_not(tokens, topk):
+    """Both sides of the rules on when a CTA takes a whole tile and when tiles may be cut; a few long lists among short ones."""
+    cache, indices, lens, q, sink = sparse_case(tokens, 128, topk, seed=topk)
+    lens[1:] = lens[1:] % 50
+    lens[tokens // 2] = topk - 1
+    out, lse = run_sparse(cache, indices, lens, q, sink)
+    check(out, lse, [definition(q[t], key_rows(cache, 64, indices[t, : lens[t]].tolist()), SCALE, sink) for t in range(tokens)])
+
+
+@gpu
 def test_sparse_lengths_outside_the_list():
     case = sparse_case(4, 16, 70, seed=20)
     cache, indices, lens, q, sink = case
