@@ -19,8 +19,9 @@ q is bfloat16 [tokens, heads, 512] with unit inner stride, any number of heads; 
 
 A row that sees no key is zero, with an lse of -inf.  Keys that a row does not see do not influence it, whatever their bytes: pages behind a
 sequence's end, later tokens of a chunk, entries behind `lens`.  A page or slot outside the cache, and a position behind the block table, is
-seen by nobody.  A key with a value that is not finite makes the rows that see it NaN.  Rows of q behind the last request stay as they are in `out`
-and `lse` (in an `out` that was allocated here they are not defined).
+seen by nobody.  A key with a value that is not finite makes the rows that see it NaN, all of them or, where the score is -inf, at least the
+dimensions that are not finite (a row all of whose scores are -inf counts as one that sees no key).  Rows of q behind the last request stay as
+they are in `out` and `lse` (in an `out` that was allocated here they are not defined).
 """
 from __future__ import annotations
 

@@ -349,8 +349,8 @@ int dsv4_fused_add_rmsnorm_quant_fp8(const void* x, int64_t x_row_stride, void* 
  *   lse        fp32, strides in elements
  *   k_cache    as written by the prologue, num_blocks blocks; base and block stride on 16-byte boundaries
  *   workspace  dsv4_latent_attention_workspace_bytes(...) bytes, 16-byte aligned, of this call alone until it has run
- * Keys never influence a row that does not see them, whatever their bytes.  A key with a value that is not finite makes the whole output of
- * the rows that see it NaN.
+ * Keys never influence a row that does not see them, whatever their bytes.  A key with a value that is not finite makes the output of the
+ * rows that see it NaN, all of it or, where the score is -inf, at least in the dimensions that are not finite.
  *
  * Paged: request r has the tokens query_start_loc[r] .. query_start_loc[r+1]-1 (non-decreasing, [num_reqs + 1]), the last of them at
  * position seq_lens[r] - 1.  A token at position p sees position j if j <= p and, where window_size > 0, j > p - window_size or
