@@ -543,8 +543,9 @@ int dsv4_sparse_latent_attention(const void* q, int64_t q_stride_token, int64_t 
     if (rc != DSV4_OK) return rc;
     if (topk < 0 || topk >= (1LL << 31) - 256) return DSV4_ERR_BAD_SIZE;
     if (num_tokens == 0 || num_heads == 0) return DSV4_OK;
-    if (!lens || !indices) return DSV4_ERR_NULL_POINTER;
-    p.indices = indices, p.indices_stride = indices_stride, p.topk = static_cast<int32_t>(topk), p.lens = lens;
+    if (!lens || (!indices && topk > 0)) return DSV4_ERR_NULL_POINTER;
+    // (lists of no entries have no memory, and none of it is read: any pointer says that this is the form with lists)
+    p.indices = indices ? indices : lens, p.indices_stride = indices_stride, p.topk = static_cast<int32_t>(topk), p.lens = lens;
     return static_cast<int>(launch_latent_attention(p, workspace, static_cast<cudaStream_t>(cuda_stream)));
 }
 

@@ -359,6 +359,98 @@ def test_sparse_lengths_outside_the_list():
 
 
 @gpu
+def test_lists_and_tables_of_no_entries():
+    """Nobody sees a key: rows of zeros."""
+    cache, _, _, q, sink = sparse_case(5, 16, 4, seed=21)
+    for lens in (0, 3):
+        out, lse = run_sparse(cache, torch.empty(5, 0, dtype=torch.int32), torch.full((5,), lens, dtype=torch.int32), q, sink)
+        assert (out == 0).all() and (lse == -math.inf).all()
+    b = Batch([70, 9], [4, 3], 16, 64, seed=22)
+    b.table = b.table[:, :0].contiguous()
+    out, lse = b.run()
+    assert (out == 0).all() and (lse == -math.inf).all()
+    b.cache = b.cache[:0]
+    b.table = torch.zeros(2, 2, dtype=torch.int32)
+    out, lse = b.run()
+    assert (out == 0).all() and (lse == -math.inf).all()
+
+
+def table_of_rows(cache, block_size):
+    """All rows of a small cache at once, in 64 bits."""
+    return key_rows(cache, block_size, range(cache.shape[0] * block_size))
+
+
+@gpu
+@pytest.mark.parametrize("tokens", [57000, 70000])
+def test_sparse_of_very_many_tokens(tokens):
+    """More lengths than shared memory holds while the shares are worked out, and just as many as it does; rows of one head."""
+    g = torch.Generator().manual_seed(tokens)
+    cache = make_cache(4, 16, g)
+    indices = torch.randint(0, 64, (tokens, 3), generator=g, dtype=torch.int32)
+    lens = torch.randint(0, 4, (tokens,), generator=g, dtype=torch.int32)
+    q = torch.randn(tokens, 1, 512, generator=g).to(torch.bfloat16)
+    out, lse = run_sparse(cache, indices, lens, q, torch.zeros(1), 16)
+    rows = table_of_rows(cache, 16)
+    for t in torch.cat([torch.arange(0, tokens, 997), torch.arange(tokens - 5, tokens)]).tolist():
+        check(out[t : t + 1], lse[t : t + 1], [definition(q[t], rows[indices[t, : lens[t]].long()], SCALE, torch.zeros(1))])
+    # the rest against sums over all rows at once, in 32 bits: the module's bound, with scores that are off by d on both sides
+    live = torch.arange(3)[None] < lens[:, None]
+    s = (q[:, 0].float() @ rows.float().t() * SCALE).gather(1, indices.long()).masked_fill(~live, -math.inf)
+    d = (q[:, 0].float().abs() @ rows.float().abs().t()).amax(1) * SCALE * 512 * 2.0 ** -23
+    weights = torch.exp(s) / (1 + torch.exp(s).sum(1, keepdim=True))
+    for start in range(0, tokens, 10000):
+        part = slice(start, start + 10000)
+        keys = rows.float()[indices[part].long()]
+        want, a = (weights[part, :, None] * keys).sum(1), (weights[part, :, None] * keys.abs()).sum(1)
+        bound = (2.0 ** -8 + torch.expm1(4 * d[part])[:, None] + 22 * 2.0 ** -23) * a + 2.0 ** -8 * want.abs() + 2.0 ** -100
+        assert (out[part, 0].float() - want).abs().le(bound).all()
+
+
+@gpu
+def test_very_many_requests():
+    """Starts and lengths of 30000 requests do not fit in shared memory; some bring no token."""
+    g = torch.Generator().manual_seed(30)
+    n, heads = 30000, 2
+    cache = make_cache(4, 16, g)
+    new = torch.randint(0, 3, (n,), generator=g)
+    starts = torch.cat([torch.zeros(1, dtype=torch.int64), new.cumsum(0)]).to(torch.int32)
+    tokens, seq = int(starts[-1]), (new + torch.randint(0, 12, (n,), generator=g)).to(torch.int32)
+    table = torch.randint(0, 4, (n, 1), generator=g, dtype=torch.int32)
+    q = torch.randn(tokens, heads, 512, generator=g).to(torch.bfloat16)
+    lse = torch.zeros(tokens, heads, device=DEV)
+    out = fg.paged_latent_attention(q.to(DEV), cache.to(DEV), table.to(DEV), seq.to(DEV), starts.to(DEV), 16, SCALE, None, 0, None, None, lse).cpu()
+    assert _native.device_error() == 0
+    rows = table_of_rows(cache, 16)
+    lse = lse.cpu()
+    for r in [*range(0, n, 101), n - 2, n - 1]:
+        for i in range(int(new[r])):
+            t, p = int(starts[r]) + i, int(seq[r]) - int(new[r]) + i
+            page = int(table[r, 0]) * 16
+            check(out[t : t + 1], lse[t : t + 1], [definition(q[t], rows[page : page + p + 1], SCALE, None)])
+
+
+@gpu
+def test_a_replayed_graph_follows_lengths_and_tables():
+    """What a captured call was given by its shapes holds for every replay; lengths, starts and pages may change between replays."""
+    b = Batch([900, 40, 300], [1, 1, 1], 64, 64, seed=23)
+    dev = [t.to(DEV) for t in (b.q, b.cache, b.table, torch.tensor(b.seq_lens, dtype=torch.int32), b.starts)]
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        fg.paged_latent_attention(*dev, 64, SCALE)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            out = fg.paged_latent_attention(*dev, 64, SCALE)
+    torch.cuda.synchronize()
+    for lens in ([900, 40, 300], [1, 64, 65], [512, 0, 299], [7, 40, 1]):
+        dev[3].copy_(torch.tensor(lens, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        b.seq_lens = lens
+        want = b.want(sink=False)
+        check(out.cpu(), torch.stack([w[1] for w in want]).float(), want)
+
+
+@gpu
 def test_sparse_equals_paged():
     """The list of a token's positions gives what the block table gives."""
     b = Batch([500, 90], [1, 1], 64, 64, seed=13)
