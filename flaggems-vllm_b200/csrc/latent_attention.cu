@@ -22,10 +22,10 @@
 // over the tiles' numbers of blocks and takes its share, which may begin and end inside a tile.  Pieces of a tile go to a workspace as
 // unnormalised sums and are joined, in a fixed order, by a second small kernel.  Where lists are short, tiles are not cut (see kLeastSplit).
 //
-// What bounds it.  A block takes about 2450 cycles: the products 1700 (a product of 64 rows runs at half the rate of one of 128, which would need 128 KiB for
-// q and 512 columns for O, and leave nothing for S), the softmax 1650, the readers 2100, of which 1000 wait for L2: a warp cannot have loads in flight
-// across its hand-over, and there is no room for records copied ahead.  Tensor pipe 63% active, half of the issue slots used.  Large chunks also run at about
-// 1.6 GHz for power.
+// What bounds it.  In the largest chunk a block takes 2000 to 2100 cycles at the 1.56 GHz that power leaves: the products 1700 of them (a product of 64 rows
+// runs at half the rate of one of 128, which would need 128 KiB for q and 512 columns for O, and leave nothing for S), the rest the way from S to P and back
+// that the order S, O leaves open.  Softmax and readers take 1650 and 2100 beside it, half of the issue slots.  Readers that ask for the next block's values before
+// they convert this one's (and hand over by hardware barriers, which do not wait for loads) change nothing: 3.25 ms both.
 // 1024 tokens x 128 heads over 8192 keys: 3.4 ms (690 TFLOP/s); 61 requests of up to 16384 keys, 64 heads: 158 us; one of 65536 keys, 128 heads: 46 us;
 // a window of 128 tokens, one request: 11.6 us, of which two thirds are the way in (plan, look-up, keys, q: each waits for memory that the one before names) and out.
 // Other forms that were built: blocks of 64 keys in two stages, 6.9 ms; two groups of readers in turn, 4.5; eight softmax warps, 4.1 (this form then 3.9);
