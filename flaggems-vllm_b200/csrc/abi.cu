@@ -481,6 +481,9 @@ int latent_attention_common(LatentAttention& p, const void* q, int64_t q_stride_
     if (num_tokens >= lim || num_heads >= lim || num_blocks >= lim || cache_block_size >= lim) return DSV4_ERR_TOO_LARGE;
     if (num_heads > 0 && num_tokens > (lim - 1) / num_heads) return DSV4_ERR_TOO_LARGE;
     if (num_tokens == 0 || num_heads == 0) return DSV4_OK;
+    // strides that are not used may be anything
+    if (num_tokens == 1) q_stride_token = out_stride_token = lse_stride_token = 0;
+    if (num_heads == 1) q_stride_head = out_stride_head = lse_stride_head = 0;
     if (!q || !out || (num_blocks > 0 && !k_cache) || (!workspace && latent_attention_workspace(num_tokens, num_heads) > 0))
         return DSV4_ERR_NULL_POINTER;
     if (!aligned16(q) || !aligned16(out) || !aligned16(k_cache) || !aligned16(workspace) || q_stride_token % 8 != 0 || q_stride_head % 8 != 0 ||

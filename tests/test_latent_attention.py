@@ -529,6 +529,26 @@ def test_unaligned_arguments_are_refused(what):
 
 
 @gpu
+@pytest.mark.parametrize("tokens,heads", [(1, 12), (5, 1), (1, 1)])
+def test_strides_of_single_tokens_and_heads_are_not_used(tokens, heads):
+    b = Batch([50], [tokens], heads, 64, seed=24)
+    strides = (3 if tokens == 1 else heads * 512, 5 if heads == 1 else 512, 1)
+    q, out = (torch.empty(tokens * heads * 512, dtype=torch.bfloat16, device=DEV).as_strided((tokens, heads, 512), strides) for _ in range(2))
+    q.copy_(b.q)
+    out, lse = b.run(q=q, out=out)
+    check(out, lse, b.want())
+
+
+@gpu
+def test_queries_shared_by_tokens_and_heads():
+    """A broadcast q is read, not written."""
+    b = Batch([90, 40], [3, 2], 20, 64, seed=25)
+    b.q[:] = b.q[:1, :1]
+    out, lse = b.run(q=b.q[0, 0].to(DEV).expand(5, 20, 512))
+    check(out, lse, b.want())
+
+
+@gpu
 def test_overlapping_results_are_refused():
     b = Batch([20], [2], 4, 64, seed=18)
     q = b.q.to(DEV)
