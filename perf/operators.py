@@ -280,20 +280,17 @@ def _plain_sparse(s):
 # ---- the package's calls --------------------------------------------------------------------------------------------------
 
 
-_package = None  # imported at the first call, as a user's program does once
-
-
-def _import():
-    global _package
-    sys.path.insert(0, os.path.abspath("flaggems-vllm_b200"))
+def _package():
+    here = os.path.abspath("flaggems-vllm_b200")
+    if here not in sys.path:
+        sys.path.insert(0, here)
     import flaggems_vllm
 
-    _package = flaggems_vllm
-    return _package
+    return flaggems_vllm
 
 
 def _own(s):
-    fg, case = _package or _import(), s["case"]
+    fg, case = _package(), s["case"]
     if case["kind"] == "norm":
         x_q, scales = fg.fused_add_rmsnorm_quant_fp8(s["x"], s["residual"], s["weight"], EPS, case["group"], case["column_major"], case["pow2"])
         return {"x_q": x_q, "scales": scales, "residual": s["residual"]}
