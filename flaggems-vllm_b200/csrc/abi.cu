@@ -67,6 +67,9 @@ int current_table_staging() {
 // microseconds; 2e8 cycles are about a tenth of a second at B200 clocks.
 std::atomic<long long> g_bulk_wait_cycles{200000000LL};
 
+// Latent attention: tries of a wait (each of up to two microseconds) before the kernel gives up.
+std::atomic<uint32_t> g_attention_wait_tries{kMostWaitTries};
+
 // total >= count * each for count > 0, each >= 0, without the product: sizes come from callers, and one that wraps would let a
 // kernel read far outside the cache.
 bool holds(int64_t total, int64_t count, int64_t each) { return each == 0 ? total >= 0 : total / each >= count; }
@@ -498,6 +501,7 @@ int latent_attention_common(LatentAttention& p, const void* q, int64_t q_stride_
     p.num_tokens = static_cast<int32_t>(num_tokens), p.num_heads = static_cast<int32_t>(num_heads);
     p.block_size = static_cast<uint32_t>(cache_block_size);
     make_fast_divisor(p.block_size, &p.block_mul, &p.block_shift);
+    p.wait_tries = g_attention_wait_tries.load(std::memory_order_relaxed);
     return DSV4_OK;
 }
 }  // namespace
@@ -608,6 +612,12 @@ int dsv4_set_pdl(int mode) {
 int64_t dsv4_set_bulk_wait_cycles(int64_t cycles) {
     const long long previous = g_bulk_wait_cycles.load(std::memory_order_relaxed);
     if (cycles > 0) g_bulk_wait_cycles.store(cycles > 2000000000LL ? 2000000000LL : cycles, std::memory_order_relaxed);
+    return previous;
+}
+
+int64_t dsv4_set_attention_wait_tries(int64_t tries) {
+    const int64_t previous = g_attention_wait_tries.load(std::memory_order_relaxed);
+    if (tries >= 0) g_attention_wait_tries.store(tries > kMostWaitTries ? kMostWaitTries : static_cast<uint32_t>(tries), std::memory_order_relaxed);
     return previous;
 }
 

@@ -105,21 +105,25 @@ __device__ __forceinline__ bool barrier_try(uint64_t* bar, uint32_t parity) {
                  : "memory");
     return done != 0;
 }
-// Bounded: false, and the CTA's other roles told to leave, where the phase does not complete within 2^22 tries, each of which the hardware
-// suspends for up to two microseconds (some seconds in all; a phase takes a few microseconds).
-constexpr uint32_t kTries = 1u << 22;
-__device__ __forceinline__ bool barrier_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
-    for (uint32_t i = 0; i < kTries; ++i) {
+// What bounds a wait: a number of tries (launch parameter), each of which the hardware suspends for up to two microseconds, and the word by which
+// a role that has given up tells the CTA's others to leave.
+struct Limit {
+    volatile int* abort;
+    uint32_t tries;
+};
+// False, and the others told, where the phase does not complete within the limit.  (The default allows some seconds; a phase takes a few microseconds.)
+__device__ __forceinline__ bool barrier_wait(uint64_t* bar, uint32_t parity, const Limit& limit) {
+    for (uint32_t i = 0; i < limit.tries; ++i) {
         if (barrier_try(bar, parity)) return true;
-        if (*abort) return false;
+        if (*limit.abort) return false;
     }
-    *abort = 1;
+    *limit.abort = 1;
     atomicOr(&g_attention_error, 1);
     return false;
 }
 // The same by a whole warp, with one answer.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* abort) {
-    return __all_sync(0xffffffffu, barrier_wait(bar, parity, abort));
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const Limit& limit) {
+    return __all_sync(0xffffffffu, barrier_wait(bar, parity, limit));
 }
 // Between a thread's ordinary writes of shared memory and the products that read them.  It waits for the thread's loads that are under way, too.
 __device__ __forceinline__ void fence_to_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -468,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
     __syncthreads();
     fence_tmem_after();
     const uint32_t tmem = rest.tmem, tmem_scores = tmem + 256;
-    int* abort = &rest.abort;
+    const Limit limit{&rest.abort, p.a.wait_tries};
     Walk w;
     w.at = rest.from, w.end_of_share = &rest.to;
 
@@ -494,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
             for (int block = w.begin; block < w.end; ++block, ++it) {
                 const int buffer = it & 1;
                 const uint32_t parity = (it >> 1) & 1;
-                if (!warp_wait(&rest.s_full[buffer], parity, abort) || !warp_wait(&rest.kv_full[stage], stage_phase, abort)) {
+                if (!warp_wait(&rest.s_full[buffer], parity, limit) || !warp_wait(&rest.kv_full[stage], stage_phase, limit)) {
                     ok = false;
                     break;
                 }
@@ -545,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                     }
                     if (__any_sync(0xffffffffu, correct)) {
                         // O has been written up to the block before this one
-                        if (!warp_wait(&rest.pv_done[buffer ^ 1], ((it - 1) >> 1) & 1, abort)) {
+                        if (!warp_wait(&rest.pv_done[buffer ^ 1], ((it - 1) >> 1) & 1, limit)) {
                             ok = false;
                             break;
                         }
@@ -574,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                     l[r] = add2(l[r], make_float2(s[i], s[i + 1]));
                 }
                 // P of two blocks ago has been read
-                if (it >= 2 && !warp_wait(&rest.pv_done[buffer], ((it >> 1) - 1) & 1, abort)) {
+                if (it >= 2 && !warp_wait(&rest.pv_done[buffer], ((it >> 1) - 1) & 1, limit)) {
                     ok = false;
                     break;
                 }
@@ -629,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                 }
                 continue;
             }
-            if (!warp_wait(&rest.pv_done[(it - 1) & 1], ((it - 1) >> 1) & 1, abort)) {
+            if (!warp_wait(&rest.pv_done[(it - 1) & 1], ((it - 1) >> 1) & 1, limit)) {
                 ok = false;
                 break;
             }
@@ -730,7 +734,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
         uint32_t phase = 1;  // of kv_empty[stage]: the first round finds it "complete"
         for (int it = 0;; ++it) {
             const int entry = it & 1;
-            if (!warp_wait(&rest.look_full[entry], (it >> 1) & 1, abort)) break;
+            if (!warp_wait(&rest.look_full[entry], (it >> 1) & 1, limit)) break;
             const uint64_t exist = rest.exist[entry];
             if (exist >> 63) break;
             const uint32_t valid = static_cast<uint32_t>(exist >> (kWarpKeys * reader)) & 0xfu;
@@ -750,7 +754,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                 if (coded) high[i] = ld_stream16(data + 256 + 16 * sub);
                 rotary[i] = __ldg(reinterpret_cast<const uint2*>(data + kNopeDim + 8 * rotary_sub));
             }
-            if (!warp_wait(&rest.kv_empty[stage], phase, abort)) break;
+            if (!warp_wait(&rest.kv_empty[stage], phase, limit)) break;
             uint32_t none = ~valid;  // keys of this warp that are stored as zeros
             if (mixed) {
                 // Keys that some rows of the tile do not see: those with a value that is not finite are stored as zeros, which the rows that do
@@ -805,8 +809,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
             uint32_t phase = 0;
             const auto product_o = [&](int i, bool first, int tile) {  // O += P V of block i, the one before the last
                 const int buffer = i & 1;
-                if (!barrier_wait(&rest.p_full[buffer], (i >> 1) & 1, abort)) return false;
-                if (first && tile > 0 && !barrier_wait(&rest.o_empty, (tile - 1) & 1, abort)) return false;
+                if (!barrier_wait(&rest.p_full[buffer], (i >> 1) & 1, limit)) return false;
+                if (first && tile > 0 && !barrier_wait(&rest.o_empty, (tile - 1) & 1, limit)) return false;
                 fence_tmem_after();
                 const uint64_t a = operand(base + kOffsetP + buffer * kQueryChunk, 16);
                 const uint64_t b = operand(base + kOffsetKeys + stage_before * kKeyBytes, kKeyChunk);
@@ -827,10 +831,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                 // (q of this tile is on its way while the last product of the one before runs)
                 if (pending && !product_o(it - 1, pending_first, pending_tile)) break;
                 pending = false;
-                if (!barrier_wait(&rest.q_full, tiles & 1, abort)) break;
+                if (!barrier_wait(&rest.q_full, tiles & 1, limit)) break;
                 for (int block = w.begin; block < w.end; ++block, ++it) {
                     const int buffer = it & 1;
-                    ok = barrier_wait(&rest.kv_full[stage], phase, abort);
+                    ok = barrier_wait(&rest.kv_full[stage], phase, limit);
                     if (!ok) break;
                     fence_tmem_after();
                     const uint64_t a = operand(base, 16), b = operand(base + kOffsetKeys + stage * kKeyBytes, 16);
@@ -851,9 +855,9 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                 ++tiles;
             }
             if (ok && pending) product_o(it - 1, pending_first, pending_tile);
-            // nothing of this CTA may be in flight when its memory is given back
+            // nothing of this CTA may be in flight when its memory is given back, whatever the limit of the other waits
             commit_to(&rest.drained);
-            for (uint32_t i = 0; i < kTries && !barrier_try(&rest.drained, 0); ++i) {}
+            for (uint32_t i = 0; i < kMostWaitTries && !barrier_try(&rest.drained, 0); ++i) {}
         }
         __syncwarp();
     } else if (warp == kLookupWarp) {
@@ -893,7 +897,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                     at[i].y = reinterpret_cast<uint64_t>(there ? block_at + codes_from + static_cast<int64_t>(in_block) * kScaleBytes : p.a.q);
                     exist |= static_cast<uint64_t>(__ballot_sync(0xffffffffu, there)) << (32 * i);
                 }
-                ok = warp_wait(&rest.look_empty[entry], ((it >> 1) - 1) & 1, abort);
+                ok = warp_wait(&rest.look_empty[entry], ((it >> 1) - 1) & 1, limit);
                 if (!ok) break;
                 rest.keys[entry][lane] = at[0];
                 if (lane + 32 < kBlockKeys) rest.keys[entry][lane + 32] = at[1];
@@ -903,7 +907,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
             }
         }
         // the end
-        ok = ok && warp_wait(&rest.look_empty[it & 1], ((it >> 1) - 1) & 1, abort);
+        ok = ok && warp_wait(&rest.look_empty[it & 1], ((it >> 1) - 1) & 1, limit);
         if (ok && lane == 0) rest.exist[it & 1] = 1ull << 63, barrier_arrive(&rest.look_full[it & 1]);
     } else {
         // ------------------------------------------------------------------------------------------------ queries
@@ -912,7 +916,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
         for (; w.settle(p); w.step(p)) {
             if (w.begin == w.end) continue;
             const Tile& t = w.tile;
-            if (tiles > 0 && !warp_wait(&rest.q_empty, (tiles - 1) & 1, abort)) break;
+            if (tiles > 0 && !warp_wait(&rest.q_empty, (tiles - 1) & 1, limit)) break;
             // Atoms of eight rows in turn; a row is 64 pieces of 16 bytes, two passes of the warp.  (These warps share their schedulers with the
             // readers: the time that a tile's queries take is that of the instructions for them.)
             const int own = warp - kLookupWarp - 1;
@@ -959,6 +963,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_pieces_kernel(const Laun
     __shared__ float4 part[kJoinWarps][kHeadDim / 4];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     for (int i = tid; i < 2 * kMaxCtas; i += kJoinWarps * 32) pieces[i] = p.pieces[i];
+    if (tid < kMaxCtas) ends[tid] = -1;
     if (tid == 0) most = 0;
     __syncthreads();
     // The tiles: the CTA with the head and the one with the end of each, which follow one another.
@@ -974,7 +979,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_pieces_kernel(const Laun
     if (head) heads[heads_before] = tid;
     if (end) ends[ends_before] = tid;
     __syncthreads();
-    if (tid < tiles) atomicMax(&most, ends[tid] - heads[tid] + 1);
+    // Heads and ends pair up in order, unless a wait of the kernel above ran out: a CTA that gave up has left no record of one or the other.  A head keeps its
+    // end only where that lies behind it, before the next head's CTA or in it, and is of the same tile; a tile without one is left as it was.
+    if (tid < tiles) {
+        const int from = heads[tid], to = ends[tid], most_to = tid + 1 < tiles ? heads[tid + 1] : kMaxCtas - 1;
+        const bool pair = to > from && to <= most_to && pieces[2 * to].x == pieces[2 * from + 1].x && pieces[2 * to].y == pieces[2 * from + 1].y;
+        if (pair) atomicMax(&most, to - from + 1);
+        else ends[tid] = -1;
+    }
     __syncthreads();
     const int each = most <= 4 ? 1 : most <= 16 ? 4 : 16, rows = kJoinWarps / each, turn = warp % each;  // warps for a row, rows at once
     const float c = p.a.scale * kLog2e;
@@ -982,6 +994,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_pieces_kernel(const Laun
     for (int item = blockIdx.x; item < tiles * (kRows / rows); item += kJoinCtas) {
         const int tile = item / (kRows / rows), row = item % (kRows / rows) * rows + warp / each;
         const int first = heads[tile], count = ends[tile] - first + 1;
+        if (ends[tile] < 0) continue;  // (the same for the whole CTA)
         const int4 of = pieces[2 * first + 1];
         const bool live = row < of.z;
         // piece i: that of CTA first + i, where it has one
