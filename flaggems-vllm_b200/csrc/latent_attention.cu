@@ -45,9 +45,12 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kRows = 64, kBlockKeys = 48, kStages = 3;
 constexpr int kSoftmaxWarps = 4, kReaderWarps = 12, kIssuerWarp = kSoftmaxWarps + kReaderWarps, kLookupWarp = kIssuerWarp + 1, kQueryWarps = 2;
 constexpr int kThreads = 32 * (kLookupWarp + 1 + kQueryWarps), kWarpKeys = kBlockKeys / kReaderWarps;
-// Registers a thread: 96 at launch (65536 / 640 threads, in steps of 8), then other shares of the same sum.
-constexpr int kSoftmaxRegisters = 128, kReaderRegisters = 80, kOtherRegisters = 96;
-static_assert(kThreads == 640 && kWarpKeys == 4 && 4 * kSoftmaxRegisters + 12 * kReaderRegisters + 4 * kOtherRegisters <= 20 * 96, "");
+// Registers a thread: 96 at launch (65536 / 640 threads, in steps of 8), then other shares of the same sum for the softmax and the readers.  All threads of a
+// warpgroup (four warps) must execute the same setmaxnreg instruction, so roles that have one are whole warpgroups; the last warpgroup, which has three roles, keeps its 96.
+constexpr int kSoftmaxRegisters = 128, kReaderRegisters = 80, kLaunchRegisters = 96;
+static_assert(kThreads == 640 && kWarpKeys == 4, "");
+static_assert(kSoftmaxWarps * kSoftmaxRegisters + kReaderWarps * kReaderRegisters + (20 - kSoftmaxWarps - kReaderWarps) * kLaunchRegisters <= 20 * kLaunchRegisters, "");
+static_assert(kSoftmaxWarps % 4 == 0 && kReaderWarps % 4 == 0, "whole warpgroups");
 constexpr uint64_t kAllKeys = (1ull << kBlockKeys) - 1;
 constexpr float kMostGrowth = 8.0f;  // log2 of the factor that a row's maximum may have grown by before O is corrected (with 0: 61 requests 209 us, not 155)
 constexpr int kMaxCtas = 148;        // a B200's SMs: one CTA on each (its shared memory allows no second)
@@ -802,7 +805,6 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
         }
     } else if (warp == kIssuerWarp) {
         // ------------------------------------------------------------------------------------------------ products
-        set_registers<kOtherRegisters, false>();
         if (elected()) {
             bool ok = true;
             int it = 0, tiles = 0, stage = 0, stage_before = 0;
@@ -862,7 +864,6 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
         __syncwarp();
     } else if (warp == kLookupWarp) {
         // ------------------------------------------------------------------------------------------------ look-ups
-        set_registers<kOtherRegisters, false>();
         // Keys lane and lane + 32 of each block.  Keys that do not exist are given q as their place, and zeroed when they have been read.
         bool ok = true;
         int it = 0;
@@ -911,7 +912,6 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
         if (ok && lane == 0) rest.exist[it & 1] = 1ull << 63, barrier_arrive(&rest.look_full[it & 1]);
     } else {
         // ------------------------------------------------------------------------------------------------ queries
-        set_registers<kOtherRegisters, false>();
         int tiles = 0;
         for (; w.settle(p); w.step(p)) {
             if (w.begin == w.end) continue;
