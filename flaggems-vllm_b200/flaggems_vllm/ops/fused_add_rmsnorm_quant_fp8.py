@@ -11,7 +11,7 @@ For `x` and `residual` [T, K] in bfloat16 or float16, per row:
 Nothing between z and x_q is rounded to 16 bits, and the mean is formed in 64, so scales and bytes do not depend on an order of summation.
 Returns (x_q [T, K] float8_e4m3fn, scales [T, K / group_size] float32, transposed storage when `column_major_scales`), as
 `per_token_group_quant_fp8` does (src/flaggems_vllm/ops/per_token_group_quant_fp8.py:226-330), whose input this norm would otherwise write.
-`group_size`: 32, 64, 128, 256, or K for one scale per token.  A group with a NaN has a NaN scale.  `residual` must not overlap `x`.
+`group_size`: 32, 64, 128, 256, or K for one scale per token.  A group with a NaN has a NaN scale.  `residual` must not overlap `x` or `weight`.
 """
 from __future__ import annotations
 

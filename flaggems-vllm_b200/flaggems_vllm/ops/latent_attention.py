@@ -15,7 +15,8 @@ A cached row of 512 values, shared by all heads, is key and value at once.  Per 
   entries are skipped.
 
 q is bfloat16 [tokens, heads, 512] with unit inner stride, any number of heads; rows, cache and cache blocks on 16-byte boundaries.  `out`
-(like q, not overlapping it) and `lse` (float32 [tokens, heads]) are written where given; `out` is allocated otherwise, and returned.
+(like q) and `lse` (float32 [tokens, heads]) are written where given; `out` is allocated otherwise, and returned.  Neither may share memory with the
+other or with an argument that is read.
 
 A row that sees no key is zero, with an lse of -inf.  Keys that a row does not see do not influence it, whatever their bytes: pages behind a
 sequence's end, later tokens of a chunk, entries behind `lens`.  A page or slot outside the cache, and a position behind the block table, is

@@ -27,6 +27,7 @@ extern "C" {
 #define DSV4_ERR_MISALIGNED (-3)   /* a pointer or stride is not aligned as the entry point requires */
 #define DSV4_ERR_BAD_VARIANT (-4)  /* unknown kernel variant id */
 #define DSV4_ERR_TOO_LARGE (-5)    /* size exceeds what the entry point supports */
+#define DSV4_ERR_OVERLAP (-6)      /* a result shares memory with another argument */
 
 /* Layout constants of one cached token (reference:
  * src/flaggems_vllm/ops/fused_deepseek_v4_qnorm_rope_kv_rope_quant_insert.py:35-43). */
@@ -332,7 +333,7 @@ int dsv4_fused_indexer_q_rope_quant(const int64_t* positions, const void* index_
  *   out = e4m3(y / scale), contiguous [num_rows, num_cols] bytes; a group with a NaN has a NaN scale
  * x, residual: bf16 (is_fp16 = 0) or fp16 (1), row strides in elements, unit inner stride; weight [num_cols] of that type or, with
  * weight_is_fp32, fp32.  group_size: 32, 64, 128, 256, or num_cols (one scale per row); num_cols a multiple of it and of 8, at most 32768.
- * All rows on 16-byte boundaries.  residual must not overlap x or out.
+ * All rows on 16-byte boundaries.  residual, out and scales must share no memory with each other, x or weight (DSV4_ERR_OVERLAP).
  */
 int dsv4_fused_add_rmsnorm_quant_fp8(const void* x, int64_t x_row_stride, void* residual, int64_t residual_row_stride, const void* weight,
                                      void* out, float* scales, int64_t scale_stride_row, int64_t scale_stride_group, int64_t num_rows,
@@ -345,10 +346,11 @@ int dsv4_fused_add_rmsnorm_quant_fp8(const void* x, int64_t x_row_stride, void* 
  *   s_j = softmax_scale * q . k_j,  out = sum_j e^(s_j) k_j / (sum_j e^(s_j) + e^(sink[head])),  lse = ln sum_j e^(s_j)
  * over the keys that the token sees; a row that sees none, or none with a score above -inf, has out = 0 and lse = -inf.  The e^(sink)
  * term is there where attn_sink is not NULL; lse does not contain it, and is only written where it is not NULL.
- *   q, out     bf16 [num_tokens, num_heads, 512], strides in elements (multiples of 8), 16-byte aligned, not overlapping
+ *   q, out     bf16 [num_tokens, num_heads, 512], strides in elements (multiples of 8), 16-byte aligned
  *   lse        fp32, strides in elements
  *   k_cache    as written by the prologue, num_blocks blocks; base and block stride on 16-byte boundaries
  *   workspace  dsv4_latent_attention_workspace_bytes(...) bytes, 16-byte aligned, of this call alone until it has run
+ * out and lse must share no memory with each other or with an argument that is read (DSV4_ERR_OVERLAP).
  * Keys never influence a row that does not see them, whatever their bytes.  A key with a value that is not finite makes the output of the
  * rows that see it NaN, all of it or, where the score is -inf, at least in the dimensions that are not finite.
  *
