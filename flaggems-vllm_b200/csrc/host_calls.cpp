@@ -25,6 +25,7 @@
 
 #include "../../include/dsv4_prologue.h"
 #include "current_device.h"
+#include "memory_regions.h"
 
 namespace {
 
@@ -104,18 +105,13 @@ struct Arguments {
 bool is(const Tensor& t, ScalarType type) { return t.scalar_type() == type; }
 bool on(const Tensor& t, const Tensor& first) { return t.is_cuda() && t.get_device() == first.get_device(); }
 
-// The bytes that a tensor's elements lie in: [first, second).
-std::pair<const uint8_t*, const uint8_t*> extent(const Tensor& t) {
-    const auto* at = static_cast<const uint8_t*>(t.data_ptr());
-    int64_t last = 0;
-    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-    return {at, at + (last + 1) * static_cast<int64_t>(t.element_size())};
+// Whether two tensors that are not empty, the last dimension of unit stride, share no memory (flaggems_vllm/utils/memory.py decides the same way).
+dsv4::Region region_of(const Tensor& t) {
+    const int64_t size = static_cast<int64_t>(t.element_size()), last = t.dim() - 1;
+    const auto outer = [&](int64_t d) { return d < last ? dsv4::Region::Dimension{t.size(d), t.stride(d) * size} : dsv4::Region::Dimension{1, 0}; };
+    return dsv4::Region(t.data_ptr(), t.size(last) * size, {outer(0), outer(1)});
 }
-// Whether two tensors that are not empty lie in ranges of memory apart from each other.
-bool apart(const Tensor& a, const Tensor& b) {
-    const auto x = extent(a), y = extent(b);
-    return x.second <= y.first || y.second <= x.first;
-}
+bool apart(const Tensor& a, const Tensor& b) { return dsv4::regions_apart(region_of(a), region_of(b)); }
 // Whether no two elements of [tokens, heads] or [tokens, heads, row], the last unit stride, share memory: one of the two outer strides spans
 // the other dimension's rows.
 bool rows_apart(const Tensor& t) {

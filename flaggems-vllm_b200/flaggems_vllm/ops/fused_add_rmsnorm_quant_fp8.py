@@ -20,6 +20,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _native
+from ..utils.memory import apart
 
 _call = None  # the native front end, looked up once
 
@@ -56,13 +57,8 @@ def fused_add_rmsnorm_quant_fp8(
     assert weight.dtype in (x.dtype, torch.float32), "weight: float32 or the type of x"
     assert weight.device == x.device, "all tensors must be on the same device"
     assert rows <= 1 or (x.stride(0) >= cols and (residual is None or residual.stride(0) >= cols)), "rows must not overlap"
-    assert residual is None or rows == 0 or _apart(x, residual), "residual must not overlap x"
+    assert residual is None or rows == 0 or apart(x, residual), "residual must not overlap x"
     _native.refuse()
-
-
-def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
-    ends = [(t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()) for t in (a, b)]
-    return ends[0][1] <= ends[1][0] or ends[1][1] <= ends[0][0]
 
 
 __all__ = ["fused_add_rmsnorm_quant_fp8"]

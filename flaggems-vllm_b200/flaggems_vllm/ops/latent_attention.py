@@ -32,6 +32,7 @@ from typing import Optional
 import torch
 
 from .. import _native
+from ..utils.memory import apart, rows_apart
 
 HEAD_DIM, TOKEN_BYTES = 512, 584
 
@@ -118,19 +119,8 @@ def _check(q, k_cache, cache_block_size, softmax_scale, attn_sink, out, lse):
     if lse is not None:
         assert lse.dtype == torch.float32 and lse.shape == (tokens, heads), "lse: float32 [tokens, heads]"
     if tokens and heads:
-        assert out is None or (_apart(out, q) and _rows_apart(out)), "out must not overlap q or itself"
-        assert lse is None or _rows_apart(lse), "lse must not overlap itself"
-
-
-def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
-    ends = [(t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()) for t in (a, b)]
-    return ends[0][1] <= ends[1][0] or ends[1][1] <= ends[0][0]
-
-
-def _rows_apart(t: torch.Tensor) -> bool:
-    row = t.shape[2] if t.dim() == 3 else 1
-    (n0, n1), (s0, s1) = t.shape[:2], t.stride()[:2]
-    return (n1 == 1 or s1 >= row) and (n0 == 1 or s0 >= row) and (n0 == 1 or n1 == 1 or s0 >= (n1 - 1) * s1 + row or s1 >= (n0 - 1) * s0 + row)
+        assert out is None or (apart(out, q) and rows_apart(out)), "out must not overlap q or itself"
+        assert lse is None or rows_apart(lse), "lse must not overlap itself"
 
 
 __all__ = ["paged_latent_attention", "sparse_latent_attention"]

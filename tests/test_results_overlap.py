@@ -133,6 +133,46 @@ def test_regions_against_their_bytes(regions):
     assert regions([1000, 1 << 40, far, far, 1, 0, 1, 0], [1000, 0, 1, 0, 1, 0, 1, 0]) and not regions([1000, 1 << 40, far, far, 1, 0, 1, 0], [1000 + far, 4, 1, 0, 1, 0, 1, 0])
 
 
+def test_tensors_against_their_elements():
+    """The assertions' form of the same decision: never apart where an element is shared, apart for disjoint columns of one buffer."""
+    import random
+
+    from flaggems_vllm.utils.memory import apart
+
+    rng, buffer = random.Random(2), torch.arange(4000, dtype=torch.int16)
+
+    def some():
+        return buffer.as_strided((rng.randrange(1, 4), rng.randrange(1, 4), rng.randrange(1, 6)), (rng.choice([1, 5, 6, 8, 12, 24, 48]), rng.choice([1, 5, 6, 8, 12, 24]), 1), rng.randrange(60))
+
+    for _ in range(5000):
+        a, b = some(), some()
+        assert not (apart(a, b) and set(a.flatten().tolist()) & set(b.flatten().tolist())), (a.stride(), a.shape, b.stride(), b.shape)
+    wide = buffer.view(10, 20, 20)
+    assert apart(wide[:, :8], wide[:, 8:]) and apart(wide[..., :12], wide[..., 12:]) and apart(wide[:, 3:7, 5:9], wide[:, 2:9, 9:14])
+    assert not apart(wide[:, :9], wide[:, 8:]) and not apart(wide[..., :13], wide[..., 12:])
+
+
+@pytest.mark.gpu
+def test_disjoint_parts_of_one_buffer_are_taken():
+    """q and out, x and residual as columns of one buffer: what a call with tensors of their own gives."""
+    g = torch.Generator().manual_seed(1)
+    q = torch.randn(5, 6, 512, generator=g).to(torch.bfloat16).to("cuda:0")
+    cache = torch.randint(0, 120, (3, 64 * 584), generator=g, dtype=torch.uint8).to("cuda:0")
+    indices = torch.randint(0, 3 * 64, (5, 40), generator=g, dtype=torch.int32).to("cuda:0")
+    lens = torch.full((5,), 40, dtype=torch.int32, device="cuda:0")
+    want = fg.sparse_latent_attention(q, cache, indices, lens, 64, 0.05)
+    for wide, (a, b) in ((torch.zeros(5, 6, 1024, dtype=torch.bfloat16, device="cuda:0"), (lambda t: t[..., :512], lambda t: t[..., 512:])),
+                         (torch.zeros(5, 12, 512, dtype=torch.bfloat16, device="cuda:0"), (lambda t: t[:, 6:], lambda t: t[:, :6]))):
+        a(wide).copy_(q)
+        assert torch.equal(fg.sparse_latent_attention(a(wide), cache, indices, lens, 64, 0.05, None, b(wide)), want) and torch.equal(a(wide), q)
+    x, residual = (torch.randn(9, 640, generator=g).to(torch.bfloat16).to("cuda:0") for _ in range(2))
+    wide = torch.cat([x, residual], 1)
+    weight = torch.ones(640, dtype=torch.bfloat16, device="cuda:0")
+    want = fg.fused_add_rmsnorm_quant_fp8(x, residual, weight, 1e-6)
+    got = fg.fused_add_rmsnorm_quant_fp8(wide[:, :640], wide[:, 640:], weight, 1e-6)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want)) and torch.equal(wide, torch.cat([x, residual], 1))
+
+
 @pytest.mark.gpu
 def test_overlapping_lse_and_cache_are_refused():
     q = torch.zeros(2, 4, 512, dtype=torch.bfloat16, device="cuda:0")
@@ -147,3 +187,39 @@ def test_overlapping_lse_and_cache_are_refused():
     weights = torch.ones(512, dtype=torch.bfloat16, device="cuda:0")
     with pytest.raises(_native.Dsv4Error, match="overlap"):
         fg.fused_add_rmsnorm_quant_fp8(torch.zeros(1, 512, dtype=torch.bfloat16, device="cuda:0"), weights.view(1, 512), weights, 1e-6)
+
+
+@no_gpu
+def test_front_ends_and_assertions_agree_on_parts_of_one_buffer(monkeypatch):
+    """Native front end and Python assertions on out beside q, and residual beside x, in one buffer that is no memory."""
+    from test_attention_operator_checks import OPS, accepts
+    from test_host_checks_agree import BF16, Spec
+
+    monkeypatch.setattr(torch.cuda, "_lazy_init", lambda: None)
+
+    class At(Spec):
+        def __init__(self, offset, *args, **kwargs):
+            super().__init__(*args, **kwargs)
+            self.offset = offset
+
+        def make(self, keep):
+            from test_attention_operator_checks import _capsule
+
+            super().make(keep)
+            keep[-1].data = (1 << 32) + self.offset
+            return torch.utils.dlpack.from_dlpack(_capsule(keep[-1]))
+
+    for name, index in (("paged", 10), ("sparse", 7)):
+        op, args, _ = OPS[name]
+        taken = 0
+        for token, head, offset in ((4096, 1024, 1024), (4096, 1024, 1008), (4096, 512, 4096), (2048, 512, 4096), (4096, 1024, 1040), (4608, 1024, 1024), (4096, 512, 2048), (2064, 512, 4096)):
+            changed = list(args)
+            changed[0], changed[index] = At(0, BF16, 6, 4, 512, strides=(token, head, 1)), At(offset, BF16, 6, 4, 512, strides=(token, head, 1))
+            native, python = accepts(op, tuple(changed), None, True, monkeypatch), accepts(op, tuple(changed), None, False, monkeypatch)
+            assert native[0] == python[0], (name, token, head, offset, native, python)
+            taken += native[0]
+        assert taken == 2
+    op, args, _ = OPS["norm"]
+    for pitch, offset, fine in ((1024, 1024, True), (1016, 1024, False), (1024, 1008, False), (1024, 1040, False), (1040, 1040, True), (4096, 4096, True)):
+        changed = (At(0, BF16, 6, 512, strides=(pitch, 1)), At(offset, BF16, 6, 512, strides=(pitch, 1))) + args[2:]
+        assert accepts(op, changed, None, True, monkeypatch)[0] == accepts(op, changed, None, False, monkeypatch)[0] == fine, (pitch, offset)
