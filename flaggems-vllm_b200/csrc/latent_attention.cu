@@ -259,8 +259,8 @@ __device__ __forceinline__ Tile tile_at(const Tiles& p, const Lists& lists, int 
         t.count = 1;
         t.keys = min(max(lists.lens[token], 0), p.a.topk);
     } else {
-        const int end = min(lists.starts[request + 1], p.a.num_tokens);
-        t.count = min(p.tokens_per_tile, end - token);
+        const int end = lists.starts[request + 1];  // (it may lie behind the last row of q: positions count from it all the same)
+        t.count = min(p.tokens_per_tile, min(end, p.a.num_tokens) - token);
         t.position = max(lists.lens[request], 0) - end + token;
         t.low = p.a.window > 0 && t.position >= p.a.window ? t.position - p.a.window + 1 : 0;
         t.first = min(min(t.low, p.a.first), p.a.capacity);

@@ -9,8 +9,8 @@ A cached row of 512 values, shared by all heads, is key and value at once.  Per 
 
 * `paged_latent_attention`: requests with a row of `block_table` each.  Request r has the tokens query_start_loc[r] ..
   query_start_loc[r + 1] - 1 of q, the last of them at position seq_lens[r] - 1 of its sequence, whose keys are in the cache already: a
-  chunk of a prompt, or one token per request.  Position p sees j <= p and, with a window, of those j > p - window_size or
-  j < num_first_tokens.
+  chunk of a prompt, or one token per request.  Of these tokens those are computed that q has rows for.  Position p sees j <= p and, with a
+  window, of those j > p - window_size or j < num_first_tokens.
 * `sparse_latent_attention`: token t sees the cache slots indices[t, : lens[t]], as `compute_global_topk_indices_and_lens` makes them; negative
   entries are skipped.
 

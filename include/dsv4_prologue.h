@@ -355,7 +355,7 @@ int dsv4_fused_add_rmsnorm_quant_fp8(const void* x, int64_t x_row_stride, void* 
  * rows that see it NaN, all of it or, where the score is -inf, at least in the dimensions that are not finite.
  *
  * Paged: request r has the tokens query_start_loc[r] .. query_start_loc[r+1]-1 (non-decreasing, [num_reqs + 1]), the last of them at
- * position seq_lens[r] - 1.  A token at position p sees position j if j <= p and, where window_size > 0, j > p - window_size or
+ * position seq_lens[r] - 1, also where it lies behind the num_tokens rows of q.  A token at position p sees position j if j <= p and, where window_size > 0, j > p - window_size or
  * j < num_first_tokens; a page that is outside 0 .. num_blocks-1, or beyond max_blocks_per_seq, is seen by no token.  Rows of q behind the
  * last request's are left as they are in out and lse.
  * Sparse: token t sees the slots indices[t, 0 .. lens[t]-1] (block * cache_block_size + offset); negative ones and ones outside
