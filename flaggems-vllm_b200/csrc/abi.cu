@@ -486,7 +486,8 @@ int latent_attention_common(LatentAttention& p, const void* q, int64_t q_stride_
     const int64_t lim = 1LL << 31;
     if (num_tokens < 0 || num_heads < 0 || num_blocks < 0 || cache_block_size <= 0) return DSV4_ERR_BAD_SIZE;
     if (!holds(kv_block_stride_bytes, cache_block_size, kTokenDataBytes + kScaleBytes)) return DSV4_ERR_BAD_SIZE;
-    if (!(softmax_scale > 0.0f) || softmax_scale > 3.4e38f) return DSV4_ERR_BAD_SIZE;
+    // (the kernels' exponentials are powers of two: log2(e) times the scale has to be a number too)
+    if (!(softmax_scale > 0.0f && softmax_scale * 1.4426950408889634f <= 3.402823466e38f)) return DSV4_ERR_BAD_SIZE;
     if (num_tokens >= lim || num_heads >= lim || num_blocks >= lim || cache_block_size >= lim) return DSV4_ERR_TOO_LARGE;
     if (num_heads > 0 && num_tokens > (lim - 1) / num_heads) return DSV4_ERR_TOO_LARGE;
     if (num_tokens == 0 || num_heads == 0) return DSV4_OK;

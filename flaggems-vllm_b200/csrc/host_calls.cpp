@@ -647,7 +647,7 @@ void require_attention(Arguments& a, const AttentionTensors& t) {
     REQUIRE(t.q->is_cuda() && t.q->dim() == 3 && t.q->size(2) == 512 && is(*t.q, at::kBFloat16) && t.q->stride(2) == 1);
     REQUIRE(is(*t.cache, at::kByte) && t.cache->dim() == 2 && t.cache->stride(1) == 1 && t.block > 0 && t.cache->size(1) / 584 >= t.block);
     REQUIRE(t.cache->size(0) <= 1 || t.cache->stride(0) >= t.cache->size(1));
-    REQUIRE(t.scale > 0.0f && t.scale < INFINITY);
+    REQUIRE(t.scale > 0.0f && t.scale * 1.4426950408889634f < INFINITY);
     REQUIRE(on(*t.cache, *t.q));
     if (!a.ok) return;
     const int64_t tokens = t.q->size(0), heads = t.q->size(1);

@@ -26,7 +26,6 @@ they are in `out` and `lse` (in an `out` that was allocated here they are not de
 """
 from __future__ import annotations
 
-import math
 from typing import Optional
 
 import torch
@@ -107,8 +106,8 @@ def _check(q, k_cache, cache_block_size, softmax_scale, attn_sink, out, lse):
     assert k_cache.dtype == torch.uint8 and k_cache.dim() == 2 and k_cache.stride(1) == 1, "k_cache: uint8 [blocks, bytes]"
     assert int(cache_block_size) > 0 and k_cache.shape[1] // TOKEN_BYTES >= int(cache_block_size), "a cache block holds cache_block_size tokens of 584 bytes"
     assert k_cache.shape[0] <= 1 or k_cache.stride(0) >= k_cache.shape[1], "cache blocks must not overlap"
-    scale = torch.tensor(float(softmax_scale), dtype=torch.float32).item()
-    assert math.isfinite(scale) and scale > 0, "a positive softmax_scale"
+    scale = torch.tensor(float(softmax_scale), dtype=torch.float32)
+    assert scale > 0 and torch.isfinite(scale * 1.4426950408889634), "a positive softmax_scale, and in 32 bits a number also when it is divided by ln 2"
     tokens, heads = q.shape[:2]
     for t in (k_cache, attn_sink, out, lse):
         assert t is None or t.device == q.device, "all tensors must be on the same device"

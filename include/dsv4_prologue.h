@@ -349,6 +349,7 @@ int dsv4_fused_add_rmsnorm_quant_fp8(const void* x, int64_t x_row_stride, void* 
  *   q, out     bf16 [num_tokens, num_heads, 512], strides in elements (multiples of 8), 16-byte aligned
  *   lse        fp32, strides in elements
  *   k_cache    as written by the prologue, num_blocks blocks; base and block stride on 16-byte boundaries
+ *   softmax_scale  positive, at most 2.3e38
  *   workspace  dsv4_latent_attention_workspace_bytes(...) bytes, 16-byte aligned, of this call alone until it has run
  * out and lse must share no memory with each other or with an argument that is read (DSV4_ERR_OVERLAP).
  * Keys never influence a row that does not see them, whatever their bytes.  A key with a value that is not finite makes the output of the
