@@ -11,6 +11,7 @@ import torch
 
 import flaggems_vllm as fg
 from flaggems_vllm import _native, build
+from test_latent_attention import make_cache
 
 i64, f32, ptr = ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
 OVERLAP, STEP = -6, 1 << 32
@@ -160,11 +161,14 @@ def test_disjoint_parts_of_one_buffer_are_taken():
     cache = torch.randint(0, 120, (3, 64 * 584), generator=g, dtype=torch.uint8).to("cuda:0")
     indices = torch.randint(0, 3 * 64, (5, 40), generator=g, dtype=torch.int32).to("cuda:0")
     lens = torch.full((5,), 40, dtype=torch.int32, device="cuda:0")
-    want = fg.sparse_latent_attention(q, cache, indices, lens, 64, 0.05)
-    for wide, (a, b) in ((torch.zeros(5, 6, 1024, dtype=torch.bfloat16, device="cuda:0"), (lambda t: t[..., :512], lambda t: t[..., 512:])),
-                         (torch.zeros(5, 12, 512, dtype=torch.bfloat16, device="cuda:0"), (lambda t: t[:, 6:], lambda t: t[:, :6]))):
-        a(wide).copy_(q)
-        assert torch.equal(fg.sparse_latent_attention(a(wide), cache, indices, lens, 64, 0.05, None, b(wide)), want) and torch.equal(a(wide), q)
+    bits = lambda t: t.view(torch.int16)  # noqa: E731  (any bytes are a cache: rows may be NaN)
+    for cache in (cache, make_cache(3, 64, g).to("cuda:0")):
+        want = fg.sparse_latent_attention(q, cache, indices, lens, 64, 0.05)
+        for wide, (a, b) in ((torch.zeros(5, 6, 1024, dtype=torch.bfloat16, device="cuda:0"), (lambda t: t[..., :512], lambda t: t[..., 512:])),
+                             (torch.zeros(5, 12, 512, dtype=torch.bfloat16, device="cuda:0"), (lambda t: t[:, 6:], lambda t: t[:, :6]))):
+            a(wide).copy_(q)
+            assert torch.equal(bits(fg.sparse_latent_attention(a(wide), cache, indices, lens, 64, 0.05, None, b(wide))), bits(want)) and torch.equal(a(wide), q)
+    assert torch.isfinite(want).all()
     x, residual = (torch.randn(9, 640, generator=g).to(torch.bfloat16).to("cuda:0") for _ in range(2))
     wide = torch.cat([x, residual], 1)
     weight = torch.ones(640, dtype=torch.bfloat16, device="cuda:0")
