@@ -68,8 +68,8 @@ int current_table_staging() {
 // microseconds; 2e8 cycles are about a tenth of a second at B200 clocks.
 std::atomic<long long> g_bulk_wait_cycles{200000000LL};
 
-// Latent attention: tries of a wait (each of up to two microseconds) before the kernel gives up.
-std::atomic<uint32_t> g_attention_wait_tries{kMostWaitTries};
+// Latent attention: tries of a wait behind the first (each of up to two microseconds) before the kernel gives up.
+std::atomic<uint32_t> g_attention_wait_retries{kMostWaitRetries};
 
 // total >= count * each for count > 0, each >= 0, without the product: sizes come from callers, and one that wraps would let a
 // kernel read far outside the cache.
@@ -508,7 +508,7 @@ int latent_attention_common(LatentAttention& p, const void* q, int64_t q_stride_
     p.num_tokens = static_cast<int32_t>(num_tokens), p.num_heads = static_cast<int32_t>(num_heads);
     p.block_size = static_cast<uint32_t>(cache_block_size);
     make_fast_divisor(p.block_size, &p.block_mul, &p.block_shift);
-    p.wait_tries = g_attention_wait_tries.load(std::memory_order_relaxed);
+    p.wait_retries = g_attention_wait_retries.load(std::memory_order_relaxed);
     return DSV4_OK;
 }
 
@@ -637,9 +637,9 @@ int64_t dsv4_set_bulk_wait_cycles(int64_t cycles) {
     return previous;
 }
 
-int64_t dsv4_set_attention_wait_tries(int64_t tries) {
-    const int64_t previous = g_attention_wait_tries.load(std::memory_order_relaxed);
-    if (tries >= 0) g_attention_wait_tries.store(tries > kMostWaitTries ? kMostWaitTries : static_cast<uint32_t>(tries), std::memory_order_relaxed);
+int64_t dsv4_set_attention_wait_retries(int64_t retries) {
+    const int64_t previous = g_attention_wait_retries.load(std::memory_order_relaxed);
+    if (retries >= 0) g_attention_wait_retries.store(retries > kMostWaitRetries ? kMostWaitRetries : static_cast<uint32_t>(retries), std::memory_order_relaxed);
     return previous;
 }
 

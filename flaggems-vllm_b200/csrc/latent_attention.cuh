@@ -28,10 +28,10 @@ struct LatentAttention {
     int32_t capacity;       // positions that a row of the block table has pages for
     int32_t num_blocks;
     uint32_t block_size, block_mul, block_shift;
-    uint32_t wait_tries;  // of a wait inside the kernel before it gives up
+    uint32_t wait_retries;  // of a wait inside the kernel, behind the first try, before it gives up
 };
 
-constexpr uint32_t kMostWaitTries = 1u << 22;  // the default: of up to two microseconds each, some seconds in all
+constexpr uint32_t kMostWaitRetries = 1u << 22;  // the default: of up to two microseconds each, some seconds in all
 
 size_t latent_attention_workspace(int64_t num_tokens, int64_t num_heads);
 cudaError_t launch_latent_attention(const LatentAttention& p, void* workspace, cudaStream_t stream);

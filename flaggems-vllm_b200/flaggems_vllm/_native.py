@@ -40,7 +40,7 @@ EXPORTS = (
     "dsv4_set_variant",
     "dsv4_get_variant",
     "dsv4_set_bulk_wait_cycles",
-    "dsv4_set_attention_wait_tries",
+    "dsv4_set_attention_wait_retries",
     "dsv4_bulk_wait_selftest",
     "dsv4_set_pdl",
     "dsv4_set_table_staging",
@@ -93,8 +93,8 @@ def lib() -> ctypes.CDLL:
     L.dsv4_set_pdl.restype = i32
     L.dsv4_set_bulk_wait_cycles.argtypes = [i64]
     L.dsv4_set_bulk_wait_cycles.restype = i64
-    L.dsv4_set_attention_wait_tries.argtypes = [i64]
-    L.dsv4_set_attention_wait_tries.restype = i64
+    L.dsv4_set_attention_wait_retries.argtypes = [i64]
+    L.dsv4_set_attention_wait_retries.restype = i64
     L.dsv4_bulk_wait_selftest.argtypes = [vp, vp, vp, vp, vp, vp, f32, i64, i64, i64, i64, i64, i64, vp]
     L.dsv4_bulk_wait_selftest.restype = i32
     L.dsv4_set_table_staging.argtypes = [i32]

@@ -398,12 +398,12 @@ int dsv4_get_variant(void);
  * dsv4_device_error at its next synchronisation point.  Returns the previous limit. */
 int64_t dsv4_set_bulk_wait_cycles(int64_t cycles);
 
-/* Latent attention only.  Every wait of that kernel is bounded by a number of tries, each of which the hardware suspends for up to two microseconds
- * (default 2^22, some seconds in all; larger values are clamped to it, negative ones only read the setting; with 0 every wait gives up at once, which
- * test suites use).  After that the CTA's roles leave their loops, the products it has issued run to their end, bit 1 of the device error word is set,
- * and the call's results are incomplete: rows may be missing or wrong.  The entry points still return 0 in that case: a caller reads
- * dsv4_device_error at a synchronisation point.  The setting is that of the launch, a captured call keeps it.  Returns the previous limit. */
-int64_t dsv4_set_attention_wait_tries(int64_t tries);
+/* Latent attention only.  Every wait of that kernel is bounded: a first try and `retries` more, each of which the hardware suspends for up to two
+ * microseconds (default 2^22, some seconds in all; larger values are clamped to it, negative ones only read the setting).  After that the CTA's roles leave
+ * their loops, the products it has issued run to their end, bit 1 of the device error word is set, and the call's results are incomplete: rows may be
+ * missing or wrong.  The entry points still return 0 in that case: a caller reads dsv4_device_error at a synchronisation point.  The setting is
+ * that of the launch, a captured call keeps it.  Returns the previous limit. */
+int64_t dsv4_set_attention_wait_retries(int64_t retries);
 
 /* Self-test of the bulk variant's give-up path, for test suites; not an operator.  Same arguments and effects as
  * dsv4_qnorm_rope_kv_insert on the bulk variant, except that the loader of tile `short_tile` (tiles are 16 rows:

@@ -1,9 +1,9 @@
 """Waits of the latent attention that run out (csrc/latent_attention.cu), without faulting or hanging anything.
 
-Every wait of that kernel has a limit, and the limit is a setting.  With 0 every wait gives up at once; with a few tries, of up to two microseconds
-each, some CTAs get further than others, so pieces of tiles are missing when the kernel behind joins them.  What must then happen: both kernels
-return by themselves, bit 1 of the device error word is set and cleared by the read, memory behind the results stays, and the next ordinary call
-gives what it gave before, bit for bit."""
+Every wait of that kernel has a limit, and the limit is a setting: how often a try, of up to two microseconds, is made again.  With 0 to 12 the calls below, which
+take 20 us and more, do not get through: some CTAs get further than others, so pieces of tiles are missing when the kernel behind joins them.
+What must then happen: both kernels return by themselves, bit 1 of the device error word is set and cleared by the read, memory beside the
+results stays, and the next ordinary call gives what it gave before, bit for bit."""
 from __future__ import annotations
 
 import pytest
@@ -18,14 +18,14 @@ DEFAULT = 1 << 22
 
 def test_limit_round_trip():
     lib = _native.lib()
-    assert lib.dsv4_set_attention_wait_tries(-1) == DEFAULT  # only reads
+    assert lib.dsv4_set_attention_wait_retries(-1) == DEFAULT  # only reads
     try:
-        assert lib.dsv4_set_attention_wait_tries(0) == DEFAULT
-        assert lib.dsv4_set_attention_wait_tries(1 << 40) == 0
-        assert lib.dsv4_set_attention_wait_tries(7) == DEFAULT  # clamped
+        assert lib.dsv4_set_attention_wait_retries(0) == DEFAULT
+        assert lib.dsv4_set_attention_wait_retries(1 << 40) == 0
+        assert lib.dsv4_set_attention_wait_retries(7) == DEFAULT  # clamped
     finally:
-        assert lib.dsv4_set_attention_wait_tries(DEFAULT) == 7
-    assert lib.dsv4_set_attention_wait_tries(-1) == DEFAULT
+        assert lib.dsv4_set_attention_wait_retries(DEFAULT) == 7
+    assert lib.dsv4_set_attention_wait_retries(-1) == DEFAULT
 
 
 def _calls():
@@ -52,19 +52,21 @@ def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(name):
     torch.cuda.synchronize()
     want = out.clone()
     assert _native.device_error() == 0
+    reported = 0
     for tries in (0, 1, 2, 3, 4, 6, 8, 12, 0):
-        assert lib.dsv4_set_attention_wait_tries(tries) == DEFAULT
+        assert lib.dsv4_set_attention_wait_retries(tries) == DEFAULT
         try:
             call(out)
             torch.cuda.synchronize()  # returns: the kernels ended by themselves
         finally:
-            assert lib.dsv4_set_attention_wait_tries(DEFAULT) == tries
+            assert lib.dsv4_set_attention_wait_retries(DEFAULT) == tries
         error = _native.device_error()
-        assert error == 2 if tries == 0 else error in (0, 2)
-        assert error == 2 or torch.equal(out, want)
+        assert error == 2 or (error == 0 and torch.equal(out, want))
+        reported += error == 2
         assert _native.device_error() == 0, "reading the error word clears it"
         assert (holder[0] == 7).all() and (holder[-1] == 7).all()
         out.fill_(3.0)
         call(out)
         torch.cuda.synchronize()
         assert _native.device_error() == 0 and torch.equal(out, want)
+    assert reported > 0, "none of the waits ran out"
