@@ -470,7 +470,7 @@ int dsv4_fused_add_rmsnorm_quant_fp8(const void* x, int64_t x_row_stride, void* 
     const Region read(x, 2 * num_cols, {{num_rows, 2 * x_row_stride}}), weights(weight, (weight_is_fp32 ? 4 : 2) * num_cols),
         sums(residual, 2 * num_cols, {{num_rows, 2 * residual_row_stride}}), bytes(out, num_rows * num_cols),
         factors(scales, 4, {{num_rows, 4 * scale_stride_row}, {num_cols / group_size, 4 * scale_stride_group}});
-    if (!apart_from_all(sums, {read, weights, bytes, factors}) || !apart_from_all(bytes, {read, weights, factors}) || !apart_from_all(factors, {read, weights}))
+    if (!apart_from_all(sums, {&read, &weights, &bytes, &factors}) || !apart_from_all(bytes, {&read, &weights, &factors}) || !apart_from_all(factors, {&read, &weights}))
         return DSV4_ERR_OVERLAP;
     return static_cast<int>(launch_add_rmsnorm_quant(x, x_row_stride, residual, residual_row_stride, weight, out, scales, scale_stride_row,
                                                      scale_stride_group, num_rows, num_cols, group_size, eps, is_fp16 ? 1 : 0,
@@ -513,14 +513,14 @@ int latent_attention_common(LatentAttention& p, const void* q, int64_t q_stride_
 }
 
 // Whether the results share no memory with each other, q, cache, sinks or `lists` (requests or lists of slots).
-bool latent_attention_results_apart(const LatentAttention& p, std::initializer_list<Region> lists) {
+bool latent_attention_results_apart(const LatentAttention& p, std::initializer_list<const Region*> lists) {
     const auto rows = [&](const void* at, int64_t bytes, int64_t stride_token, int64_t stride_head) {
         return Region(at, bytes, {{p.num_tokens, stride_token}, {p.num_heads, stride_head}});
     };
     const Region q = rows(p.q, kRowBytes, p.q_stride_token, p.q_stride_head), out = rows(p.out, kRowBytes, p.out_stride_token, p.out_stride_head),
                  lse = rows(p.lse, 4, 4 * p.lse_stride_token, 4 * p.lse_stride_head), sink(p.sink, 4 * static_cast<int64_t>(p.num_heads)),
                  cache(p.k_cache, static_cast<int64_t>(p.block_size) * (kTokenDataBytes + kScaleBytes), {{p.num_blocks, p.block_stride}});
-    return apart_from_all(out, {q, lse, sink, cache}) && apart_from_all(lse, {q, sink, cache}) && apart_from_all(out, lists) && apart_from_all(lse, lists);
+    return apart_from_all(out, {&q, &lse, &sink, &cache}) && apart_from_all(lse, {&q, &sink, &cache}) && apart_from_all(out, lists) && apart_from_all(lse, lists);
 }
 }  // namespace
 
@@ -553,9 +553,8 @@ int dsv4_paged_latent_attention(const void* q, int64_t q_stride_token, int64_t q
     p.window = window_size < lim ? static_cast<int32_t>(window_size) : 0;
     p.first = static_cast<int32_t>(num_first_tokens < most ? num_first_tokens : most);
     p.capacity = static_cast<int32_t>(max_blocks_per_seq > most / cache_block_size ? most : max_blocks_per_seq * cache_block_size);
-    if (!latent_attention_results_apart(p, {Region(block_table, 4 * max_blocks_per_seq, {{num_reqs, 4 * block_table_stride}}), Region(seq_lens, 4 * num_reqs),
-                                            Region(query_start_loc, 4 * (num_reqs + 1))}))
-        return DSV4_ERR_OVERLAP;
+    const Region table(block_table, 4 * max_blocks_per_seq, {{num_reqs, 4 * block_table_stride}}), lengths(seq_lens, 4 * num_reqs), starts(query_start_loc, 4 * (num_reqs + 1));
+    if (!latent_attention_results_apart(p, {&table, &lengths, &starts})) return DSV4_ERR_OVERLAP;
     return static_cast<int>(launch_latent_attention(p, workspace, static_cast<cudaStream_t>(cuda_stream)));
 }
 
@@ -574,7 +573,8 @@ int dsv4_sparse_latent_attention(const void* q, int64_t q_stride_token, int64_t 
     if (!lens || (!indices && topk > 0)) return DSV4_ERR_NULL_POINTER;
     // (lists of no entries have no memory, and none of it is read: any pointer says that this is the form with lists)
     p.indices = indices ? indices : lens, p.indices_stride = indices_stride, p.topk = static_cast<int32_t>(topk), p.lens = lens;
-    if (!latent_attention_results_apart(p, {Region(indices, 4 * topk, {{num_tokens, 4 * indices_stride}}), Region(lens, 4 * num_tokens)})) return DSV4_ERR_OVERLAP;
+    const Region slots(indices, 4 * topk, {{num_tokens, 4 * indices_stride}}), lengths(lens, 4 * num_tokens);
+    if (!latent_attention_results_apart(p, {&slots, &lengths})) return DSV4_ERR_OVERLAP;
     return static_cast<int>(launch_latent_attention(p, workspace, static_cast<cudaStream_t>(cuda_stream)));
 }
 

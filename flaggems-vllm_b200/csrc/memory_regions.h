@@ -12,7 +12,7 @@ struct Region {
     struct Dimension {
         int64_t count, stride;
     };
-    __int128 at = 0, row = 0;  // no bytes where row is 0; products of sizes that a caller names need not fit into 64 bits
+    __int128 at = 0, row = 0, end = 0;  // no bytes where row is 0; products of sizes that a caller names need not fit into 64 bits
     Dimension dims[3] = {{1, 0}, {1, 0}, {1, 0}};
 
     Region(const void* p, __int128 bytes, std::initializer_list<Dimension> outer = {}) : at(reinterpret_cast<uintptr_t>(p)), row(p ? bytes : 0) {
@@ -25,12 +25,13 @@ struct Region {
             }
             ++d;
         }
+        end = at + span(0);
     }
     // Bytes from the first to behind the last one, dimensions whose stride is a multiple of `modulus` left out (0: none left out).
     __int128 span(int64_t modulus) const {
         __int128 n = row;
         for (const Dimension& d : dims)
-            if (modulus == 0 || d.stride % modulus != 0) n += static_cast<__int128>(d.count - 1) * d.stride;
+            if (d.count > 1 && (modulus == 0 || d.stride % modulus != 0)) n += static_cast<__int128>(d.count - 1) * d.stride;
         return n;
     }
 };
@@ -39,7 +40,7 @@ struct Region {
 // one wide buffer, say).  Interleaved in another way they count as overlapping.
 inline bool regions_apart(const Region& a, const Region& b) {
     if (a.row <= 0 || b.row <= 0) return true;
-    if (a.at + a.span(0) <= b.at || b.at + b.span(0) <= a.at) return true;
+    if (a.end <= b.at || b.end <= a.at) return true;
     for (const Region* r : {&a, &b})
         for (const Region::Dimension& d : r->dims) {
             if (d.count <= 1 || d.stride <= 0) continue;
@@ -50,9 +51,9 @@ inline bool regions_apart(const Region& a, const Region& b) {
 }
 
 // Whether `a` shares memory with none of `others`.
-inline bool apart_from_all(const Region& a, std::initializer_list<Region> others) {
-    for (const Region& o : others)
-        if (!regions_apart(a, o)) return false;
+inline bool apart_from_all(const Region& a, std::initializer_list<const Region*> others) {
+    for (const Region* o : others)
+        if (!regions_apart(a, *o)) return false;
     return true;
 }
 
