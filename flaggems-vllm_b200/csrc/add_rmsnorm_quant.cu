@@ -4,14 +4,14 @@
 //   scale = max(max |y| of a group, 1e-10) / 448 or the power of two at or above it, x_q = e4m3(y / scale)
 //
 // Nothing between the sum and the e4m3 byte is rounded to 16 bits.  The mean is formed in 64 bits: squares of fp32 values are exact
-// there, so r is the correctly rounded value whatever the order of summation, and with it y, the scales and the bytes are those of the
-// definition bit for bit; a power-of-two scale would otherwise move by a factor of two where the last bit of a 32-bit sum carries it
-// across.
+// there, and their sum is off by less than 2^-48 of it in any order.  So r is the definition's 32-bit value but for rows whose root lies that near to the
+// middle of two of them (one row in 2^23), and with it y, the scales and the bytes; a power-of-two scale would otherwise move by a factor of two where the
+// last bit of a 32-bit sum carries it across.
 //
 // As many CTAs as fit take rows in turn, the row's sum in registers: thread i holds the 16-byte pieces i, i + blockDim, ..., so every access of a
 // warp is 512 contiguous bytes and a group of 64 / 128 / 256 values is 8 / 16 / 32 neighbouring lanes.  The next row is copied to shared memory
 // while this one is worked on (with a CTA for each row instead, 4097 x 7168 took 47.7 us).  Bound by HBM, 7 bytes a value, for many long rows: 4097 x 7168
-// bf16 38.3 us (82% of the time that a copy of as many bytes takes), 8192 x 4096 fp16, a scale a row, 45.8; the rest is the arithmetic, about 60
+// bf16 38.3 to 39.0 us (a copy of as many bytes takes 82% of that time), 8192 x 4096 fp16, a scale a row, 44 to 49; the rest is the arithmetic, about 60
 // instructions a piece.  One to 148 rows: 2.9 us, the latency of one row's loads, two reductions and stores.
 #include <algorithm>
 
@@ -100,8 +100,9 @@ __device__ __forceinline__ float inverse_root(double v) {
     return static_cast<float>(y);
 }
 
-// x / d correctly rounded, from the correctly rounded reciprocal y of d: the quotient x y corrected once by the exact remainder (Markstein, 1990).
-// (The remainder is exact for every quotient by a scale that is not rounded to a zero byte: the scale is at least 2^-43.)
+// x / d from the correctly rounded reciprocal y of d: the quotient x y corrected once by the remainder (Markstein, 1990).  Off by less than 2^-46 of x / d before its
+// one rounding, so its byte is that of the IEEE quotient: a test finds every pair of significands near enough to a border of two bytes to differ, and none does.
+// (No step of it underflows for a quotient that is not rounded to a zero byte: the scale is at least 2^-43.)
 __device__ __forceinline__ float2 divide(float2 x, float d, float y) {
     const float2 q = mul2(x, both(y));
     return fma2(fma2(both(-d), q, x), both(y), q);

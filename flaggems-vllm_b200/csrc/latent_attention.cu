@@ -9,7 +9,9 @@
 // request where there are fewer heads.  A CTA of 20 warps holds a tile's q (64 KiB) and streams its keys in blocks of 48, three of them in flight:
 //   warps 0-3    "softmax": S from TMEM, masks, running maximum and sum, P as bf16 to shared memory; O is multiplied by a correction only where a row's
 //                maximum has grown by more than a factor of 2^8 (P and the sum may exceed one by that factor; fp32 holds them).  At a tile's end: O to the
-//                output, or to the workspace as a piece.
+//                output, or to the workspace as a piece.  P is the one value that is held in fewer bits than its definition's: the products take operands of 16, and both
+//                of one type, which the keys fix (bf16 holds them all, fp16 does not).  A weight is off by at most 2^-8 of itself, the sum of the weights stays in fp32;
+//                against 64 bits `out` is off by 0.0017 to 0.0022 of its norm, where rounding it to bf16 alone makes 0.0017.
 //   warps 4-15   "readers": four keys of each block a warp.  They convert the cached rows to bf16 and store them swizzled, once; the same bytes are the
 //                K-major operand of S = Q K^T and the MN-major operand of O += P V.
 //   warp 16      one elected lane issues the products: S of the next block before O of this one, so that they run while the softmax does.
@@ -23,11 +25,13 @@
 // unnormalised sums and are joined, in a fixed order, by a second small kernel.  Where lists are short, tiles are not cut (see kLeastSplit).
 //
 // What bounds it.  In the largest chunk a block takes 2000 to 2100 cycles at the 1.56 GHz that power leaves: the products 1700 of them (a product of 64 rows
-// runs at half the rate of one of 128, which would need 128 KiB for q and 512 columns for O, and leave nothing for S), the rest the way from S to P and back
-// that the order S, O leaves open.  Softmax and readers take 1650 and 2100 beside it, half of the issue slots.  Readers that ask for the next block's values before
+// takes as long as one of 128: 128.8 cycles for 256 columns and a depth of 16), the rest the way from S to P and back that the order S, O leaves open.  In one CTA 128 rows
+// would need 128 KiB for q and 512 columns for O, and leave nothing for S.  A pair of CTAs with 64 rows of q each needs neither, in products that both
+// take part in (cta_group::2: 64.9 cycles for the same 256 columns of 128 rows, 25.7 for 64); that form is timed as a bare product only, not built.
+// Softmax and readers take 1650 and 2100 cycles beside the products, half of the issue slots.  Readers that ask for the next block's values before
 // they convert this one's (and hand over by hardware barriers, which do not wait for loads) change nothing: 3.25 ms both.
-// 1024 tokens x 128 heads over 8192 keys: 3.4 ms (690 TFLOP/s); 61 requests of up to 16384 keys, 64 heads: 158 us; one of 65536 keys, 128 heads: 46 us;
-// a window of 128 tokens, one request: 11.6 us, of which two thirds are the way in (plan, look-up, keys, q: each waits for memory that the one before names) and out.
+// 1024 tokens x 128 heads over 8192 keys: 3.3 ms (700 TFLOP/s); 61 requests of up to 16384 keys, 64 heads: 154 us; one of 65536 keys, 128 heads: 46 us;
+// a window of 128 tokens, one request: 10.9 us, of which two thirds are the way in (plan, look-up, keys, q: each waits for memory that the one before names) and out.
 // Other forms that were built: blocks of 64 keys in two stages, 6.9 ms; two groups of readers in turn, 4.5; eight softmax warps, 4.1 (this form then 3.9);
 // two CTAs that share out keys and exchange S and P, 128 rows a product: 5.0, since each exchange takes 400 cycles one way.
 #include <algorithm>

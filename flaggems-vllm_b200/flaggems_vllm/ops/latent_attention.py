@@ -14,6 +14,9 @@ A cached row of 512 values, shared by all heads, is key and value at once.  Per 
 * `sparse_latent_attention`: token t sees the cache slots indices[t, : lens[t]], as `compute_global_topk_indices_and_lens` makes them; negative
   entries are skipped.
 
+Scores, sums and both products' accumulators are of 32 bits, cached keys exactly what the cache holds.  The weights exp(s_j) are rounded to bfloat16, in which the
+second product takes them (2^-8 of each; their sum is that of the unrounded ones), the exponentials are the hardware's (2^-21), and `out` is rounded once.
+
 q is bfloat16 [tokens, heads, 512] with unit inner stride, any number of heads; rows, cache and cache blocks on 16-byte boundaries.  `out`
 (like q) and `lse` (float32 [tokens, heads]) are written where given; `out` is allocated otherwise, and returned.  Neither may share memory with the
 other or with an argument that is read.

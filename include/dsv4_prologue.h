@@ -348,6 +348,7 @@ int dsv4_fused_add_rmsnorm_quant_fp8(const void* x, int64_t x_row_stride, void* 
  * term is there where attn_sink is not NULL; lse does not contain it, and is only written where it is not NULL.
  *   q, out     bf16 [num_tokens, num_heads, 512], strides in elements (multiples of 8), 16-byte aligned
  *   lse        fp32, strides in elements
+ *   (scores, sums and accumulators are fp32; the weights e^(s_j) are rounded to bf16 for the second product, 2^-8 of each; out is rounded once)
  *   k_cache    as written by the prologue, num_blocks blocks; base and block stride on 16-byte boundaries
  *   softmax_scale  positive, at most 2.3e38
  *   workspace  dsv4_latent_attention_workspace_bytes(...) bytes, 16-byte aligned, of this call alone until it has run
