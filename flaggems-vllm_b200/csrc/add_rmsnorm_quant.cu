@@ -287,8 +287,11 @@ cudaError_t launch_rows(int64_t rows, int threads, cudaStream_t stream, const Ad
     constexpr int kMost = PIECES == 1 ? 1024 : PIECES == 2 ? 128 : PIECES == 4 ? 256 : 512, kSmThreads = PIECES <= 2 ? 1024 : PIECES == 4 ? 768 : 512;
     const auto kernel = add_rmsnorm_quant_kernel<PIECES, T, WEIGHT_F32, EXACT, kMost, kSmThreads / kMost>;
     const int row_bytes = 2 * PIECES * threads * 16, two_rows = row_bytes <= 52 * 1024, shared_bytes = (1 + two_rows) * row_bytes;
-    if (shared_bytes > 48 * 1024) {
-        const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared_bytes);
+    // From 48 KiB on, the kernel's own `sums` and `maxima` included, the function has to allow it: the same number each time, the most that any row takes (8 pieces of 512
+    // threads), so that a call on another thread with shorter rows does not take it back.
+    constexpr int kOwnBytes = 2 * 32 * (sizeof(double) + sizeof(float)), kMostBytes = 2 * 8 * 512 * 16;
+    if (shared_bytes + kOwnBytes > 48 * 1024) {
+        const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostBytes);
         if (rc != cudaSuccess) return rc;
     }
     // CTAs that fit on an SM, each of which takes rows in turn.
