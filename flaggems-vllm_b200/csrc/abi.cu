@@ -7,6 +7,7 @@
 #include "dsv4_common.cuh"
 #include "latent_attention.cuh"
 #include "memory_regions.h"
+#include "paged_batch.cuh"
 
 namespace dsv4 {
 namespace {
@@ -81,7 +82,8 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 // *any_alignment says whether the launch has to take the kernel for such pointers; where NULL, 16 bytes are required.
 int validate(const void* q, const void* kv, const void* k_cache, const int64_t* slot_mapping,
              const int64_t* position_ids, const float* cos_sin_cache, int64_t num_tokens, int64_t num_heads,
-             int64_t num_tokens_insert, int64_t cache_block_size, int64_t kv_block_stride_bytes, bool* any_alignment = nullptr) {
+             int64_t num_tokens_insert, int64_t cache_block_size, int64_t kv_block_stride_bytes, bool* any_alignment = nullptr,
+             int64_t token_bytes = kTokenDataBytes + kScaleBytes) {
     if (any_alignment) *any_alignment = false;
     if (num_tokens < 0 || num_heads < 0 || num_tokens_insert < 0 || num_tokens_insert > num_tokens)
         return DSV4_ERR_BAD_SIZE;
@@ -90,7 +92,7 @@ int validate(const void* q, const void* kv, const void* k_cache, const int64_t* 
     if (num_heads > 0 && !q) return DSV4_ERR_NULL_POINTER;
     if (num_tokens_insert > 0) {
         if (!kv || !k_cache || !slot_mapping) return DSV4_ERR_NULL_POINTER;
-        if (cache_block_size <= 0 || !holds(kv_block_stride_bytes, cache_block_size, kTokenDataBytes + kScaleBytes))
+        if (cache_block_size <= 0 || !holds(kv_block_stride_bytes, cache_block_size, token_bytes))
             return DSV4_ERR_BAD_SIZE;
     }
     if (!aligned16(q) || !aligned16(kv) || !aligned16(cos_sin_cache)) {
@@ -151,12 +153,25 @@ int dsv4_qnorm_rope_kv_insert(void* q, const void* kv, void* k_cache, const int6
     const PrologueParams p = make_params(q, kv, k_cache, slot_mapping, position_ids, cos_sin_cache, eps, num_tokens,
                                          num_heads, num_tokens_insert, cache_block_size, kv_block_stride_bytes);
     cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-    if (any_alignment) return static_cast<int>(launch_prologue_rows_any_alignment(p, stream));
+    if (any_alignment) return static_cast<int>(launch_prologue_rows_any_alignment(p, false, stream));
     int variant = current_variant();
     if (variant == DSV4_VARIANT_AUTO) variant = DSV4_VARIANT_ROWS;
     const cudaError_t err = variant == DSV4_VARIANT_BULK ? launch_prologue_bulk(p, stream)
                                                          : launch_prologue_rows(p, false, stream);
     return static_cast<int>(err);
+}
+
+int dsv4_qnorm_rope_kv_insert_mxfp4(void* q, const void* kv, void* k_cache, const int64_t* slot_mapping, const int64_t* position_ids,
+                                    const float* cos_sin_cache, float eps, int64_t num_tokens, int64_t num_heads, int64_t num_tokens_insert,
+                                    int64_t cache_block_size, int64_t kv_block_stride_bytes, void* cuda_stream) {
+    bool any_alignment = false;
+    const int rc = validate(q, kv, k_cache, slot_mapping, position_ids, cos_sin_cache, num_tokens, num_heads, num_tokens_insert, cache_block_size,
+                            kv_block_stride_bytes, &any_alignment, kMxTokenDataBytes + kMxScaleBytes);
+    if (rc != DSV4_OK || num_tokens == 0) return rc;
+    const PrologueParams p = make_params(q, kv, k_cache, slot_mapping, position_ids, cos_sin_cache, eps, num_tokens, num_heads, num_tokens_insert,
+                                         cache_block_size, kv_block_stride_bytes);
+    cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    return static_cast<int>(any_alignment ? launch_prologue_rows_any_alignment(p, true, stream) : launch_prologue_rows_mxfp4(p, stream));
 }
 
 int dsv4_qnorm_rope_kv_insert_padded(const void* q, void* q_out, const void* kv, void* k_cache, const int64_t* slot_mapping,
@@ -478,14 +493,16 @@ int dsv4_fused_add_rmsnorm_quant_fp8(const void* x, int64_t x_row_stride, void* 
 }
 
 namespace {
+int64_t cached_token_bytes(bool mxfp4) { return mxfp4 ? kMxTokenDataBytes + kMxScaleBytes : kTokenDataBytes + kScaleBytes; }
+
 // The arguments that both forms of the latent attention share, checked.
 int latent_attention_common(LatentAttention& p, const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_cache,
                             int64_t num_blocks, int64_t kv_block_stride_bytes, int64_t cache_block_size, const float* attn_sink,
                             float softmax_scale, void* out, int64_t out_stride_token, int64_t out_stride_head, float* lse,
-                            int64_t lse_stride_token, int64_t lse_stride_head, int64_t num_tokens, int64_t num_heads, const void* workspace) {
+                            int64_t lse_stride_token, int64_t lse_stride_head, int64_t num_tokens, int64_t num_heads, const void* workspace, bool mxfp4) {
     const int64_t lim = 1LL << 31;
     if (num_tokens < 0 || num_heads < 0 || num_blocks < 0 || cache_block_size <= 0) return DSV4_ERR_BAD_SIZE;
-    if (!holds(kv_block_stride_bytes, cache_block_size, kTokenDataBytes + kScaleBytes)) return DSV4_ERR_BAD_SIZE;
+    if (!holds(kv_block_stride_bytes, cache_block_size, cached_token_bytes(mxfp4))) return DSV4_ERR_BAD_SIZE;
     // (the kernels' exponentials are powers of two: log2(e) times the scale has to be a number too)
     if (!(softmax_scale > 0.0f && softmax_scale * 1.4426950408889634f <= 3.402823466e38f)) return DSV4_ERR_BAD_SIZE;
     if (num_tokens >= lim || num_heads >= lim || num_blocks >= lim || cache_block_size >= lim) return DSV4_ERR_TOO_LARGE;
@@ -513,33 +530,27 @@ int latent_attention_common(LatentAttention& p, const void* q, int64_t q_stride_
 }
 
 // Whether the results share no memory with each other, q, cache, sinks or `lists` (requests or lists of slots).
-bool latent_attention_results_apart(const LatentAttention& p, std::initializer_list<const Region*> lists) {
+bool latent_attention_results_apart(const LatentAttention& p, bool mxfp4, std::initializer_list<const Region*> lists) {
     const auto rows = [&](const void* at, int64_t bytes, int64_t stride_token, int64_t stride_head) {
         return Region(at, bytes, {{p.num_tokens, stride_token}, {p.num_heads, stride_head}});
     };
     const Region q = rows(p.q, kRowBytes, p.q_stride_token, p.q_stride_head), out = rows(p.out, kRowBytes, p.out_stride_token, p.out_stride_head),
                  lse = rows(p.lse, 4, 4 * p.lse_stride_token, 4 * p.lse_stride_head), sink(p.sink, 4 * static_cast<int64_t>(p.num_heads)),
-                 cache(p.k_cache, static_cast<int64_t>(p.block_size) * (kTokenDataBytes + kScaleBytes), {{p.num_blocks, p.block_stride}});
+                 cache(p.k_cache, static_cast<int64_t>(p.block_size) * cached_token_bytes(mxfp4), {{p.num_blocks, p.block_stride}});
     return apart_from_all(out, {&q, &lse, &sink, &cache}) && apart_from_all(lse, {&q, &sink, &cache}) && apart_from_all(out, lists) && apart_from_all(lse, lists);
 }
-}  // namespace
 
-int64_t dsv4_latent_attention_workspace_bytes(int64_t num_tokens, int64_t num_heads) {
-    if (num_tokens <= 0 || num_heads <= 0) return 0;
-    return static_cast<int64_t>(latent_attention_workspace(num_tokens, num_heads));
-}
-
-int dsv4_paged_latent_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_cache, int64_t num_blocks,
-                                int64_t kv_block_stride_bytes, int64_t cache_block_size, const int32_t* block_table,
-                                int64_t block_table_stride, int64_t max_blocks_per_seq, const int32_t* seq_lens,
-                                const int32_t* query_start_loc, int64_t num_reqs, int64_t window_size, int64_t num_first_tokens,
-                                const float* attn_sink, float softmax_scale, void* out, int64_t out_stride_token, int64_t out_stride_head,
-                                float* lse, int64_t lse_stride_token, int64_t lse_stride_head, int64_t num_tokens, int64_t num_heads,
-                                void* workspace, void* cuda_stream) {
+int paged_attention(bool mxfp4, const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_cache, int64_t num_blocks,
+                    int64_t kv_block_stride_bytes, int64_t cache_block_size, const int32_t* block_table,
+                    int64_t block_table_stride, int64_t max_blocks_per_seq, const int32_t* seq_lens,
+                    const int32_t* query_start_loc, int64_t num_reqs, int64_t window_size, int64_t num_first_tokens,
+                    const float* attn_sink, float softmax_scale, void* out, int64_t out_stride_token, int64_t out_stride_head,
+                    float* lse, int64_t lse_stride_token, int64_t lse_stride_head, int64_t num_tokens, int64_t num_heads,
+                    void* workspace, void* cuda_stream) {
     LatentAttention p{};
     const int rc = latent_attention_common(p, q, q_stride_token, q_stride_head, k_cache, num_blocks, kv_block_stride_bytes, cache_block_size,
                                            attn_sink, softmax_scale, out, out_stride_token, out_stride_head, lse, lse_stride_token,
-                                           lse_stride_head, num_tokens, num_heads, workspace);
+                                           lse_stride_head, num_tokens, num_heads, workspace, mxfp4);
     if (rc != DSV4_OK) return rc;
     const int64_t lim = 1LL << 31;
     if (num_reqs < 0 || max_blocks_per_seq < 0 || window_size < 0 || num_first_tokens < 0) return DSV4_ERR_BAD_SIZE;
@@ -554,19 +565,19 @@ int dsv4_paged_latent_attention(const void* q, int64_t q_stride_token, int64_t q
     p.first = static_cast<int32_t>(num_first_tokens < most ? num_first_tokens : most);
     p.capacity = static_cast<int32_t>(max_blocks_per_seq > most / cache_block_size ? most : max_blocks_per_seq * cache_block_size);
     const Region table(block_table, 4 * max_blocks_per_seq, {{num_reqs, 4 * block_table_stride}}), lengths(seq_lens, 4 * num_reqs), starts(query_start_loc, 4 * (num_reqs + 1));
-    if (!latent_attention_results_apart(p, {&table, &lengths, &starts})) return DSV4_ERR_OVERLAP;
-    return static_cast<int>(launch_latent_attention(p, workspace, static_cast<cudaStream_t>(cuda_stream)));
+    if (!latent_attention_results_apart(p, mxfp4, {&table, &lengths, &starts})) return DSV4_ERR_OVERLAP;
+    return static_cast<int>(launch_latent_attention(p, mxfp4, workspace, static_cast<cudaStream_t>(cuda_stream)));
 }
 
-int dsv4_sparse_latent_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_cache, int64_t num_blocks,
-                                 int64_t kv_block_stride_bytes, int64_t cache_block_size, const int32_t* indices, int64_t indices_stride,
-                                 int64_t topk, const int32_t* lens, const float* attn_sink, float softmax_scale, void* out,
-                                 int64_t out_stride_token, int64_t out_stride_head, float* lse, int64_t lse_stride_token,
-                                 int64_t lse_stride_head, int64_t num_tokens, int64_t num_heads, void* workspace, void* cuda_stream) {
+int sparse_attention(bool mxfp4, const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_cache, int64_t num_blocks,
+                     int64_t kv_block_stride_bytes, int64_t cache_block_size, const int32_t* indices, int64_t indices_stride,
+                     int64_t topk, const int32_t* lens, const float* attn_sink, float softmax_scale, void* out,
+                     int64_t out_stride_token, int64_t out_stride_head, float* lse, int64_t lse_stride_token,
+                     int64_t lse_stride_head, int64_t num_tokens, int64_t num_heads, void* workspace, void* cuda_stream) {
     LatentAttention p{};
     const int rc = latent_attention_common(p, q, q_stride_token, q_stride_head, k_cache, num_blocks, kv_block_stride_bytes, cache_block_size,
                                            attn_sink, softmax_scale, out, out_stride_token, out_stride_head, lse, lse_stride_token,
-                                           lse_stride_head, num_tokens, num_heads, workspace);
+                                           lse_stride_head, num_tokens, num_heads, workspace, mxfp4);
     if (rc != DSV4_OK) return rc;
     if (topk < 0 || topk >= (1LL << 31) - 256) return DSV4_ERR_BAD_SIZE;
     if (num_tokens == 0 || num_heads == 0) return DSV4_OK;
@@ -574,8 +585,143 @@ int dsv4_sparse_latent_attention(const void* q, int64_t q_stride_token, int64_t 
     // (lists of no entries have no memory, and none of it is read: any pointer says that this is the form with lists)
     p.indices = indices ? indices : lens, p.indices_stride = indices_stride, p.topk = static_cast<int32_t>(topk), p.lens = lens;
     const Region slots(indices, 4 * topk, {{num_tokens, 4 * indices_stride}}), lengths(lens, 4 * num_tokens);
-    if (!latent_attention_results_apart(p, {&slots, &lengths})) return DSV4_ERR_OVERLAP;
-    return static_cast<int>(launch_latent_attention(p, workspace, static_cast<cudaStream_t>(cuda_stream)));
+    if (!latent_attention_results_apart(p, mxfp4, {&slots, &lengths})) return DSV4_ERR_OVERLAP;
+    return static_cast<int>(launch_latent_attention(p, mxfp4, workspace, static_cast<cudaStream_t>(cuda_stream)));
+}
+
+}  // namespace
+
+int64_t dsv4_latent_attention_workspace_bytes(int64_t num_tokens, int64_t num_heads) {
+    if (num_tokens <= 0 || num_heads <= 0) return 0;
+    return static_cast<int64_t>(latent_attention_workspace(num_tokens, num_heads));
+}
+
+int dsv4_paged_latent_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_cache, int64_t num_blocks,
+                                int64_t kv_block_stride_bytes, int64_t cache_block_size, const int32_t* block_table,
+                                int64_t block_table_stride, int64_t max_blocks_per_seq, const int32_t* seq_lens,
+                                const int32_t* query_start_loc, int64_t num_reqs, int64_t window_size, int64_t num_first_tokens,
+                                const float* attn_sink, float softmax_scale, void* out, int64_t out_stride_token, int64_t out_stride_head,
+                                float* lse, int64_t lse_stride_token, int64_t lse_stride_head, int64_t num_tokens, int64_t num_heads,
+                                void* workspace, void* cuda_stream) {
+    return paged_attention(false, q, q_stride_token, q_stride_head, k_cache, num_blocks, kv_block_stride_bytes, cache_block_size,
+                           block_table, block_table_stride, max_blocks_per_seq, seq_lens, query_start_loc, num_reqs, window_size,
+                           num_first_tokens, attn_sink, softmax_scale, out, out_stride_token, out_stride_head, lse, lse_stride_token,
+                           lse_stride_head, num_tokens, num_heads, workspace, cuda_stream);
+}
+
+int dsv4_paged_latent_attention_mxfp4(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_cache, int64_t num_blocks,
+                                      int64_t kv_block_stride_bytes, int64_t cache_block_size, const int32_t* block_table,
+                                      int64_t block_table_stride, int64_t max_blocks_per_seq, const int32_t* seq_lens,
+                                      const int32_t* query_start_loc, int64_t num_reqs, int64_t window_size, int64_t num_first_tokens,
+                                      const float* attn_sink, float softmax_scale, void* out, int64_t out_stride_token, int64_t out_stride_head,
+                                      float* lse, int64_t lse_stride_token, int64_t lse_stride_head, int64_t num_tokens, int64_t num_heads,
+                                      void* workspace, void* cuda_stream) {
+    return paged_attention(true, q, q_stride_token, q_stride_head, k_cache, num_blocks, kv_block_stride_bytes, cache_block_size,
+                           block_table, block_table_stride, max_blocks_per_seq, seq_lens, query_start_loc, num_reqs, window_size,
+                           num_first_tokens, attn_sink, softmax_scale, out, out_stride_token, out_stride_head, lse, lse_stride_token,
+                           lse_stride_head, num_tokens, num_heads, workspace, cuda_stream);
+}
+
+int dsv4_sparse_latent_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_cache, int64_t num_blocks,
+                                 int64_t kv_block_stride_bytes, int64_t cache_block_size, const int32_t* indices, int64_t indices_stride,
+                                 int64_t topk, const int32_t* lens, const float* attn_sink, float softmax_scale, void* out,
+                                 int64_t out_stride_token, int64_t out_stride_head, float* lse, int64_t lse_stride_token,
+                                 int64_t lse_stride_head, int64_t num_tokens, int64_t num_heads, void* workspace, void* cuda_stream) {
+    return sparse_attention(false, q, q_stride_token, q_stride_head, k_cache, num_blocks, kv_block_stride_bytes, cache_block_size,
+                            indices, indices_stride, topk, lens, attn_sink, softmax_scale, out, out_stride_token, out_stride_head, lse,
+                            lse_stride_token, lse_stride_head, num_tokens, num_heads, workspace, cuda_stream);
+}
+
+int dsv4_sparse_latent_attention_mxfp4(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_cache, int64_t num_blocks,
+                                       int64_t kv_block_stride_bytes, int64_t cache_block_size, const int32_t* indices, int64_t indices_stride,
+                                       int64_t topk, const int32_t* lens, const float* attn_sink, float softmax_scale, void* out,
+                                       int64_t out_stride_token, int64_t out_stride_head, float* lse, int64_t lse_stride_token,
+                                       int64_t lse_stride_head, int64_t num_tokens, int64_t num_heads, void* workspace, void* cuda_stream) {
+    return sparse_attention(true, q, q_stride_token, q_stride_head, k_cache, num_blocks, kv_block_stride_bytes, cache_block_size,
+                            indices, indices_stride, topk, lens, attn_sink, softmax_scale, out, out_stride_token, out_stride_head, lse,
+                            lse_stride_token, lse_stride_head, num_tokens, num_heads, workspace, cuda_stream);
+}
+
+namespace {
+// What both operators on block tables take, checked.
+int paged_batch_common(PagedBatch& p, int64_t num_reqs, const int32_t* block_table, int64_t block_table_stride, int64_t max_blocks_per_seq,
+                       const int32_t* free_blocks, int64_t free_capacity, const int32_t* num_free, const int32_t* num_free_out,
+                       int64_t cache_block_size) {
+    const int64_t lim = 1LL << 31;
+    if (num_reqs < 0 || max_blocks_per_seq < 0 || free_capacity < 0 || cache_block_size <= 0) return DSV4_ERR_BAD_SIZE;
+    if (num_reqs > kMostRequests || max_blocks_per_seq >= lim || free_capacity >= lim || cache_block_size >= lim) return DSV4_ERR_TOO_LARGE;
+    if (num_reqs > 1 && block_table_stride < max_blocks_per_seq) return DSV4_ERR_BAD_SIZE;
+    if (!num_free || !num_free_out || (!free_blocks && free_capacity > 0) || (!block_table && num_reqs > 0 && max_blocks_per_seq > 0))
+        return DSV4_ERR_NULL_POINTER;
+    p.block_table = const_cast<int32_t*>(block_table), p.table_stride = num_reqs > 1 ? block_table_stride : 0;
+    p.free_blocks = free_blocks, p.num_free = num_free, p.num_free_out = const_cast<int32_t*>(num_free_out);
+    p.num_reqs = static_cast<int32_t>(num_reqs), p.max_blocks = static_cast<int32_t>(max_blocks_per_seq);
+    p.free_capacity = static_cast<int32_t>(free_capacity), p.block_size = static_cast<uint32_t>(cache_block_size);
+    make_fast_divisor(p.block_size, &p.block_mul, &p.block_shift);
+    return DSV4_OK;
+}
+
+bool on_words(std::initializer_list<const void*> pointers, uintptr_t bytes) {
+    for (const void* p : pointers)
+        if ((reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0) return false;
+    return true;
+}
+}  // namespace
+
+int dsv4_extend_block_tables(const int32_t* context_lens, const int32_t* new_lens, int64_t num_reqs, int32_t* block_table,
+                             int64_t block_table_stride, int64_t max_blocks_per_seq, const int32_t* free_blocks, int64_t free_capacity,
+                             const int32_t* num_free, int64_t cache_block_size, int64_t num_tokens, int32_t* query_start_loc, int32_t* seq_lens,
+                             int64_t* position_ids, int64_t* slot_mapping, int32_t* token_to_req_indices, int32_t* num_free_out,
+                             int32_t* num_missing, void* cuda_stream) {
+    PagedBatch p{};
+    const int rc = paged_batch_common(p, num_reqs, block_table, block_table_stride, max_blocks_per_seq, free_blocks, free_capacity, num_free,
+                                      num_free_out, cache_block_size);
+    if (rc != DSV4_OK) return rc;
+    if (num_tokens < 0) return DSV4_ERR_BAD_SIZE;
+    if (num_tokens >= (1LL << 31)) return DSV4_ERR_TOO_LARGE;
+    if (!query_start_loc || !num_missing || (num_reqs > 0 && (!context_lens || !new_lens || !seq_lens)) ||
+        (num_tokens > 0 && (!position_ids || !slot_mapping || !token_to_req_indices)))
+        return DSV4_ERR_NULL_POINTER;
+    if (!on_words({context_lens, new_lens, block_table, free_blocks, num_free, query_start_loc, seq_lens, token_to_req_indices, num_free_out, num_missing}, 4) ||
+        !on_words({position_ids, slot_mapping}, 8))
+        return DSV4_ERR_MISALIGNED;
+    const Region contexts(context_lens, 4 * num_reqs), lens(new_lens, 4 * num_reqs), table(block_table, 4 * max_blocks_per_seq, {{num_reqs, 4 * block_table_stride}}),
+        blocks(free_blocks, 4 * free_capacity), there(num_free, 4), starts(query_start_loc, 4 * (num_reqs + 1)), ends(seq_lens, 4 * num_reqs),
+        positions(position_ids, 8 * num_tokens), slots(slot_mapping, 8 * num_tokens), requests(token_to_req_indices, 4 * num_tokens), left(num_free_out, 4),
+        missing(num_missing, 4);
+    // two results may stand in the place of the argument that they continue
+    const bool own_lens = seq_lens == context_lens, own_free = num_free_out == num_free;
+    if (!apart_from_all(table, {&contexts, &lens, &blocks, &there, &starts, &ends, &positions, &slots, &requests, &left, &missing}) ||
+        !apart_from_all(starts, {&contexts, &lens, &blocks, &there, &ends, &positions, &slots, &requests, &left, &missing}) ||
+        !apart_from_all(ends, {&lens, &blocks, &there, &positions, &slots, &requests, &left, &missing}) || (!own_lens && !regions_apart(ends, contexts)) ||
+        !apart_from_all(positions, {&contexts, &lens, &blocks, &there, &slots, &requests, &left, &missing}) ||
+        !apart_from_all(slots, {&contexts, &lens, &blocks, &there, &requests, &left, &missing}) ||
+        !apart_from_all(requests, {&contexts, &lens, &blocks, &there, &left, &missing}) ||
+        !apart_from_all(left, {&contexts, &lens, &blocks, &missing}) || (!own_free && !regions_apart(left, there)) ||
+        !apart_from_all(missing, {&contexts, &lens, &blocks, &there}))
+        return DSV4_ERR_OVERLAP;
+    p.context_lens = context_lens, p.new_lens = new_lens, p.query_start_loc = query_start_loc, p.seq_lens = seq_lens;
+    p.position_ids = position_ids, p.slot_mapping = slot_mapping, p.token_to_req = token_to_req_indices, p.num_missing = num_missing;
+    p.num_tokens = num_tokens;
+    return static_cast<int>(launch_extend_block_tables(p, static_cast<cudaStream_t>(cuda_stream)));
+}
+
+int dsv4_release_block_tables(const int32_t* seq_lens, const uint8_t* finished, int64_t num_reqs, const int32_t* block_table,
+                              int64_t block_table_stride, int64_t max_blocks_per_seq, int32_t* free_blocks, int64_t free_capacity,
+                              const int32_t* num_free, int64_t cache_block_size, int32_t* num_free_out, void* cuda_stream) {
+    PagedBatch p{};
+    const int rc = paged_batch_common(p, num_reqs, block_table, block_table_stride, max_blocks_per_seq, free_blocks, free_capacity, num_free,
+                                      num_free_out, cache_block_size);
+    if (rc != DSV4_OK) return rc;
+    if (num_reqs > 0 && (!seq_lens || !finished)) return DSV4_ERR_NULL_POINTER;
+    if (!on_words({seq_lens, block_table, free_blocks, num_free, num_free_out}, 4)) return DSV4_ERR_MISALIGNED;
+    const Region lens(seq_lens, 4 * num_reqs), done(finished, num_reqs), table(block_table, 4 * max_blocks_per_seq, {{num_reqs, 4 * block_table_stride}}),
+        blocks(free_blocks, 4 * free_capacity), there(num_free, 4), left(num_free_out, 4);
+    if (!apart_from_all(blocks, {&lens, &done, &table, &there, &left}) || !apart_from_all(left, {&lens, &done, &table}) ||
+        (num_free_out != num_free && !regions_apart(left, there)))
+        return DSV4_ERR_OVERLAP;
+    p.context_lens = seq_lens, p.finished = finished, p.free_to = free_blocks;
+    return static_cast<int>(launch_release_block_tables(p, static_cast<cudaStream_t>(cuda_stream)));
 }
 
 int dsv4_fused_indexer_q_rope_quant(const int64_t* positions, const void* index_q, int64_t q_stride0, int64_t q_stride1,

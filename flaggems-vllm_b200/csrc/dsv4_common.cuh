@@ -25,6 +25,10 @@ constexpr int kNopeDim = 448;
 constexpr int kRowBytes = kHeadDim * 2;
 constexpr int kTokenDataBytes = 576;
 constexpr int kScaleBytes = 8;
+// The cache in 4 bits: 448 e2m1 values (two a byte, the first in the low bits) and the 64 bf16 ones, then 14 scale codes, of 32 values each, and two zeros.
+constexpr int kMxNopeBytes = kNopeDim / 2;
+constexpr int kMxTokenDataBytes = kMxNopeBytes + 2 * kRopeDim;
+constexpr int kMxScaleBytes = 16;
 constexpr int kCosSinRowBytes = 256;
 constexpr int kFirstRopeLane = 24;
 
@@ -237,6 +241,12 @@ __device__ __forceinline__ void st_stream16(void* p, uint4 v) {
     asm volatile("st.global.L1::no_allocate.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z),
                  "r"(v.w)
                  : "memory");
+}
+
+__device__ __forceinline__ uint2 ld_stream8(const void* p) {
+    uint2 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
 }
 
 __device__ __forceinline__ uint32_t ld_stream4(const void* p) {
@@ -532,6 +542,40 @@ __device__ __forceinline__ float2 scaled_pair(uint32_t pair, uint16_t factor) {
     return r;
 }
 
+// ---- MXFP4: e2m1 values in blocks of 32 with a power-of-two scale ----
+// UE8M0 byte of an MXFP4 block whose absolute maximum is `amax`: ceil(log2(max(amax, 6*2^-126) / 6)) + 127 clamped to
+// [0, 254], without the division: 6 = 1.5 * 4, so with the clamped maximum m * 2^(E-127), 1 <= m < 2, the quotient is
+// below, at or above 2^(E-129) for m below, at or above 1.5.  Equal to the log2/ceil statement for every bf16
+// maximum (a CPU test enumerates them).
+__device__ __forceinline__ uint32_t mxfp4_code(float amax) {
+    const uint32_t u = __float_as_uint(fmaxf(amax, 6.0f * 1.17549435e-38f));
+    const uint32_t code = (u >> 23) - 2u + ((u & 0x7fffffu) > 0x400000u ? 1u : 0u);
+    return code > 254u ? 254u : code;
+}
+
+// Two floats -> one byte of two e2m1 codes (lo in bits 0-3), round to nearest even, saturating at +-6.
+__device__ __forceinline__ uint32_t pack_e2m1x2(float lo, float hi) {
+    uint32_t r;
+    asm("{.reg .b8 t; cvt.rn.satfinite.e2m1x2.f32 t, %1, %2; cvt.u32.u8 %0, t;}" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// Four packed bf16 pairs times 2^(127 - code), the factor given as bf16 -> one word of eight e2m1 codes (element 0 in bits 0-3),
+// round to nearest even, saturating at +-6.  Exact before the conversion (scaled_pair()).
+__device__ __forceinline__ uint32_t pack_e2m1x8(const uint4& v, uint16_t factor) {
+    const float2 x0 = scaled_pair(v.x, factor), x1 = scaled_pair(v.y, factor), x2 = scaled_pair(v.z, factor), x3 = scaled_pair(v.w, factor);
+    uint32_t r;
+    asm("{.reg .b8 t0, t1, t2, t3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 t0, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 t1, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 t2, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 t3, %8, %7;\n\t"
+        "mov.b32 %0, {t0, t1, t2, t3};}"
+        : "=r"(r)
+        : "f"(x0.x), "f"(x0.y), "f"(x1.x), "f"(x1.y), "f"(x2.x), "f"(x2.y), "f"(x3.x), "f"(x3.y));
+    return r;
+}
+
 // 8 bf16 values times a power of two, given as bf16, to e4m3.
 __device__ __forceinline__ uint2 quant8_times(const uint4& v, uint32_t factor) {
     const auto f = static_cast<uint16_t>(factor);
@@ -607,9 +651,67 @@ __device__ __forceinline__ void kv_row_to_cache(const uint4& a, const uint4& b, 
     }
 }
 
+// Scale code of a group of the cache in 4 bits, from the largest magnitude's bits as fp32 (any bf16): mxfp4_code(), and 255, which stands for NaN, where a
+// value is infinite or NaN: neither has an e2m1 value, and the readers make the whole group NaN.
+__device__ __forceinline__ uint32_t mxfp4_cache_code(uint32_t magnitude) { return magnitude >= 0x7f800000u ? 255u : mxfp4_code(__uint_as_float(magnitude)); }
+// Largest magnitude of eight bf16 values, as the bits of an fp32.  (Magnitudes are ordered like integers, NaN above infinity.)
+__device__ __forceinline__ uint32_t magnitude8(const uint4& v) {
+    const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+    return max(m << 16, m & 0xffff0000u);
+}
+// Eight values of a group as e2m1, zeros where the group's code says that they are no numbers.
+__device__ __forceinline__ uint32_t mxfp4_word(const uint4& v, uint32_t code) {
+    const uint32_t word = pack_e2m1x8(v, static_cast<uint16_t>(pow2_reciprocal(code)));
+    return code == 255u ? 0u : word;
+}
+
+// kv_row_to_cache() for the cache in 4 bits: `data` is a record of 352 bytes, `scales` are its 16 scale bytes.  A group of 32 values is four
+// lanes of one register.
+__device__ __forceinline__ void kv_row_to_cache_mxfp4(const uint4& a, const uint4& b, int lane, const float4& c, const float4& s, uint8_t* data,
+                                                      uint8_t* scales, bool aligned16) {
+    uint32_t ma = magnitude8(a), mb = magnitude8(b);
+#pragma unroll
+    for (int m = 1; m <= 2; m <<= 1) {
+        ma = max(ma, __shfl_xor_sync(0xffffffffu, ma, m));
+        mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, m));
+    }
+    const bool rope_lane = lane >= kFirstRopeLane;
+    const uint32_t code_a = mxfp4_cache_code(ma), code_b = rope_lane ? 0u : mxfp4_cache_code(mb);
+    const uint32_t qa = mxfp4_word(a, code_a);
+    uint32_t qb = 0u;
+    uint4 rb = make_uint4(0u, 0u, 0u, 0u);
+    if (rope_lane) {
+        float x[8];
+        unpack8(b, x);
+        rotate4(x, c, s);
+        rb = pack8(x);
+    } else {
+        qb = mxfp4_word(b, code_b);
+    }
+    if (aligned16) {
+        *reinterpret_cast<uint32_t*>(data + 4 * lane) = qa;
+        if (rope_lane) *reinterpret_cast<uint4*>(data + kMxNopeBytes + 16 * (lane - kFirstRopeLane)) = rb;
+        else *reinterpret_cast<uint32_t*>(data + 128 + 4 * lane) = qb;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) data[4 * lane + i] = static_cast<uint8_t>(qa >> (8 * i));
+        if (rope_lane) {
+            const uint32_t wr[4] = {rb.x, rb.y, rb.z, rb.w};
+#pragma unroll
+            for (int i = 0; i < 16; ++i) data[kMxNopeBytes + 16 * (lane - kFirstRopeLane) + i] = static_cast<uint8_t>(wr[i >> 2] >> (8 * (i & 3)));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) data[128 + 4 * lane + i] = static_cast<uint8_t>(qb >> (8 * i));
+        }
+    }
+    // the codes of eight groups in every fourth lane: groups 0-7 from a, 8-13 and the two zeros from b
+    if ((lane & 3) == 0) scales[lane >> 2] = static_cast<uint8_t>(code_a), scales[8 + (lane >> 2)] = static_cast<uint8_t>(code_b);
+}
+
 // Launchers implemented by the kernel files; each returns cudaGetLastError() of its launch.
 cudaError_t launch_prologue_rows(const PrologueParams& p, bool checked, cudaStream_t stream);
 cudaError_t launch_prologue_rows_padded(const PrologueParams& p, cudaStream_t stream);
+cudaError_t launch_prologue_rows_mxfp4(const PrologueParams& p, cudaStream_t stream);
 cudaError_t launch_prologue_bulk(const PrologueParams& p, cudaStream_t stream);
 cudaError_t launch_gather_dequant(const uint8_t* k_cache, const int64_t* slots, int64_t num_slots, uint8_t* out,
                                   int64_t out_row_stride, int64_t block_size, int64_t block_stride,
@@ -664,7 +766,7 @@ cudaError_t launch_inv_rope_fp8_quant_any(const void* o, int64_t o_stride_token,
                                           int64_t scale_stride_group, int64_t num_tokens, int64_t padded_tokens, int num_heads,
                                           int heads_per_group, int nope_dim, int rope_dim, int group_size, float eps, int packed,
                                           cudaStream_t stream);
-cudaError_t launch_prologue_rows_any_alignment(const PrologueParams& p, cudaStream_t stream);
+cudaError_t launch_prologue_rows_any_alignment(const PrologueParams& p, bool mxfp4, cudaStream_t stream);
 void count_launch();
 cudaError_t read_device_error(int* value);
 

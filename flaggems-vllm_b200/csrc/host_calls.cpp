@@ -183,7 +183,8 @@ PyObject* entry(PyObject*, PyObject* const* values, Py_ssize_t count) {
 }
 
 // q, kv, k_cache, slot_mapping, position_ids, cos_sin_cache, eps, cache_block_size
-PyObject* prologue(Arguments& a) {
+template <bool MXFP4>
+PyObject* prologue_into(Arguments& a) {
     const Tensor *q = a.tensor(0), *kv = a.tensor(1), *cache = a.tensor(2), *slots = a.tensor(3), *pos = a.tensor(4), *cs = a.tensor(5);
     const float eps = a.real(6);
     const int64_t block = a.integer(7);
@@ -196,18 +197,20 @@ PyObject* prologue(Arguments& a) {
     REQUIRE(slots->dim() == 1 && is(*slots, at::kLong) && slots->is_contiguous() && slots->size(0) <= tokens);
     REQUIRE(pos->dim() == 1 && is(*pos, at::kLong) && pos->is_contiguous() && pos->size(0) == tokens);
     REQUIRE(cs->dim() == 2 && cs->size(1) == 64 && is(*cs, at::kFloat) && cs->is_contiguous());
-    REQUIRE(cache->dim() == 2 && cache->stride(1) == 1 && block > 0 && cache->size(1) / 584 >= block);
+    REQUIRE(cache->dim() == 2 && cache->stride(1) == 1 && block > 0 && cache->size(1) / (MXFP4 ? 368 : 584) >= block);
     REQUIRE(on(*kv, *q) && on(*cache, *q) && on(*slots, *q) && on(*pos, *q) && on(*cs, *q));
     if (!a.ok) Py_RETURN_NONE;
     if (tokens == 0) Py_RETURN_TRUE;
     if (!launch_on(on_device_of(*q, OnDevice::kLaunchesOnly), [&](void* stream) {
-            return dsv4_qnorm_rope_kv_insert(q->data_ptr(), kv->data_ptr(), cache->data_ptr(), static_cast<const int64_t*>(slots->data_ptr()),
-                                             static_cast<const int64_t*>(pos->data_ptr()), static_cast<const float*>(cs->data_ptr()), eps,
-                                             tokens, heads, slots->size(0), block, cache->stride(0), stream);
+            return (MXFP4 ? dsv4_qnorm_rope_kv_insert_mxfp4 : dsv4_qnorm_rope_kv_insert)(
+                q->data_ptr(), kv->data_ptr(), cache->data_ptr(), static_cast<const int64_t*>(slots->data_ptr()), static_cast<const int64_t*>(pos->data_ptr()),
+                static_cast<const float*>(cs->data_ptr()), eps, tokens, heads, slots->size(0), block, cache->stride(0), stream);
         }))
         return nullptr;
     Py_RETURN_TRUE;
 }
+PyObject* prologue(Arguments& a) { return prologue_into<false>(a); }
+PyObject* prologue_mxfp4(Arguments& a) { return prologue_into<true>(a); }
 
 // The library's code of a row or weight type, -1 for a type it does not take.
 int dtype_code(const Tensor& t) {
@@ -643,9 +646,9 @@ struct AttentionTensors {
     float scale;
 };
 
-void require_attention(Arguments& a, const AttentionTensors& t) {
+void require_attention(Arguments& a, const AttentionTensors& t, int64_t token_bytes) {
     REQUIRE(t.q->is_cuda() && t.q->dim() == 3 && t.q->size(2) == 512 && is(*t.q, at::kBFloat16) && t.q->stride(2) == 1);
-    REQUIRE(is(*t.cache, at::kByte) && t.cache->dim() == 2 && t.cache->stride(1) == 1 && t.block > 0 && t.cache->size(1) / 584 >= t.block);
+    REQUIRE(is(*t.cache, at::kByte) && t.cache->dim() == 2 && t.cache->stride(1) == 1 && t.block > 0 && t.cache->size(1) / token_bytes >= t.block);
     REQUIRE(t.cache->size(0) <= 1 || t.cache->stride(0) >= t.cache->size(1));
     REQUIRE(t.scale > 0.0f && t.scale * 1.4426950408889634f < INFINITY);
     REQUIRE(on(*t.cache, *t.q));
@@ -661,14 +664,15 @@ void require_attention(Arguments& a, const AttentionTensors& t) {
 
 // q, k_cache, block_table, seq_lens, query_start_loc, cache_block_size, softmax_scale, window_size or None, num_first_tokens,
 // attn_sink or None, out or None, lse or None -> out
-PyObject* paged_latent_attention(Arguments& a) {
+template <bool MXFP4>
+PyObject* paged_attention_over(Arguments& a) {
     const Tensor *q = a.tensor(0), *cache = a.tensor(1), *table = a.tensor(2), *seq = a.tensor(3), *start = a.tensor(4);
     const AttentionTensors t{q, cache, a.is_none(9) ? nullptr : a.tensor(9), a.is_none(10) ? nullptr : a.tensor(10),
                              a.is_none(11) ? nullptr : a.tensor(11), a.integer_of(5), a.real(6)};
     const bool windowed = !a.is_none(7);
     const int64_t window = windowed ? a.integer_of(7) : 0, first = a.integer_of(8);
     if (!a.ok) Py_RETURN_NONE;
-    require_attention(a, t);
+    require_attention(a, t, MXFP4 ? 368 : 584);
     REQUIRE(table->dim() == 2 && is(*table, at::kInt) && table->stride(1) == 1 && on(*table, *q));
     REQUIRE(seq->dim() == 1 && is(*seq, at::kInt) && seq->is_contiguous() && on(*seq, *q));
     REQUIRE(start->dim() == 1 && is(*start, at::kInt) && start->is_contiguous() && on(*start, *q));
@@ -682,7 +686,7 @@ PyObject* paged_latent_attention(Arguments& a) {
     if (tokens > 0 && heads > 0 && requests > 0) {
         const Tensor workspace = make_empty({dsv4_latent_attention_workspace_bytes(tokens, heads)}, at::kByte, here);
         if (!launch_on(here, [&](void* stream) {
-                return dsv4_paged_latent_attention(
+                return (MXFP4 ? dsv4_paged_latent_attention_mxfp4 : dsv4_paged_latent_attention)(
                     q->data_ptr(), q->stride(0), q->stride(1), cache->data_ptr(), cache->size(0), cache->stride(0), t.block,
                     static_cast<const int32_t*>(table->data_ptr()), table->stride(0), table->size(1), static_cast<const int32_t*>(seq->data_ptr()),
                     static_cast<const int32_t*>(start->data_ptr()), requests, window, first,
@@ -696,12 +700,13 @@ PyObject* paged_latent_attention(Arguments& a) {
 }
 
 // q, k_cache, indices, lens, cache_block_size, softmax_scale, attn_sink or None, out or None, lse or None -> out
-PyObject* sparse_latent_attention(Arguments& a) {
+template <bool MXFP4>
+PyObject* sparse_attention_over(Arguments& a) {
     const Tensor *q = a.tensor(0), *cache = a.tensor(1), *indices = a.tensor(2), *lens = a.tensor(3);
     const AttentionTensors t{q, cache, a.is_none(6) ? nullptr : a.tensor(6), a.is_none(7) ? nullptr : a.tensor(7),
                              a.is_none(8) ? nullptr : a.tensor(8), a.integer_of(4), a.real(5)};
     if (!a.ok) Py_RETURN_NONE;
-    require_attention(a, t);
+    require_attention(a, t, MXFP4 ? 368 : 584);
     REQUIRE(indices->dim() == 2 && is(*indices, at::kInt) && indices->stride(1) == 1 && on(*indices, *q));
     REQUIRE(lens->dim() == 1 && is(*lens, at::kInt) && lens->is_contiguous() && on(*lens, *q));
     if (!a.ok) Py_RETURN_NONE;
@@ -713,7 +718,7 @@ PyObject* sparse_latent_attention(Arguments& a) {
     if (tokens > 0 && heads > 0) {
         const Tensor workspace = make_empty({dsv4_latent_attention_workspace_bytes(tokens, heads)}, at::kByte, here);
         if (!launch_on(here, [&](void* stream) {
-                return dsv4_sparse_latent_attention(
+                return (MXFP4 ? dsv4_sparse_latent_attention_mxfp4 : dsv4_sparse_latent_attention)(
                     q->data_ptr(), q->stride(0), q->stride(1), cache->data_ptr(), cache->size(0), cache->stride(0), t.block,
                     static_cast<const int32_t*>(indices->data_ptr()), indices->stride(0), indices->size(1), static_cast<const int32_t*>(lens->data_ptr()),
                     t.sink ? static_cast<const float*>(t.sink->data_ptr()) : nullptr, t.scale, made.data_ptr(), made.stride(0), made.stride(1),
@@ -722,6 +727,106 @@ PyObject* sparse_latent_attention(Arguments& a) {
             }))
             return nullptr;
     }
+    return wrap(std::move(made));
+}
+
+PyObject* paged_latent_attention(Arguments& a) { return paged_attention_over<false>(a); }
+PyObject* paged_latent_attention_mxfp4(Arguments& a) { return paged_attention_over<true>(a); }
+PyObject* sparse_latent_attention(Arguments& a) { return sparse_attention_over<false>(a); }
+PyObject* sparse_latent_attention_mxfp4(Arguments& a) { return sparse_attention_over<true>(a); }
+
+bool is_list(const Tensor& t, ScalarType type, int64_t size, const Tensor& first) {
+    return t.dim() == 1 && is(t, type) && t.size(0) == size && t.is_contiguous() && on(t, first);
+}
+bool shares(const Tensor& a, const Tensor& b) { return a.numel() > 0 && b.numel() > 0 && !apart(a, b); }
+int32_t* ints(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
+int64_t* longs(const Tensor& t) { return static_cast<int64_t*>(t.data_ptr()); }
+
+// Lengths, block table, free blocks and their number, as both operators on block tables take them.
+void require_pool(Arguments& a, const Tensor& lens, const Tensor& table, const Tensor& free, const Tensor& count, int64_t block) {
+    REQUIRE(lens.is_cuda() && lens.dim() == 1 && is(lens, at::kInt) && lens.is_contiguous());
+    if (!a.ok) return;
+    REQUIRE(lens.size(0) <= 8192 && block > 0 && block <= 0x7fffffff);
+    REQUIRE(table.dim() == 2 && is(table, at::kInt) && table.size(0) == lens.size(0) && table.stride(1) == 1 && on(table, lens));
+    REQUIRE(table.size(0) <= 1 || table.stride(0) >= table.size(1));
+    REQUIRE(free.dim() == 1 && is(free, at::kInt) && free.is_contiguous() && on(free, lens));
+    REQUIRE(is_list(count, at::kInt, 1, lens));
+}
+
+// context_lens, new_lens, block_table, free_blocks, num_free, cache_block_size, num_tokens, then query_start_loc, seq_lens, position_ids, slot_mapping,
+// token_to_req_indices, num_free and num_missing of the result, or none of them -> True, or those in a tuple
+PyObject* extend_block_tables(Arguments& a) {
+    const Tensor *context = a.tensor(0), *fresh = a.tensor(1), *table = a.tensor(2), *free = a.tensor(3), *count = a.tensor(4);
+    const int64_t block = a.integer_of(5), tokens = a.integer_of(6);
+    if (!a.ok) Py_RETURN_NONE;
+    require_pool(a, *context, *table, *free, *count, block);
+    if (!a.ok) Py_RETURN_NONE;
+    const int64_t reqs = context->size(0);
+    REQUIRE(is_list(*fresh, at::kInt, reqs, *context) && tokens >= 0 && tokens <= 0x7fffffff);
+    if (!a.ok) Py_RETURN_NONE;
+    constexpr int kResults = 7;
+    const ScalarType types[kResults] = {at::kInt, at::kInt, at::kLong, at::kLong, at::kInt, at::kInt, at::kInt};
+    const int64_t sizes[kResults] = {reqs + 1, reqs, tokens, tokens, tokens, 1, 1};
+    const bool given = a.count > 7;
+    REQUIRE(!given || a.count == 7 + kResults);
+    if (!a.ok) Py_RETURN_NONE;
+    Tensor to[kResults];
+    if (given) {
+        for (int i = 0; i < kResults; ++i) {
+            const Tensor* t = a.tensor(7 + i);
+            if (!a.ok) Py_RETURN_NONE;
+            REQUIRE(is_list(*t, types[i], sizes[i], *context));
+            if (!a.ok) Py_RETURN_NONE;
+            to[i] = *t;
+        }
+        for (int i = 0; i < kResults; ++i) {
+            for (int k = 0; k < i; ++k) REQUIRE(!shares(to[i], to[k]));
+            REQUIRE(!shares(to[i], *table) && !shares(to[i], *free) && !shares(to[i], *fresh));
+            REQUIRE((i == 1 && to[i].data_ptr() == context->data_ptr()) || !shares(to[i], *context));
+            REQUIRE((i == 5 && to[i].data_ptr() == count->data_ptr()) || !shares(to[i], *count));
+        }
+    }
+    REQUIRE(!shares(*table, *context) && !shares(*table, *fresh) && !shares(*table, *free) && !shares(*table, *count));
+    if (!a.ok) Py_RETURN_NONE;
+    const OnDevice here = on_device_of(*context);
+    if (!given)
+        for (int i = 0; i < kResults; ++i) to[i] = make_empty({sizes[i]}, types[i], here);
+    if (!launch_on(here, [&](void* stream) {
+            return dsv4_extend_block_tables(ints(*context), ints(*fresh), reqs, ints(*table), table->stride(0), table->size(1), ints(*free), free->size(0),
+                                            ints(*count), block, tokens, ints(to[0]), ints(to[1]), longs(to[2]), longs(to[3]), ints(to[4]), ints(to[5]),
+                                            ints(to[6]), stream);
+        }))
+        return nullptr;
+    if (given) Py_RETURN_TRUE;
+    PyObject* result = PyTuple_New(kResults);
+    for (int i = 0; result && i < kResults; ++i) {
+        PyObject* t = wrap(std::move(to[i]));
+        if (t) PyTuple_SET_ITEM(result, i, t);
+        else Py_CLEAR(result);
+    }
+    return result;
+}
+
+// seq_lens, finished, block_table, free_blocks, num_free, cache_block_size, num_free of the result or None -> that
+PyObject* release_block_tables(Arguments& a) {
+    const Tensor *lens = a.tensor(0), *finished = a.tensor(1), *table = a.tensor(2), *free = a.tensor(3), *count = a.tensor(4);
+    const int64_t block = a.integer_of(5);
+    const Tensor* out = a.is_none(6) ? nullptr : a.tensor(6);
+    if (!a.ok) Py_RETURN_NONE;
+    require_pool(a, *lens, *table, *free, *count, block);
+    if (!a.ok) Py_RETURN_NONE;
+    REQUIRE(is_list(*finished, at::kBool, lens->size(0), *lens) && (!out || is_list(*out, at::kInt, 1, *lens)));
+    if (!a.ok) Py_RETURN_NONE;
+    REQUIRE(!shares(*free, *lens) && !shares(*free, *finished) && !shares(*free, *table) && !shares(*free, *count));
+    REQUIRE(!out || (!shares(*out, *lens) && !shares(*out, *finished) && !shares(*out, *table) && !shares(*out, *free)));
+    if (!a.ok) Py_RETURN_NONE;
+    const OnDevice here = on_device_of(*lens);
+    Tensor made = out ? *out : make_empty({1}, at::kInt, here);
+    if (!launch_on(here, [&](void* stream) {
+            return dsv4_release_block_tables(ints(*lens), static_cast<const uint8_t*>(finished->data_ptr()), lens->size(0), ints(*table), table->stride(0),
+                                             table->size(1), ints(*free), free->size(0), ints(*count), block, ints(made), stream);
+        }))
+        return nullptr;
     return wrap(std::move(made));
 }
 
@@ -752,6 +857,11 @@ PyMethodDef kMethods[] = {
     DSV4_ENTRY(add_rmsnorm_quant),
     DSV4_ENTRY(paged_latent_attention),
     DSV4_ENTRY(sparse_latent_attention),
+    DSV4_ENTRY(prologue_mxfp4),
+    DSV4_ENTRY(paged_latent_attention_mxfp4),
+    DSV4_ENTRY(sparse_latent_attention_mxfp4),
+    DSV4_ENTRY(extend_block_tables),
+    DSV4_ENTRY(release_block_tables),
     {"bind", bind, METH_O, nullptr},
     {"_refusal", refusal, METH_NOARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -49,39 +49,6 @@ __device__ __forceinline__ float load_weight(const uint8_t* base, int64_t idx, i
     return weight_value(dtype == 2 ? reinterpret_cast<const uint32_t*>(base)[idx] : reinterpret_cast<const uint16_t*>(base)[idx], dtype);
 }
 
-// UE8M0 byte of an MXFP4 block whose absolute maximum is `amax`: ceil(log2(max(amax, 6*2^-126) / 6)) + 127 clamped to
-// [0, 254], without the division: 6 = 1.5 * 4, so with the clamped maximum m * 2^(E-127), 1 <= m < 2, the quotient is
-// below, at or above 2^(E-129) for m below, at or above 1.5.  Equal to the log2/ceil statement for every bf16
-// maximum (a CPU test enumerates them).
-__device__ __forceinline__ uint32_t mxfp4_code(float amax) {
-    const uint32_t u = __float_as_uint(fmaxf(amax, 6.0f * 1.17549435e-38f));
-    const uint32_t code = (u >> 23) - 2u + ((u & 0x7fffffu) > 0x400000u ? 1u : 0u);
-    return code > 254u ? 254u : code;
-}
-
-// Two floats -> one byte of two e2m1 codes (lo in bits 0-3), round to nearest even, saturating at +-6.
-__device__ __forceinline__ uint32_t pack_e2m1x2(float lo, float hi) {
-    uint32_t r;
-    asm("{.reg .b8 t; cvt.rn.satfinite.e2m1x2.f32 t, %1, %2; cvt.u32.u8 %0, t;}" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
-// Four packed bf16 pairs times 2^(127 - code), the factor given as bf16 -> one word of eight e2m1 codes (element 0 in bits 0-3),
-// round to nearest even, saturating at +-6.  Exact before the conversion (scaled_pair()).
-__device__ __forceinline__ uint32_t pack_e2m1x8(const uint4& v, uint16_t factor) {
-    const float2 x0 = scaled_pair(v.x, factor), x1 = scaled_pair(v.y, factor), x2 = scaled_pair(v.z, factor), x3 = scaled_pair(v.w, factor);
-    uint32_t r;
-    asm("{.reg .b8 t0, t1, t2, t3;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 t0, %2, %1;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 t1, %4, %3;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 t2, %6, %5;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 t3, %8, %7;\n\t"
-        "mov.b32 %0, {t0, t1, t2, t3};}"
-        : "=r"(r)
-        : "f"(x0.x), "f"(x0.y), "f"(x1.x), "f"(x1.y), "f"(x2.x), "f"(x2.y), "f"(x3.x), "f"(x3.y));
-    return r;
-}
-
 // mxfp4_code() of the two magnitudes in a bf16 pair, in 16-bit fields: a mantissa above 0x40 (1.5) is one that carries into the
 // exponent when 0x3f is added.  The floor of the maximum is a bf16 value, 0x01c0 (a NaN becomes it, as in fmaxf).
 __device__ __forceinline__ uint32_t mxfp4_codes(uint32_t magnitudes) {

@@ -35,6 +35,7 @@
 // Other forms that were built: blocks of 64 keys in two stages, 6.9 ms; two groups of readers in turn, 4.5; eight softmax warps, 4.1 (this form then 3.9);
 // two CTAs that share out keys and exchange S and P, 128 rows a product: 5.0, since each exchange takes 400 cycles one way.
 #include <algorithm>
+#include <type_traits>
 
 #include "dsv4_common.cuh"
 #include "latent_attention.cuh"
@@ -437,6 +438,25 @@ __device__ __forceinline__ uint32_t two_values(uint32_t word, uint32_t scale) {
 // `codes` has the code twice, one in each half.
 __device__ __forceinline__ uint32_t power_of_codes(uint32_t codes) { return __vmaxu2(codes << 7, 0x400040u); }
 
+// The same, but 255 is NaN.
+__device__ __forceinline__ uint32_t power_of_mx_codes(uint32_t codes) { return power_of_codes(codes) | (((codes + 0x00010001u) >> 2) & 0x00400040u); }
+
+// Eight e2m1 values (the first in the low bits) times a power of two.
+__device__ __forceinline__ uint4 eight_values(uint32_t word, uint32_t scale) {
+    uint32_t h[4], v[4];
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+        : "r"(word));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float lo, hi;
+        asm("{.reg .f16 l, h; mov.b32 {l, h}, %2; cvt.f32.f16 %0, l; cvt.f32.f16 %1, h;}" : "=f"(lo), "=f"(hi) : "r"(h[i]));
+        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(v[i]) : "r"(pack_bf16x2(lo, hi)), "r"(scale));
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
 // Whether one of a bf16 pair is infinite or NaN.
 __device__ __forceinline__ bool not_finite(uint32_t pair) { return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u; }
 __device__ __forceinline__ bool not_finite(const uint4& v) { return not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w); }
@@ -456,7 +476,10 @@ __device__ __forceinline__ void set_registers() {
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(COUNT));
 }
 
+// MX: the cache in 4 bits.
+template <bool MX>
 __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Launched<Tiles> p) {
+    constexpr int kDataBytes = MX ? kMxTokenDataBytes : kTokenDataBytes, kCodeBytes = MX ? kMxScaleBytes : kScaleBytes;
     extern __shared__ __align__(1024) uint8_t shared[];
     Rest& rest = *reinterpret_cast<Rest*>(shared + kOffsetRest);
     const uint32_t base = shared_address(shared);
@@ -724,12 +747,20 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
         const uint32_t store_row = base + kOffsetKeys + key_a * 128, unit = 2 * (sub & 3);
         const bool coded = sub < 12;
         const int rotary_sub = sub ^ (8 * odd);  // (the two keys' halves, so that their stores use different banks)
-        const uint32_t code_select = 0x4040u + 0x0101u * (sub >> 2);  // of a byte and of zeros: the byte in both halves
-        // 16 e4m3 values to two 16-byte columns
-        const auto convert = [&](const uint4& v, uint32_t code_word, uint4& a, uint4& b) {
-            const uint32_t scale = power_of_codes(__byte_perm(code_word, 0u, code_select));
-            a = make_uint4(two_values<0>(v.x, scale), two_values<1>(v.x, scale), two_values<0>(v.y, scale), two_values<1>(v.y, scale));
-            b = make_uint4(two_values<0>(v.z, scale), two_values<1>(v.z, scale), two_values<0>(v.w, scale), two_values<1>(v.w, scale));
+        // of a byte of a code word and of zeros: the byte in both halves
+        const uint32_t code_select = 0x4040u + 0x0101u * (MX ? (sub >> 1) & 3 : sub >> 2);
+        // 16 cached values to two 16-byte columns
+        using Values = std::conditional_t<MX, uint2, uint4>;
+        const auto convert = [&](const Values& v, uint32_t code_word, uint4& a, uint4& b) {
+            const uint32_t codes = __byte_perm(code_word, 0u, code_select);
+            if constexpr (MX) {
+                const uint32_t scale = power_of_mx_codes(codes);
+                a = eight_values(v.x, scale), b = eight_values(v.y, scale);
+            } else {
+                const uint32_t scale = power_of_codes(codes);
+                a = make_uint4(two_values<0>(v.x, scale), two_values<1>(v.x, scale), two_values<0>(v.y, scale), two_values<1>(v.y, scale));
+                b = make_uint4(two_values<0>(v.z, scale), two_values<1>(v.z, scale), two_values<0>(v.w, scale), two_values<1>(v.w, scale));
+            }
         };
         uint32_t to[2][2], to_rotary[2];  // where this lane's values of the two keys go: 16-byte columns of the first half's chunk, and the rotary ones
 #pragma unroll
@@ -753,15 +784,23 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
             for (int i = 0; i < 2; ++i) at[i] = rest.keys[entry][key_a + 2 * i];
             __syncwarp();
             if (lane == 0) barrier_arrive(&rest.look_empty[entry]);
-            uint4 low[2], high[2];
-            uint2 rotary[2], codes[2];
+            Values low[2], high[2];
+            uint2 rotary[2], codes[2];  // (the code words of `low` and of `high`)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const uint8_t* data = reinterpret_cast<const uint8_t*>(at[i].x);
-                codes[i] = __ldg(reinterpret_cast<const uint2*>(at[i].y));
-                low[i] = ld_stream16(data + 16 * sub);
-                if (coded) high[i] = ld_stream16(data + 256 + 16 * sub);
-                rotary[i] = __ldg(reinterpret_cast<const uint2*>(data + kNopeDim + 8 * rotary_sub));
+                if constexpr (MX) {
+                    const uint32_t* code = reinterpret_cast<const uint32_t*>(at[i].y) + (sub >> 3);
+                    codes[i] = make_uint2(__ldg(code), __ldg(code + 2));
+                    low[i] = ld_stream8(data + 8 * sub);
+                    if (coded) high[i] = ld_stream8(data + 128 + 8 * sub);
+                    rotary[i] = __ldg(reinterpret_cast<const uint2*>(data + kMxNopeBytes + 8 * rotary_sub));
+                } else {
+                    codes[i] = __ldg(reinterpret_cast<const uint2*>(at[i].y));
+                    low[i] = ld_stream16(data + 16 * sub);
+                    if (coded) high[i] = ld_stream16(data + 256 + 16 * sub);
+                    rotary[i] = __ldg(reinterpret_cast<const uint2*>(data + kNopeDim + 8 * rotary_sub));
+                }
             }
             if (!warp_wait(&rest.kv_empty[stage], phase, limit)) break;
             uint32_t none = ~valid;  // keys of this warp that are stored as zeros
@@ -787,7 +826,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
             if ((none & 0xfu) != 0) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    if ((none >> (2 * i + odd)) & 1u) low[i] = high[i] = make_uint4(0u, 0u, 0u, 0u), rotary[i] = codes[i] = make_uint2(0u, 0u);
+                    if ((none >> (2 * i + odd)) & 1u) low[i] = high[i] = Values{}, rotary[i] = codes[i] = make_uint2(0u, 0u);
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -873,7 +912,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
         // Keys lane and lane + 32 of each block.  Keys that do not exist are given q as their place, and zeroed when they have been read.
         bool ok = true;
         int it = 0;
-        const int64_t codes_from = static_cast<int64_t>(p.a.block_size) * kTokenDataBytes;
+        const int64_t codes_from = static_cast<int64_t>(p.a.block_size) * kDataBytes;
         for (; ok && w.settle(p); w.step(p)) {
             const Tile& t = w.tile;
             for (int block = w.begin; block < w.end; ++block, ++it) {
@@ -900,8 +939,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                     }
                     const bool there = number >= 0 && number < p.a.num_blocks;
                     const uint8_t* block_at = p.a.k_cache + number * p.a.block_stride;
-                    at[i].x = reinterpret_cast<uint64_t>(there ? block_at + static_cast<int64_t>(in_block) * kTokenDataBytes : p.a.q);
-                    at[i].y = reinterpret_cast<uint64_t>(there ? block_at + codes_from + static_cast<int64_t>(in_block) * kScaleBytes : p.a.q);
+                    at[i].x = reinterpret_cast<uint64_t>(there ? block_at + static_cast<int64_t>(in_block) * kDataBytes : p.a.q);
+                    at[i].y = reinterpret_cast<uint64_t>(there ? block_at + codes_from + static_cast<int64_t>(in_block) * kCodeBytes : p.a.q);
                     exist |= static_cast<uint64_t>(__ballot_sync(0xffffffffu, there)) << (32 * i);
                 }
                 ok = warp_wait(&rest.look_empty[entry], ((it >> 1) - 1) & 1, limit);
@@ -1078,7 +1117,8 @@ constexpr size_t kSumBytes = sizeof(float) * 2 * kMaxCtas * kRows * kHeadDim, kR
 
 size_t latent_attention_workspace(int64_t, int64_t) { return kSumBytes + kRowBytes2 + sizeof(int4) * 2 * kMaxCtas; }
 
-cudaError_t launch_latent_attention(const LatentAttention& a, void* workspace, cudaStream_t stream) {
+cudaError_t launch_latent_attention(const LatentAttention& a, bool mxfp4, void* workspace, cudaStream_t stream) {
+    const auto kernel = mxfp4 ? latent_attention_kernel<true> : latent_attention_kernel<false>;
     Tiles p{};
     p.a = a;
     p.lists = Lists{a.query_start_loc, a.indices ? a.lens : a.seq_lens};
@@ -1092,9 +1132,9 @@ cudaError_t launch_latent_attention(const LatentAttention& a, void* workspace, c
     auto* at = static_cast<uint8_t*>(workspace);
     p.sums = reinterpret_cast<float*>(at), p.rows = reinterpret_cast<float2*>(at + kSumBytes), p.pieces = reinterpret_cast<int4*>(at + kSumBytes + kRowBytes2);
     // Set for the current device each time: cheaper than to remember for which ones it was.
-    cudaError_t rc = cudaFuncSetAttribute(latent_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedBytes);
+    cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedBytes);
     if (rc != cudaSuccess) return rc;
-    rc = launch_dependent_cluster(latent_attention_kernel, dim3(kMaxCtas), dim3(kThreads), 1, kSharedBytes, stream, p);
+    rc = launch_dependent_cluster(kernel, dim3(kMaxCtas), dim3(kThreads), 1, kSharedBytes, stream, p);
     if (rc != cudaSuccess) return rc;
     count_launch();
     if (!may_split) return cudaGetLastError();

@@ -34,7 +34,7 @@ struct LatentAttention {
 constexpr uint32_t kMostWaitRetries = 1u << 22;  // the default: of up to two microseconds each, some seconds in all
 
 size_t latent_attention_workspace(int64_t num_tokens, int64_t num_heads);
-cudaError_t launch_latent_attention(const LatentAttention& p, void* workspace, cudaStream_t stream);
+cudaError_t launch_latent_attention(const LatentAttention& p, bool mxfp4, void* workspace, cudaStream_t stream);
 cudaError_t read_attention_error(int* value);
 
 }  // namespace dsv4

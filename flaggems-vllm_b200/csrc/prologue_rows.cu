@@ -22,7 +22,8 @@ namespace {
 // it every warp fetches position and table row of its own rows straight into registers (lane i holds cosine i and
 // sine i): 256 more bytes from L2 per row, but no barrier and no shared-memory round trip in the dependent chain
 // position -> table row, which is what a launch of a few waves waits for.
-template <int RPW, int WARPS, int MIN_CTAS, bool CHECKED, bool PADDED, int PDL = 0, bool STAGED = true>
+// MXFP4: the latent rows go to a cache in 4 bits.
+template <int RPW, int WARPS, int MIN_CTAS, bool CHECKED, bool PADDED, int PDL = 0, bool STAGED = true, bool MXFP4 = false>
 __global__ void __launch_bounds__(WARPS * 32, MIN_CTAS) prologue_rows_kernel(const Launched<PrologueParams, sizeof(int64_t)> p, const int64_t kv_ctas) {
     static_assert(STAGED || !CHECKED, "the range-checked build marks bad tokens in shared memory");
     constexpr int TILE = RPW * WARPS;
@@ -84,8 +85,12 @@ __global__ void __launch_bounds__(WARPS * 32, MIN_CTAS) prologue_rows_kernel(con
         if (PDL) let_next_kernel_start();
         const int64_t block = slot / p.block_size, in_block = slot - block * p.block_size;
         uint8_t* base = p.k_cache + block * p.block_stride;
-        kv_row_to_cache(a, b, lane, c, s, base + in_block * kTokenDataBytes,
-                        base + p.block_size * kTokenDataBytes + in_block * kScaleBytes, p.cache_aligned16 != 0);
+        if constexpr (MXFP4)
+            kv_row_to_cache_mxfp4(a, b, lane, c, s, base + in_block * kMxTokenDataBytes,
+                                  base + p.block_size * kMxTokenDataBytes + in_block * kMxScaleBytes, p.cache_aligned16 != 0);
+        else
+            kv_row_to_cache(a, b, lane, c, s, base + in_block * kTokenDataBytes,
+                            base + p.block_size * kTokenDataBytes + in_block * kScaleBytes, p.cache_aligned16 != 0);
         return;
     }
 
@@ -199,7 +204,7 @@ __global__ void __launch_bounds__(WARPS * 32, MIN_CTAS) prologue_rows_kernel(con
 // the lane's rotary pair and the pairs l + 32g are one quantisation group g of a latent-KV row.  Same arithmetic as the
 // kernels above (the sum of squares is grouped differently, within the freedom the mean has anyway); cache bytes are
 // identical.  Only this plain form exists for such pointers: no range-checked and no out-of-place variant.
-template <int WARPS>
+template <int WARPS, bool MXFP4>
 __global__ void __launch_bounds__(WARPS * 32) prologue_rows_any_alignment_kernel(const Launched<PrologueParams, sizeof(int64_t)> p, const int64_t kv_ctas) {
     const int lane = threadIdx.x & 31;
     const int warp = threadIdx.x >> 5;
@@ -243,6 +248,26 @@ __global__ void __launch_bounds__(WARPS * 32) prologue_rows_any_alignment_kernel
     }
     const int64_t block = slot / p.block_size, in_block = slot - block * p.block_size;
     uint8_t* base = p.k_cache + block * p.block_stride;
+    const uint32_t rot = pack_bf16x2(__fsub_rn(__fmul_rn(e[7], c), __fmul_rn(o[7], sn)), __fadd_rn(__fmul_rn(e[7], sn), __fmul_rn(o[7], c)));
+    if constexpr (MXFP4) {
+        // pairs l + 32g are two groups of 32 values, one in each half of the warp
+        uint8_t* data = base + in_block * kMxTokenDataBytes;
+        uint8_t* scales = base + p.block_size * kMxTokenDataBytes + in_block * kMxScaleBytes;
+#pragma unroll
+        for (int g = 0; g < 7; ++g) {
+            uint32_t top = max(__float_as_uint(fabsf(e[g])), __float_as_uint(fabsf(o[g])));
+#pragma unroll
+            for (int m = 8; m > 0; m >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, m));
+            const uint32_t code = mxfp4_cache_code(top);
+            const float factor = __uint_as_float(pow2_reciprocal(code) << 16);
+            data[32 * g + lane] = static_cast<uint8_t>(code == 255u ? 0u : pack_e2m1x2(__fmul_rn(e[g], factor), __fmul_rn(o[g], factor)));
+            if ((lane & 15) == 0) scales[2 * g + (lane >> 4)] = static_cast<uint8_t>(code);
+        }
+        if (lane < 2) scales[14 + lane] = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) data[kMxNopeBytes + 4 * lane + b] = static_cast<uint8_t>((rot >> (8 * b)) & 0xffu);
+        return;
+    }
     uint8_t* data = base + in_block * kTokenDataBytes;
     uint8_t* scales = base + p.block_size * kTokenDataBytes + in_block * kScaleBytes;
 #pragma unroll
@@ -258,12 +283,11 @@ __global__ void __launch_bounds__(WARPS * 32) prologue_rows_any_alignment_kernel
         if (lane == 0) scales[g] = static_cast<uint8_t>(code);
     }
     if (lane == 0) scales[7] = 0;
-    const uint32_t rot = pack_bf16x2(__fsub_rn(__fmul_rn(e[7], c), __fmul_rn(o[7], sn)), __fadd_rn(__fmul_rn(e[7], sn), __fmul_rn(o[7], c)));
 #pragma unroll
     for (int b = 0; b < 4; ++b) data[kNopeDim + 4 * lane + b] = static_cast<uint8_t>((rot >> (8 * b)) & 0xffu);
 }
 
-template <int RPW, int WARPS, int MIN_CTAS>
+template <int RPW, int WARPS, int MIN_CTAS, bool MXFP4 = false>
 cudaError_t launch(const PrologueParams& p, bool checked, cudaStream_t stream) {
     constexpr int TILE = RPW * WARPS;
     const int64_t kv_ctas = (p.num_tokens_insert + WARPS - 1) / WARPS;
@@ -273,12 +297,13 @@ cudaError_t launch(const PrologueParams& p, bool checked, cudaStream_t stream) {
     if (grid == 0) return cudaSuccess;
     if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
     if (checked) {
-        prologue_rows_kernel<RPW, WARPS, MIN_CTAS, true, false><<<static_cast<unsigned>(grid), WARPS * 32, 0, stream>>>(p, kv_ctas);
+        if constexpr (MXFP4) return cudaErrorNotSupported;
+        else prologue_rows_kernel<RPW, WARPS, MIN_CTAS, true, false><<<static_cast<unsigned>(grid), WARPS * 32, 0, stream>>>(p, kv_ctas);
     } else if (p.pdl) {
-        const auto kernel = p.pdl == 2 ? (p.table_staging ? prologue_rows_kernel<RPW, WARPS, MIN_CTAS, false, false, 2, true>
-                                                          : prologue_rows_kernel<RPW, WARPS, MIN_CTAS, false, false, 2, false>)
-                                       : (p.table_staging ? prologue_rows_kernel<RPW, WARPS, MIN_CTAS, false, false, 1, true>
-                                                          : prologue_rows_kernel<RPW, WARPS, MIN_CTAS, false, false, 1, false>);
+        const auto kernel = p.pdl == 2 ? (p.table_staging ? prologue_rows_kernel<RPW, WARPS, MIN_CTAS, false, false, 2, true, MXFP4>
+                                                          : prologue_rows_kernel<RPW, WARPS, MIN_CTAS, false, false, 2, false, MXFP4>)
+                                       : (p.table_staging ? prologue_rows_kernel<RPW, WARPS, MIN_CTAS, false, false, 1, true, MXFP4>
+                                                          : prologue_rows_kernel<RPW, WARPS, MIN_CTAS, false, false, 1, false, MXFP4>);
         cudaLaunchConfig_t config = {};
         config.gridDim = dim3(static_cast<unsigned>(grid)), config.blockDim = dim3(WARPS * 32), config.stream = stream;
         cudaLaunchAttribute attribute[1];
@@ -288,9 +313,9 @@ cudaError_t launch(const PrologueParams& p, bool checked, cudaStream_t stream) {
         const cudaError_t err = cudaLaunchKernelEx(&config, kernel, p, kv_ctas);
         if (err != cudaSuccess) return err;
     } else if (p.table_staging) {
-        prologue_rows_kernel<RPW, WARPS, MIN_CTAS, false, false><<<static_cast<unsigned>(grid), WARPS * 32, 0, stream>>>(p, kv_ctas);
+        prologue_rows_kernel<RPW, WARPS, MIN_CTAS, false, false, 0, true, MXFP4><<<static_cast<unsigned>(grid), WARPS * 32, 0, stream>>>(p, kv_ctas);
     } else {
-        prologue_rows_kernel<RPW, WARPS, MIN_CTAS, false, false, 0, false><<<static_cast<unsigned>(grid), WARPS * 32, 0, stream>>>(p, kv_ctas);
+        prologue_rows_kernel<RPW, WARPS, MIN_CTAS, false, false, 0, false, MXFP4><<<static_cast<unsigned>(grid), WARPS * 32, 0, stream>>>(p, kv_ctas);
     }
     count_launch();
     return cudaGetLastError();
@@ -310,17 +335,22 @@ cudaError_t launch_padded(const PrologueParams& p, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
-}  // namespace
-
-cudaError_t launch_prologue_rows_any_alignment(const PrologueParams& p, cudaStream_t stream) {
+template <bool MXFP4>
+cudaError_t launch_any_alignment(const PrologueParams& p, cudaStream_t stream) {
     constexpr int WARPS = 4;
     const int64_t kv_ctas = (p.num_tokens_insert + WARPS - 1) / WARPS;
     const int64_t grid = kv_ctas + (p.num_tokens * p.num_heads + WARPS - 1) / WARPS;
     if (grid == 0) return cudaSuccess;
     if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-    prologue_rows_any_alignment_kernel<WARPS><<<static_cast<unsigned>(grid), WARPS * 32, 0, stream>>>(p, kv_ctas);
+    prologue_rows_any_alignment_kernel<WARPS, MXFP4><<<static_cast<unsigned>(grid), WARPS * 32, 0, stream>>>(p, kv_ctas);
     count_launch();
     return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_prologue_rows_any_alignment(const PrologueParams& p, bool mxfp4, cudaStream_t stream) {
+    return mxfp4 ? launch_any_alignment<true>(p, stream) : launch_any_alignment<false>(p, stream);
 }
 
 cudaError_t launch_prologue_rows(const PrologueParams& p, bool checked, cudaStream_t stream) {
@@ -331,6 +361,9 @@ cudaError_t launch_prologue_rows(const PrologueParams& p, bool checked, cudaStre
     return launch<2, 4, 10>(p, checked, stream);
 #endif
 }
+
+// The same shape: at the sizes where its speed matters, all but the first 1 in 8 to 128 of its CTAs are those of q.
+cudaError_t launch_prologue_rows_mxfp4(const PrologueParams& p, cudaStream_t stream) { return launch<2, 4, 10, true>(p, false, stream); }
 
 cudaError_t launch_prologue_rows_padded(const PrologueParams& p, cudaStream_t stream) { return launch_padded<2, 4, 10>(p, stream); }
 

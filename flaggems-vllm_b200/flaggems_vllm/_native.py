@@ -16,6 +16,7 @@ HOST_CALLS_PATH = LIB_PATH.parent / "_host_calls.so"
 EXPORTS = (
     "dsv4_qnorm_rope_kv_insert",
     "dsv4_qnorm_rope_kv_insert_checked",
+    "dsv4_qnorm_rope_kv_insert_mxfp4",
     "dsv4_qnorm_rope_kv_insert_padded",
     "dsv4_gather_dequant_k_cache",
     "dsv4_dequantize_and_gather_k_cache",
@@ -33,6 +34,10 @@ EXPORTS = (
     "dsv4_latent_attention_workspace_bytes",
     "dsv4_paged_latent_attention",
     "dsv4_sparse_latent_attention",
+    "dsv4_paged_latent_attention_mxfp4",
+    "dsv4_sparse_latent_attention_mxfp4",
+    "dsv4_extend_block_tables",
+    "dsv4_release_block_tables",
     "dsv4_top_k_per_row_decode",
     "dsv4_top_k_per_row_prefill",
     "dsv4_fused_indexer_q_rope_quant",

@@ -11,12 +11,14 @@ from .fused_deepseek_v4_qnorm_rope_kv_rope_quant_insert import (
     fused_deepseek_v4_qnorm_rope_kv_rope_quant_insert_checked,
     fused_deepseek_v4_qnorm_rope_kv_rope_quant_insert_padded,
 )
+from .fused_deepseek_v4_qnorm_rope_kv_rope_mxfp4_insert import fused_deepseek_v4_qnorm_rope_kv_rope_mxfp4_insert
 from .fused_indexer_q_rope_quant import fused_indexer_q_rope_quant
 from .fused_inv_rope_fp8_quant import fused_inv_rope_fp8_quant
 from .gather_dequant_k_cache import gather_dequant_k_cache_slots
 from .host_staged import HostStagedPrologue
 from .indexer_k_quant_and_cache import indexer_k_quant_and_cache
-from .latent_attention import paged_latent_attention, sparse_latent_attention
+from .latent_attention import paged_latent_attention, paged_latent_attention_mxfp4, sparse_latent_attention, sparse_latent_attention_mxfp4
+from .paged_batch import PagedBatch, extend_block_tables, release_block_tables
 from .per_token_group_quant_fp8 import per_token_group_quant_fp8
 from .persistent_topk import persistent_topk
 from .top_k_per_row_decode import top_k_per_row_decode
@@ -26,6 +28,12 @@ __all__ = [
     "fused_add_rmsnorm_quant_fp8",
     "paged_latent_attention",
     "sparse_latent_attention",
+    "fused_deepseek_v4_qnorm_rope_kv_rope_mxfp4_insert",
+    "paged_latent_attention_mxfp4",
+    "sparse_latent_attention_mxfp4",
+    "PagedBatch",
+    "extend_block_tables",
+    "release_block_tables",
     "fused_indexer_q_rope_quant",
     "indexer_k_quant_and_cache",
     "cp_gather_indexer_k_quant_cache",

@@ -17,6 +17,9 @@ A cached row of 512 values, shared by all heads, is key and value at once.  Per 
 Scores, sums and both products' accumulators are of 32 bits, cached keys exactly what the cache holds.  The weights exp(s_j) are rounded to bfloat16, in which the
 second product takes them (2^-8 of each; their sum is that of the unrounded ones), the exponentials are the hardware's (2^-21), and `out` is rounded once.
 
+`paged_latent_attention_mxfp4` and `sparse_latent_attention_mxfp4` are the same over the cache in 4 bits that
+`fused_deepseek_v4_qnorm_rope_kv_rope_mxfp4_insert` writes (368 bytes a token instead of 584); a scale code of 255 makes its 32 values NaN.
+
 q is bfloat16 [tokens, heads, 512] with unit inner stride, any number of heads; rows, cache and cache blocks on 16-byte boundaries.  `out`
 (like q) and `lse` (float32 [tokens, heads]) are written where given; `out` is allocated otherwise, and returned.  Neither may share memory with the
 other or with an argument that is read.
@@ -36,15 +39,16 @@ import torch
 from .. import _native
 from ..utils.memory import apart, rows_apart
 
-HEAD_DIM, TOKEN_BYTES = 512, 584
+HEAD_DIM, TOKEN_BYTES, TOKEN_BYTES_MXFP4 = 512, 584, 368
 
-_paged = _sparse = None  # the native front ends, looked up once
+_paged = _sparse = _paged_mxfp4 = _sparse_mxfp4 = None  # the native front ends, looked up once
 
 
 def _bind():
-    global _paged, _sparse
+    global _paged, _sparse, _paged_mxfp4, _sparse_mxfp4
     calls = _native.host_calls()
     _paged, _sparse = calls.paged_latent_attention, calls.sparse_latent_attention
+    _paged_mxfp4, _sparse_mxfp4 = calls.paged_latent_attention_mxfp4, calls.sparse_latent_attention_mxfp4
 
 
 def paged_latent_attention(
@@ -67,15 +71,8 @@ def paged_latent_attention(
                     attn_sink, out, lse)
     if result is not None:
         return result
-    _check(q, k_cache, cache_block_size, softmax_scale, attn_sink, out, lse)
-    requests = seq_lens.shape[0]
-    for name, t, dims in (("block_table", block_table, 2), ("seq_lens", seq_lens, 1), ("query_start_loc", query_start_loc, 1)):
-        assert t.dtype == torch.int32 and t.dim() == dims, f"{name}: int32 of {dims} dimensions"
-        assert t.device == q.device, "all tensors must be on the same device"
-    assert block_table.stride(1) == 1 and seq_lens.is_contiguous() and query_start_loc.is_contiguous(), "indices with unit stride"
-    assert block_table.shape[0] == requests and query_start_loc.shape[0] == requests + 1, "a row of block_table and a start per request, and the end"
-    assert window_size is None or int(window_size) >= 1, "a window of at least one token, or None"
-    assert int(num_first_tokens) >= 0
+    _check_paged(q, k_cache, block_table, seq_lens, query_start_loc, cache_block_size, softmax_scale, window_size, num_first_tokens, attn_sink,
+                 out, lse, TOKEN_BYTES)
     _native.refuse()
 
 
@@ -95,19 +92,81 @@ def sparse_latent_attention(
     result = _sparse(q, k_cache, indices, lens, cache_block_size, softmax_scale, attn_sink, out, lse)
     if result is not None:
         return result
-    _check(q, k_cache, cache_block_size, softmax_scale, attn_sink, out, lse)
+    _check_sparse(q, k_cache, indices, lens, cache_block_size, softmax_scale, attn_sink, out, lse, TOKEN_BYTES)
+    _native.refuse()
+
+
+def paged_latent_attention_mxfp4(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    cache_block_size: int,
+    softmax_scale: float,
+    window_size: Optional[int] = None,
+    num_first_tokens: int = 0,
+    attn_sink: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+    lse: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    if _paged_mxfp4 is None:
+        _bind()
+    result = _paged_mxfp4(q, k_cache, block_table, seq_lens, query_start_loc, cache_block_size, softmax_scale, window_size,
+                          num_first_tokens, attn_sink, out, lse)
+    if result is not None:
+        return result
+    _check_paged(q, k_cache, block_table, seq_lens, query_start_loc, cache_block_size, softmax_scale, window_size, num_first_tokens, attn_sink,
+                 out, lse, TOKEN_BYTES_MXFP4)
+    _native.refuse()
+
+
+def sparse_latent_attention_mxfp4(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    indices: torch.Tensor,
+    lens: torch.Tensor,
+    cache_block_size: int,
+    softmax_scale: float,
+    attn_sink: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+    lse: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    if _sparse_mxfp4 is None:
+        _bind()
+    result = _sparse_mxfp4(q, k_cache, indices, lens, cache_block_size, softmax_scale, attn_sink, out, lse)
+    if result is not None:
+        return result
+    _check_sparse(q, k_cache, indices, lens, cache_block_size, softmax_scale, attn_sink, out, lse, TOKEN_BYTES_MXFP4)
+    _native.refuse()
+
+
+def _check_paged(q, k_cache, block_table, seq_lens, query_start_loc, cache_block_size, softmax_scale, window_size, num_first_tokens, attn_sink,
+                 out, lse, token_bytes):
+    _check(q, k_cache, cache_block_size, softmax_scale, attn_sink, out, lse, token_bytes)
+    requests = seq_lens.shape[0]
+    for name, t, dims in (("block_table", block_table, 2), ("seq_lens", seq_lens, 1), ("query_start_loc", query_start_loc, 1)):
+        assert t.dtype == torch.int32 and t.dim() == dims, f"{name}: int32 of {dims} dimensions"
+        assert t.device == q.device, "all tensors must be on the same device"
+    assert block_table.stride(1) == 1 and seq_lens.is_contiguous() and query_start_loc.is_contiguous(), "indices with unit stride"
+    assert block_table.shape[0] == requests and query_start_loc.shape[0] == requests + 1, "a row of block_table and a start per request, and the end"
+    assert window_size is None or int(window_size) >= 1, "a window of at least one token, or None"
+    assert int(num_first_tokens) >= 0
+
+
+def _check_sparse(q, k_cache, indices, lens, cache_block_size, softmax_scale, attn_sink, out, lse, token_bytes):
+    _check(q, k_cache, cache_block_size, softmax_scale, attn_sink, out, lse, token_bytes)
     assert indices.dtype == torch.int32 and indices.dim() == 2 and indices.stride(1) == 1, "indices: int32 [tokens, k] with unit inner stride"
     assert lens.dtype == torch.int32 and lens.dim() == 1 and lens.is_contiguous(), "lens: int32 [tokens]"
     assert indices.shape[0] == q.shape[0] and lens.shape[0] == q.shape[0], "a row of indices and a length per token"
     assert indices.device == q.device and lens.device == q.device, "all tensors must be on the same device"
-    _native.refuse()
 
 
-def _check(q, k_cache, cache_block_size, softmax_scale, attn_sink, out, lse):
+def _check(q, k_cache, cache_block_size, softmax_scale, attn_sink, out, lse, token_bytes):
     assert q.device.type == "cuda", "this operator has no CPU path"
     assert q.dim() == 3 and q.shape[2] == HEAD_DIM and q.dtype == torch.bfloat16 and q.stride(2) == 1, "q: bfloat16 [tokens, heads, 512]"
     assert k_cache.dtype == torch.uint8 and k_cache.dim() == 2 and k_cache.stride(1) == 1, "k_cache: uint8 [blocks, bytes]"
-    assert int(cache_block_size) > 0 and k_cache.shape[1] // TOKEN_BYTES >= int(cache_block_size), "a cache block holds cache_block_size tokens of 584 bytes"
+    assert int(cache_block_size) > 0 and k_cache.shape[1] // token_bytes >= int(cache_block_size), f"a cache block holds cache_block_size tokens of {token_bytes} bytes"
     assert k_cache.shape[0] <= 1 or k_cache.stride(0) >= k_cache.shape[1], "cache blocks must not overlap"
     scale = torch.tensor(float(softmax_scale), dtype=torch.float32)
     assert scale > 0 and torch.isfinite(scale * 1.4426950408889634), "a positive softmax_scale, and in 32 bits a number also when it is divided by ln 2"
@@ -125,4 +184,4 @@ def _check(q, k_cache, cache_block_size, softmax_scale, attn_sink, out, lse):
         assert lse is None or rows_apart(lse), "lse must not overlap itself"
 
 
-__all__ = ["paged_latent_attention", "sparse_latent_attention"]
+__all__ = ["paged_latent_attention", "paged_latent_attention_mxfp4", "sparse_latent_attention", "sparse_latent_attention_mxfp4"]

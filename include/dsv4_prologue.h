@@ -36,6 +36,9 @@ extern "C" {
 #define DSV4_NOPE_DIM 448
 #define DSV4_TOKEN_DATA_BYTES 576 /* 448 e4m3 + 64 bf16 */
 #define DSV4_SCALE_BYTES 8        /* 7 UE8M0 codes + 1 zero byte */
+/* The same of the cache in 4 bits (MXFP4). */
+#define DSV4_MX_TOKEN_DATA_BYTES 352 /* 448 e2m1 values, two a byte + 64 bf16 */
+#define DSV4_MX_SCALE_BYTES 16       /* 14 UE8M0 codes + 2 zero bytes */
 
 /* Kernel variants selectable with dsv4_set_variant (0 = choose by problem size). */
 #define DSV4_VARIANT_AUTO 0
@@ -67,6 +70,19 @@ int dsv4_qnorm_rope_kv_insert(void* q, const void* kv, void* k_cache, const int6
                               const int64_t* position_ids, const float* cos_sin_cache, float eps,
                               int64_t num_tokens, int64_t num_heads, int64_t num_tokens_insert,
                               int64_t cache_block_size, int64_t kv_block_stride_bytes, void* cuda_stream);
+
+/*
+ * The same for a cache in 4 bits (MXFP4), 368 bytes a token instead of 584: block b holds cache_block_size records of 352 bytes
+ * (448 e2m1 values in 224 bytes, value 2i in the low and 2i + 1 in the high four bits of byte i, then 64 rotated bf16 values) and then
+ * cache_block_size groups of 16 scale bytes (14 UE8M0 codes, one for 32 values each, and two zeros):
+ *   code = ceil(log2(max(amax, 6 * 2^-126) / 6)) + 127,  value = e2m1(x / 2^(code - 127)), to nearest, ties to even
+ * A group with an infinity or a NaN, which e2m1 does not have, gets the code 255 (NaN) and zeros: its readers make all of it NaN.
+ * q, the rotation, skipped tokens, alignments and what is not checked: as above.  Always the DSV4_VARIANT_ROWS kernel.  No counterpart in
+ * the reference.
+ */
+int dsv4_qnorm_rope_kv_insert_mxfp4(void* q, const void* kv, void* k_cache, const int64_t* slot_mapping, const int64_t* position_ids,
+                                    const float* cos_sin_cache, float eps, int64_t num_tokens, int64_t num_heads, int64_t num_tokens_insert,
+                                    int64_t cache_block_size, int64_t kv_block_stride_bytes, void* cuda_stream);
 
 /*
  * Out-of-place form with head padding: q [num_tokens, num_heads, 512] is read only, the normalised and
@@ -376,6 +392,48 @@ int dsv4_sparse_latent_attention(const void* q, int64_t q_stride_token, int64_t 
                                  int64_t topk, const int32_t* lens, const float* attn_sink, float softmax_scale, void* out,
                                  int64_t out_stride_token, int64_t out_stride_head, float* lse, int64_t lse_stride_token,
                                  int64_t lse_stride_head, int64_t num_tokens, int64_t num_heads, void* workspace, void* cuda_stream);
+
+/* The same over the cache in 4 bits that dsv4_qnorm_rope_kv_insert_mxfp4 writes.  A scale code of 255 makes its 32 values NaN. */
+int dsv4_paged_latent_attention_mxfp4(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_cache, int64_t num_blocks,
+                                      int64_t kv_block_stride_bytes, int64_t cache_block_size, const int32_t* block_table,
+                                      int64_t block_table_stride, int64_t max_blocks_per_seq, const int32_t* seq_lens,
+                                      const int32_t* query_start_loc, int64_t num_reqs, int64_t window_size, int64_t num_first_tokens,
+                                      const float* attn_sink, float softmax_scale, void* out, int64_t out_stride_token, int64_t out_stride_head,
+                                      float* lse, int64_t lse_stride_token, int64_t lse_stride_head, int64_t num_tokens, int64_t num_heads,
+                                      void* workspace, void* cuda_stream);
+int dsv4_sparse_latent_attention_mxfp4(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_cache, int64_t num_blocks,
+                                       int64_t kv_block_stride_bytes, int64_t cache_block_size, const int32_t* indices, int64_t indices_stride,
+                                       int64_t topk, const int32_t* lens, const float* attn_sink, float softmax_scale, void* out,
+                                       int64_t out_stride_token, int64_t out_stride_head, float* lse, int64_t lse_stride_token,
+                                       int64_t lse_stride_head, int64_t num_tokens, int64_t num_heads, void* workspace, void* cuda_stream);
+
+/*
+ * Block tables and slots of a step, made on the GPU from the lengths of its requests.  Request r has context_lens[r] tokens in the cache and
+ * gets new_lens[r] more (negative: none).  Entry i of row r of block_table is the cache block of its tokens i * cache_block_size on.
+ *   The entries that the new tokens need beyond those of the context are taken, in order of requests and entries, from the top of
+ *   a stack: free_blocks[0 .. *num_free - 1], block free_blocks[*num_free - 1] first.  Where the stack is empty the entry is -1.  Entries behind
+ *   max_blocks_per_seq have no place and are not taken.  All others stay as they are.
+ *   query_start_loc[0 .. num_reqs], seq_lens: sums of the new lengths, and the lengths with them (at most 2^31 - 1)
+ *   position_ids, slot_mapping (int64), token_to_req_indices: of the new tokens, request by request, the num_tokens first; the slot is -1 where the token
+ *     has no block.  Rows behind the last request's have position 0, slot -1 and request 0.
+ *   num_free_out, num_missing: what is left on the stack, and how many entries of -1 were made
+ * seq_lens may be context_lens itself and num_free_out num_free itself; otherwise no result may share memory with another argument
+ * (DSV4_ERR_OVERLAP).  int32 where not said otherwise, on boundaries of their type; num_reqs <= 8192 (DSV4_ERR_TOO_LARGE).  No counterpart in the reference.
+ */
+int dsv4_extend_block_tables(const int32_t* context_lens, const int32_t* new_lens, int64_t num_reqs, int32_t* block_table,
+                             int64_t block_table_stride, int64_t max_blocks_per_seq, const int32_t* free_blocks, int64_t free_capacity,
+                             const int32_t* num_free, int64_t cache_block_size, int64_t num_tokens, int32_t* query_start_loc, int32_t* seq_lens,
+                             int64_t* position_ids, int64_t* slot_mapping, int32_t* token_to_req_indices, int32_t* num_free_out,
+                             int32_t* num_missing, void* cuda_stream);
+
+/*
+ * The way back: the blocks of the requests with finished[r] != 0, as many as seq_lens[r] tokens take, go onto the stack in the order that undoes
+ * the taking (the last one first).  Negative entries are left out.  block_table stays as it is: the row's next request starts with a context of 0.  Blocks beyond
+ * free_capacity, of which a stack with a place for every block has none, are dropped.
+ */
+int dsv4_release_block_tables(const int32_t* seq_lens, const uint8_t* finished, int64_t num_reqs, const int32_t* block_table,
+                              int64_t block_table_stride, int64_t max_blocks_per_seq, int32_t* free_blocks, int64_t free_capacity,
+                              const int32_t* num_free, int64_t cache_block_size, int32_t* num_free_out, void* cuda_stream);
 
 /*
  * Reads into *value_host, and clears, the error word the kernels of the current device keep:
