@@ -58,6 +58,7 @@ static_assert(kSoftmaxWarps * kSoftmaxRegisters + kReaderWarps * kReaderRegister
 static_assert(kSoftmaxWarps % 4 == 0 && kReaderWarps % 4 == 0, "whole warpgroups");
 constexpr uint64_t kAllKeys = (1ull << kBlockKeys) - 1;
 constexpr float kMostGrowth = 8.0f;  // log2 of the factor that a row's maximum may have grown by before O is corrected (with 0: 61 requests 209 us, not 155)
+constexpr int kLookChunk = 6;  // of S's eight chunks, the one in front of which P is looked for (4, 6, 7: 3172, 3167, 3174 us)
 constexpr int kMaxCtas = 148;        // a B200's SMs: one CTA on each (its shared memory allows no second)
 // Splitting.  A piece costs 128 KiB of fp32 sums out and in, and the kernel that joins them 6 to 10 us, so no tile shorter than kLeastSplit blocks is cut
 // (with 8: 61 tokens x 128 heads of up to 512 listed keys 38 us, with 16: 24; a chunk with a window of 512: 515 | 462; one request of 700 keys: 24.7 | 26.6);
@@ -112,6 +113,15 @@ __device__ __forceinline__ bool barrier_try(uint64_t* bar, uint32_t parity) {
                  : "r"(shared_address(bar)), "r"(parity), "r"(kTryNs)
                  : "memory");
     return done != 0;
+}
+// Whether the phase has completed, at once.
+__device__ __forceinline__ uint32_t barrier_test(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done)
+                 : "r"(shared_address(bar)), "r"(parity)
+                 : "memory");
+    return done;
 }
 // What bounds a wait: a number of tries behind the first (launch parameter), each of which the hardware suspends for up to two microseconds, and the
 // word by which a role that has given up tells the CTA's others to leave.
@@ -853,14 +863,19 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
         if (elected()) {
             bool ok = true;
             int it = 0, tiles = 0, stage = 0, stage_before = 0;
-            uint32_t phase = 0;
-            const auto product_o = [&](int i, bool first, int tile) {  // O += P V of block i, the one before the last
+            uint32_t phase = 0, phase_next = 0;
+            int stage_next = 0;
+            // Barriers are looked at while products are issued: a look takes some 200 cycles in which nothing else is, and the queue of products is short.  (Without it a
+            // block of the chunk takes 2190 cycles, with it 2110; most of that goes into a lower clock, 3.15 -> 3.12 ms.)
+            uint32_t keys_there = 0;
+            const auto product_o = [&](int i, bool first, int tile, uint32_t there) {  // O += P V of block i, the one before the last; `there`: P has been seen
                 const int buffer = i & 1;
-                if (!barrier_wait(&rest.p_full[buffer], (i >> 1) & 1, limit)) return false;
+                if (there == 0 && !barrier_wait(&rest.p_full[buffer], (i >> 1) & 1, limit)) return false;
                 if (first && tile > 0 && !barrier_wait(&rest.o_empty, (tile - 1) & 1, limit)) return false;
                 fence_tmem_after();
                 const uint64_t a = operand(base + kOffsetP + buffer * kQueryChunk, 16);
                 const uint64_t b = operand(base + kOffsetKeys + stage_before * kKeyBytes, kKeyChunk);
+                keys_there = barrier_test(&rest.kv_full[stage_next], phase_next);
 #pragma unroll
                 for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -876,32 +891,38 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
             for (; ok && w.settle(p); w.step(p)) {
                 if (w.begin == w.end) continue;
                 // (q of this tile is on its way while the last product of the one before runs)
-                if (pending && !product_o(it - 1, pending_first, pending_tile)) break;
+                stage_next = stage, phase_next = phase;
+                if (pending && !product_o(it - 1, pending_first, pending_tile, 0)) break;
                 pending = false;
                 if (!barrier_wait(&rest.q_full, tiles & 1, limit)) break;
                 for (int block = w.begin; block < w.end; ++block, ++it) {
                     const int buffer = it & 1;
-                    ok = barrier_wait(&rest.kv_full[stage], phase, limit);
+                    ok = keys_there != 0 || barrier_wait(&rest.kv_full[stage], phase, limit);
                     if (!ok) break;
+                    keys_there = 0;
                     fence_tmem_after();
                     const uint64_t a = operand(base, 16), b = operand(base + kOffsetKeys + stage * kKeyBytes, 16);
+                    uint32_t p_there = 0;
 #pragma unroll
-                    for (int chunk = 0; chunk < 8; ++chunk)
+                    for (int chunk = 0; chunk < 8; ++chunk) {
+                        if (chunk == kLookChunk) p_there = pending ? barrier_test(&rest.p_full[buffer ^ 1], ((it - 1) >> 1) & 1) : 0u;
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             multiply(tmem_scores + 64 * buffer, a + (chunk * kQueryChunk + 32 * k) / 16, b + (chunk * kKeyChunk + 32 * k) / 16, kKindS,
                                      chunk + k > 0);
+                    }
                     commit_to(&rest.s_full[buffer]);
                     if (block + 1 == w.end) commit_to(&rest.q_empty);
-                    if (pending) ok = product_o(it - 1, pending_first, pending_tile);
+                    stage_next = stage + 1 == kStages ? 0 : stage + 1, phase_next = stage + 1 == kStages ? phase ^ 1 : phase;
+                    if (pending) ok = product_o(it - 1, pending_first, pending_tile, p_there);
                     if (!ok) break;
                     pending = true, pending_first = block == w.begin, pending_tile = tiles;
                     stage_before = stage;
-                    if (++stage == kStages) stage = 0, phase ^= 1;
+                    stage = stage_next, phase = phase_next;
                 }
                 ++tiles;
             }
-            if (ok && pending) product_o(it - 1, pending_first, pending_tile);
+            if (ok && pending) product_o(it - 1, pending_first, pending_tile, 0);
             // nothing of this CTA may be in flight when its memory is given back, whatever the limit of the other waits
             commit_to(&rest.drained);
             for (uint32_t i = 0; i < kMostWaitRetries && !barrier_try(&rest.drained, 0); ++i) {}
@@ -942,6 +963,14 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                     at[i].x = reinterpret_cast<uint64_t>(there ? block_at + static_cast<int64_t>(in_block) * kDataBytes : p.a.q);
                     at[i].y = reinterpret_cast<uint64_t>(there ? block_at + codes_from + static_cast<int64_t>(in_block) * kCodeBytes : p.a.q);
                     exist |= static_cast<uint64_t>(__ballot_sync(0xffffffffu, there)) << (32 * i);
+                    // A key's record goes to L2 two blocks before a reader asks for it (61 requests of up to 16384 keys: 116.0 -> 110.6 us).  The keys of
+                    // a page lie one behind the other, so three lines of each are all of its 22.5 KB; listed keys gain nothing (509 tokens: 369 -> 379 us).
+                    if (MX && there && !p.a.indices) {
+                        const uint8_t* record = reinterpret_cast<const uint8_t*>(at[i].x);
+#pragma unroll
+                        for (int line = 0; line < 3; ++line) prefetch_line_l2(record + 128 * line);
+                        if ((lane & 7) == 0) prefetch_line_l2(reinterpret_cast<const uint8_t*>(at[i].y));
+                    }
                 }
                 ok = warp_wait(&rest.look_empty[entry], ((it >> 1) - 1) & 1, limit);
                 if (!ok) break;
