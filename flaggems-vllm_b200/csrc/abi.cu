@@ -650,6 +650,7 @@ int paged_batch_common(PagedBatch& p, int64_t num_reqs, const int32_t* block_tab
     const int64_t lim = 1LL << 31;
     if (num_reqs < 0 || max_blocks_per_seq < 0 || free_capacity < 0 || cache_block_size <= 0) return DSV4_ERR_BAD_SIZE;
     if (num_reqs > kMostRequests || max_blocks_per_seq >= lim || free_capacity >= lim || cache_block_size >= lim) return DSV4_ERR_TOO_LARGE;
+    if (num_reqs > 0 && max_blocks_per_seq > (lim - 1) / num_reqs) return DSV4_ERR_TOO_LARGE;  // (sums of blocks are held in 32 bits)
     if (num_reqs > 1 && block_table_stride < max_blocks_per_seq) return DSV4_ERR_BAD_SIZE;
     if (!num_free || !num_free_out || (!free_blocks && free_capacity > 0) || (!block_table && num_reqs > 0 && max_blocks_per_seq > 0))
         return DSV4_ERR_NULL_POINTER;

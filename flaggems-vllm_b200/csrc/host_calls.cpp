@@ -738,7 +738,6 @@ PyObject* sparse_latent_attention_mxfp4(Arguments& a) { return sparse_attention_
 bool is_list(const Tensor& t, ScalarType type, int64_t size, const Tensor& first) {
     return t.dim() == 1 && is(t, type) && t.size(0) == size && t.is_contiguous() && on(t, first);
 }
-bool shares(const Tensor& a, const Tensor& b) { return a.numel() > 0 && b.numel() > 0 && !apart(a, b); }
 int32_t* ints(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
 int64_t* longs(const Tensor& t) { return static_cast<int64_t*>(t.data_ptr()); }
 
@@ -750,6 +749,8 @@ void require_pool(Arguments& a, const Tensor& lens, const Tensor& table, const T
     REQUIRE(table.dim() == 2 && is(table, at::kInt) && table.size(0) == lens.size(0) && table.stride(1) == 1 && on(table, lens));
     REQUIRE(table.size(0) <= 1 || table.stride(0) >= table.size(1));
     REQUIRE(free.dim() == 1 && is(free, at::kInt) && free.is_contiguous() && on(free, lens));
+    if (!a.ok) return;
+    REQUIRE(table.numel() <= 0x7fffffff && free.size(0) <= 0x7fffffff);
     REQUIRE(is_list(count, at::kInt, 1, lens));
 }
 
@@ -779,15 +780,7 @@ PyObject* extend_block_tables(Arguments& a) {
             if (!a.ok) Py_RETURN_NONE;
             to[i] = *t;
         }
-        for (int i = 0; i < kResults; ++i) {
-            for (int k = 0; k < i; ++k) REQUIRE(!shares(to[i], to[k]));
-            REQUIRE(!shares(to[i], *table) && !shares(to[i], *free) && !shares(to[i], *fresh));
-            REQUIRE((i == 1 && to[i].data_ptr() == context->data_ptr()) || !shares(to[i], *context));
-            REQUIRE((i == 5 && to[i].data_ptr() == count->data_ptr()) || !shares(to[i], *count));
-        }
     }
-    REQUIRE(!shares(*table, *context) && !shares(*table, *fresh) && !shares(*table, *free) && !shares(*table, *count));
-    if (!a.ok) Py_RETURN_NONE;
     const OnDevice here = on_device_of(*context);
     if (!given)
         for (int i = 0; i < kResults; ++i) to[i] = make_empty({sizes[i]}, types[i], here);
@@ -816,9 +809,6 @@ PyObject* release_block_tables(Arguments& a) {
     require_pool(a, *lens, *table, *free, *count, block);
     if (!a.ok) Py_RETURN_NONE;
     REQUIRE(is_list(*finished, at::kBool, lens->size(0), *lens) && (!out || is_list(*out, at::kInt, 1, *lens)));
-    if (!a.ok) Py_RETURN_NONE;
-    REQUIRE(!shares(*free, *lens) && !shares(*free, *finished) && !shares(*free, *table) && !shares(*free, *count));
-    REQUIRE(!out || (!shares(*out, *lens) && !shares(*out, *finished) && !shares(*out, *table) && !shares(*out, *free)));
     if (!a.ok) Py_RETURN_NONE;
     const OnDevice here = on_device_of(*lens);
     Tensor made = out ? *out : make_empty({1}, at::kInt, here);

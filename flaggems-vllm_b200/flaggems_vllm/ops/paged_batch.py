@@ -8,7 +8,8 @@ numbers count as none).  Entry i of its row of `block_table` is the cache block 
 * `release_block_tables` puts the blocks of finished requests back onto the stack.
 
 Both only read numbers that are on the GPU, so a step can be captured in a graph with its lengths and its pool as state: `out.seq_lens` may be
-`context_lens` itself, and the `num_free` of a result `num_free` itself.
+`context_lens` itself, and the `num_free` of a result `num_free` itself.  No other result may share memory with another argument: the library
+refuses that (`Dsv4Error`).
 """
 from __future__ import annotations
 
@@ -17,7 +18,6 @@ from typing import NamedTuple, Optional, Sequence
 import torch
 
 from .. import _native
-from ..utils.memory import apart
 
 MOST_REQUESTS = 8192
 
@@ -84,18 +84,11 @@ def extend_block_tables(
     requests, num_tokens = context_lens.shape[0], int(num_tokens)
     _check_list("new_lens", new_lens, torch.int32, requests, context_lens)
     assert 0 <= num_tokens < 1 << 31
-    inputs = [context_lens, new_lens, block_table, free_blocks, num_free]
     if out:
         assert len(out) == len(PagedBatch._fields), "out: the seven tensors of a PagedBatch"
         sizes = (requests + 1, requests, num_tokens, num_tokens, num_tokens, 1, 1)
         for i, (name, t, size) in enumerate(zip(PagedBatch._fields, out, sizes)):
             _check_list(name, t, torch.int64 if i in (2, 3) else torch.int32, size, context_lens)
-        for i, t in enumerate(out):
-            for other in list(out[:i]) + inputs:
-                continues = other is {1: context_lens, 5: num_free}.get(i) and t.data_ptr() == other.data_ptr()
-                assert continues or not _shares(t, other), f"{PagedBatch._fields[i]} must not overlap another argument"
-    for other in inputs:
-        assert other is block_table or not _shares(block_table, other), "block_table must not overlap another argument"
     _native.refuse()
 
 
@@ -130,17 +123,9 @@ def release_block_tables(
         return result
     _check_pool(seq_lens, block_table, free_blocks, num_free, cache_block_size)
     _check_list("finished", finished, torch.bool, seq_lens.shape[0], seq_lens)
-    for other in (seq_lens, finished, block_table, num_free):
-        assert not _shares(free_blocks, other), "free_blocks must not overlap another argument"
     if num_free_out is not None:
         _check_list("num_free_out", num_free_out, torch.int32, 1, seq_lens)
-        for other in (seq_lens, finished, block_table, free_blocks):
-            assert not _shares(num_free_out, other), "num_free_out must not overlap another argument but num_free"
     _native.refuse()
-
-
-def _shares(a, b):
-    return a.numel() > 0 and b.numel() > 0 and not apart(a, b)
 
 
 def _check_list(name, t, dtype, size, first):
@@ -157,6 +142,7 @@ def _check_pool(lens, block_table, free_blocks, num_free, cache_block_size):
     assert block_table.shape[0] == lens.shape[0], "a row of block_table per request"
     assert block_table.shape[0] <= 1 or block_table.stride(0) >= block_table.shape[1], "rows of block_table must not overlap"
     assert free_blocks.dim() == 1 and free_blocks.dtype == torch.int32 and free_blocks.is_contiguous(), "free_blocks: int32 [capacity], contiguous"
+    assert block_table.numel() < 1 << 31 and free_blocks.numel() < 1 << 31
     for t in (block_table, free_blocks):
         assert t.device == lens.device, "all tensors must be on the same device"
     _check_list("num_free", num_free, torch.int32, 1, lens)

@@ -418,7 +418,8 @@ int dsv4_sparse_latent_attention_mxfp4(const void* q, int64_t q_stride_token, in
  *     has no block.  Rows behind the last request's have position 0, slot -1 and request 0.
  *   num_free_out, num_missing: what is left on the stack, and how many entries of -1 were made
  * seq_lens may be context_lens itself and num_free_out num_free itself; otherwise no result may share memory with another argument
- * (DSV4_ERR_OVERLAP).  int32 where not said otherwise, on boundaries of their type; num_reqs <= 8192 (DSV4_ERR_TOO_LARGE).  No counterpart in the reference.
+ * (DSV4_ERR_OVERLAP).  int32 where not said otherwise, on boundaries of their type; num_reqs <= 8192 and num_reqs *
+ * max_blocks_per_seq < 2^31 (DSV4_ERR_TOO_LARGE).  No counterpart in the reference.
  */
 int dsv4_extend_block_tables(const int32_t* context_lens, const int32_t* new_lens, int64_t num_reqs, int32_t* block_table,
                              int64_t block_table_stride, int64_t max_blocks_per_seq, const int32_t* free_blocks, int64_t free_capacity,

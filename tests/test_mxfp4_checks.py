@@ -113,7 +113,7 @@ def test_library_refuses_sizes_and_pointers_of_block_tables():
     big = 1 << 31
     for call, names in ((c_extend, EXTEND), (c_release, RELEASE)):
         assert call() > 0  # CUDA's own error: there is no device
-        for bad, code in (({"reqs": -1}, -2), ({"width": -1}, -2), ({"capacity": -1}, -2), ({"bs": 0}, -2), ({"stride": 8}, -2), ({"reqs": 8193, "stride": 9}, -5), ({"width": big, "stride": big}, -5),
+        for bad, code in (({"reqs": -1}, -2), ({"width": -1}, -2), ({"capacity": -1}, -2), ({"bs": 0}, -2), ({"stride": 8}, -2), ({"reqs": 8193, "stride": 9}, -5), ({"width": big // 6 + 1, "stride": big}, -5), ({"width": big, "stride": big}, -5),
                           ({"capacity": big}, -5), ({"bs": big}, -5)):
             assert call(**bad) == code, bad
         assert call(stride=9) > 0

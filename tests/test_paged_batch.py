@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import flaggems_vllm as fg
+from flaggems_vllm import _native
 
 gpu = pytest.mark.gpu
 DEV = "cuda:0"
@@ -215,7 +216,22 @@ def test_extend_captured_with_its_state_in_place():
 
 
 @gpu
-@pytest.mark.parametrize("requests,context,bs,share", [(1, 100, 16, 1.0), (1, 100, 16, 0.0), (61, 16384, 64, 0.1), (61, 3000, 1, 0.5), (1021, 4000, 16, 0.5), (8192, 60, 16, 1.0), (33, 0, 16, 1.0)])
+@pytest.mark.parametrize("tokens", [900, 1025, 5000, 30000])
+def test_extend_in_place_with_many_tokens(tokens):
+    r = random.Random(tokens)
+    new = [r.randint(0, 2 * tokens // 40) for _ in range(40)]
+    p = Pool([r.randrange(300) for _ in range(40)], new, 16, seed=tokens, spare=9)
+    (lens, new_lens, table, free, num_free), _ = p.tensors()
+    n = sum(new)
+    out = [torch.zeros(41, dtype=torch.int32, device=DEV), lens, *(torch.zeros(n, dtype=torch.int64, device=DEV) for _ in range(2)), torch.zeros(n, dtype=torch.int32, device=DEV), num_free,
+           torch.zeros(1, dtype=torch.int32, device=DEV)]
+    fg.extend_block_tables(lens, new_lens, table, free, num_free, 16, n, out)
+    want, wanted_table = extended(p.context, p.new, p.table, p.free, p.num_free, 16, n)
+    assert [t.tolist() for t in out] == list(want) and table.tolist() == wanted_table
+
+
+@gpu
+@pytest.mark.parametrize("requests,context,bs,share", [(1, 100, 16, 1.0), (1, 100, 16, 0.0), (61, 16384, 64, 0.1), (61, 3000, 1, 0.5), (1021, 4000, 16, 0.5), (8192, 60, 16, 1.0), (33, 0, 16, 1.0), (3, 90000, 7, 1.0), (17, 20000, 1, 0.9)])
 @pytest.mark.parametrize("holes", [False, True])
 def test_release(requests, context, bs, share, holes):
     r = random.Random(requests)
@@ -285,23 +301,36 @@ def test_refusals_on_the_gpu():
     (context, new, table, free, num_free), _ = Pool([5, 17], [20, 1], 16).tensors()
     call = lambda *a, **k: fg.extend_block_tables(*a, **k)  # noqa: E731
     good = call(context, new, table, free, num_free, 16, 21)
-    for bad in ({0: context.long()}, {1: new[:1]}, {2: table.t()}, {3: free.view(1, -1)}, {4: num_free.long()}, {5: 0}, {6: -1}, {2: table[:1]}, {3: table[0]}, {0: context.cpu()}):
+    for bad in ({0: context.long()}, {1: new[:1]}, {2: table.t()}, {3: free.view(1, -1)}, {4: num_free.long()}, {5: 0}, {6: -1}, {2: table[:1]}, {0: context.cpu()}):
         args = [context, new, table, free, num_free, 16, 21]
         for i, v in bad.items():
             args[i] = v
         with pytest.raises(AssertionError):
             call(*args)
-    for i, v in ((0, good.query_start_loc[:2]), (2, good.position_ids.int()), (1, new), (5, good.num_missing), (4, free[:21] if len(free) >= 21 else good.seq_lens), (6, num_free)):
+    with pytest.raises(_native.Dsv4Error, match="overlap"):
+        call(context, new, table, table[0], num_free, 16, 21)
+    for i, v in ((0, good.query_start_loc[:2]), (2, good.position_ids.int()), (4, good.seq_lens)):
         out = list(good)
         out[i] = v
         with pytest.raises(AssertionError):
             call(context, new, table, free, num_free, 16, 21, out)
+    for i, v in ((1, new), (5, good.num_missing), (6, num_free)):
+        out = list(good)
+        out[i] = v
+        with pytest.raises(_native.Dsv4Error, match="overlap"):
+            call(context, new, table, free, num_free, 16, 21, out)
     with pytest.raises(AssertionError):
         call(context, new, table, free, num_free, 16, 21, list(good)[:6])
     done = torch.tensor([True, False], device=DEV)
-    for bad in ({1: done.int()}, {1: done[:1]}, {3: table[0]}, {6: free[:1]}, {6: num_free.long()}):
+    for bad in ({1: done.int()}, {1: done[:1]}, {6: num_free.long()}):
         args = [context, done, table, free, num_free, 16, None]
         for i, v in bad.items():
             args[i] = v
         with pytest.raises(AssertionError):
+            fg.release_block_tables(*args)
+    for bad in ({3: table[0]}, {6: free[:1]}):
+        args = [context, done, table, free, num_free, 16, None]
+        for i, v in bad.items():
+            args[i] = v
+        with pytest.raises(_native.Dsv4Error, match="overlap"):
             fg.release_block_tables(*args)
