@@ -1,5 +1,5 @@
 // Attention over the paged latent cache: queries [tokens, heads, 512] against cached rows of 448 e4m3 values with power-of-two scales and 64
-// bf16 values, which are keys and values at once.
+// bf16 values, or of 448 e2m1 values with such scales (the cache in 4 bits) and those 64, which are keys and values at once.
 //
 //   s_j = scale * q . k_j over the keys a token sees, o = sum_j e^(s_j - m) k_j / (sum_j e^(s_j - m) + e^(sink - m)), lse = m + ln sum_j e^(s_j - m)
 //
@@ -24,17 +24,24 @@
 // over the tiles' numbers of blocks and takes its share, which may begin and end inside a tile.  Pieces of a tile go to a workspace as
 // unnormalised sums and are joined, in a fixed order, by a second small kernel.  Where lists are short, tiles are not cut (see kLeastSplit).
 //
-// What bounds it.  In the largest chunk a block takes 2000 to 2100 cycles at the 1.56 GHz that power leaves: the products 1700 of them (a product of 64 rows
-// takes as long as one of 128: 128.8 cycles for 256 columns and a depth of 16), the rest the way from S to P and back that the order S, O leaves open.  In one CTA 128 rows
-// would need 128 KiB for q and 512 columns for O, and leave nothing for S.  A pair of CTAs with 64 rows of q each needs neither, in products that both
-// take part in (cta_group::2: 64.9 cycles for the same 256 columns of 128 rows, 25.7 for 64); that form is timed as a bare product only, not built.
-// Softmax and readers take 1650 and 2100 cycles beside the products, half of the issue slots.  Readers that ask for the next block's values before
-// they convert this one's (and hand over by hardware barriers, which do not wait for loads) change nothing: 3.25 ms both.
-// 1024 tokens x 128 heads over 8192 keys: 3.3 ms (700 TFLOP/s); 61 requests of up to 16384 keys, 64 heads: 154 us; one of 65536 keys, 128 heads: 46 us;
-// a window of 128 tokens, one request: 10.9 us, of which two thirds are the way in (plan, look-up, keys, q: each waits for memory that the one before names) and out.
-// Other forms that were built: blocks of 64 keys in two stages, 6.9 ms; two groups of readers in turn, 4.5; eight softmax warps, 4.1 (this form then 3.9);
-// two CTAs that share out keys and exchange S and P, 128 rows a product: 5.0, since each exchange takes 400 cycles one way.
+// What bounds it.  Products of 64 rows run at half the rate: 28 cycles of a depth of 16 for the 48 columns of S (its operands come out of shared memory at
+// 128 bytes a cycle), 128 for 256 columns of O, 1664 cycles a block as bare products, which a block of the largest chunk takes 2110 to 2190 of at 1.7 to 1.84 GHz: steps
+// that save cycles there cost clock, at 1000 W.  A look at a barrier takes 150 to 250 cycles beside them, so softmax (1150 cycles from S to P) and readers (1700 to
+// 2000 a block: look-up 170, asking 300, the stage 170, conversion 700 to 1000, handing over 150, and what the loads take) are not far behind.
+// At a tile's end O goes out in 6000 to 7000 cycles of the four softmax warps, in which no product runs; the next tile's keys and first S are there before that.
+// In one CTA 128 rows would need 128 KiB for q and 512 columns for O, and leave nothing for S.  A pair of CTAs with 64 rows of q each needs neither, in products
+// that both take part in (cta_group::2: 64.9 cycles for the same 256 columns of 128 rows, 25.7 for 64); that form is timed as a bare product only, not built.
+// e4m3: 1024 tokens x 128 heads over 8192 keys 3.3 ms (700 TFLOP/s); 61 requests of up to 16384 keys, 64 heads, 154 us; one of 65536 keys, 128 heads, 46 us; a window
+// of 128 tokens, one request, 10.9 us, of which two thirds are the way in (plan, look-up, keys, q: each waits for memory that the one before names) and out.
+// 4 bits: 3.08 to 3.15 ms (740 TFLOP/s), 111 to 114 us, 44.7 us; 61 tokens x 128 heads of up to 512 listed keys 23.5 us, 509 of up to 2048 374 us.
+// Other forms that were built: blocks of 64 keys in two stages, 6.9 ms; two groups of readers in turn, 4.5 (4 bits: 3.11 | 3.06, 122 us | 116); eight softmax warps, 4.1
+// (this form then 3.9); two CTAs that share out keys and exchange S and P, 128 rows a product: 5.0, since each exchange takes 400 cycles one way; for the cache
+// in 4 bits readers that ask for the next block before they convert this one (124 us | 116), a lane for a whole group of 32 values (3.08 | 3.12 ms, 113 us | 116, 376 | 370), S in
+// two accumulators (the same), S and O from two issuing warps (3.3 | 3.1 ms), e2m1 by byte permutations instead of conversions (3.28 | 3.08), the issuer's products in a loop
+// (3.8 | 3.1), O written out by the readers at the reuse of a tile's last stage (3.7 | 3.1: what it adds to their loop costs more than the 3 us a tile that it saves), a tile
+// counted as three to five blocks when they are dealt out (the same).
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "dsv4_common.cuh"
@@ -1160,6 +1167,18 @@ cudaError_t launch_latent_attention(const LatentAttention& a, bool mxfp4, void* 
     const bool may_split = !p.one_each && most_blocks >= kLeastSplit;
     auto* at = static_cast<uint8_t*>(workspace);
     p.sums = reinterpret_cast<float*>(at), p.rows = reinterpret_cast<float2*>(at + kSumBytes), p.pieces = reinterpret_cast<int4*>(at + kSumBytes + kRowBytes2);
+    // A setmaxnreg that asks for more than the block was launched with waits forever, and how many that is the compiler chooses: looked at once for each kernel.
+    const auto as_expected = [](auto* of) {
+        cudaFuncAttributes a;
+        const cudaError_t error = cudaFuncGetAttributes(&a, of);
+        return error != cudaSuccess ? error : a.numRegs == kLaunchRegisters ? cudaSuccess : cudaErrorLaunchOutOfResources;
+    };
+    static std::atomic<bool> looked[2] = {};
+    if (!looked[mxfp4].load(std::memory_order_relaxed)) {
+        const cudaError_t rc = as_expected(kernel);
+        if (rc != cudaSuccess) return rc;
+        looked[mxfp4].store(true, std::memory_order_relaxed);
+    }
     // Set for the current device each time: cheaper than to remember for which ones it was.
     cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedBytes);
     if (rc != cudaSuccess) return rc;

@@ -77,9 +77,9 @@ def extend_block_tables(
         _bind()
     result = _extend(context_lens, new_lens, block_table, free_blocks, num_free, cache_block_size, num_tokens, *(out or ()))
     if result is True:
-        return out if isinstance(out, PagedBatch) else PagedBatch(*out)
+        return out if isinstance(out, PagedBatch) else PagedBatch._make(out)
     if result is not None:
-        return PagedBatch(*result)
+        return PagedBatch._make(result)
     _check_pool(context_lens, block_table, free_blocks, num_free, cache_block_size)
     requests, num_tokens = context_lens.shape[0], int(num_tokens)
     _check_list("new_lens", new_lens, torch.int32, requests, context_lens)

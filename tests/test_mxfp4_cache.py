@@ -272,6 +272,21 @@ def test_groups_that_are_nan(heads):
 
 
 @gpu
+@pytest.mark.parametrize("code", [253, 254])
+def test_values_that_bfloat16_cannot_hold(code):
+    """6 * 2^126 and 6 * 2^127: infinite.  Rows that see the key are NaN, all of them or in that dimension; the others are as if it were not there."""
+    b = MxBatch([100], [60], 8, 64, seed=6)
+    slot = b.slot(0, 70)
+    raw, at = b.cache[slot // 64], slot % 64
+    raw[at * 352 : at * 352 + 16] = 0
+    raw[at * 352 + 5] = 0x07
+    raw[64 * 352 + at * 16] = code
+    out, lse = b.run()
+    assert out[30:, :, 10].isnan().all()
+    check(out[:30], lse[:30], b.want()[:30])
+
+
+@gpu
 def test_bytes_that_nobody_sees_do_not_matter():
     """Pages behind the end, later tokens and free slots full of NaN codes and values."""
     b = MxBatch([75, 20], [5, 20], 16, 64, seed=7)
