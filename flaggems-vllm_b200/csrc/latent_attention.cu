@@ -872,8 +872,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
             int it = 0, tiles = 0, stage = 0, stage_before = 0;
             uint32_t phase = 0, phase_next = 0;
             int stage_next = 0;
-            // Barriers are looked at while products are issued: a look takes some 200 cycles in which nothing else is, and the queue of products is short.  (Without it a
-            // block of the chunk takes 2190 cycles, with it 2110; most of that goes into a lower clock, 3.15 -> 3.12 ms.)
+            // Barriers are looked at while products are issued: a look takes some 200 cycles in which nothing else is, and the queue of products is short.  (Ahead | not:
+            // a block of the chunk 2110 | 2190 cycles; 4 bits, 3.12 | 3.15 ms, 509 listed tokens 370 | 374 us; e4m3, 3.22 | 3.28 ms, window of 512 436 | 443 us, but 61 and 509 listed
+            // tokens 25.3 | 24.7 and 381 | 376 us: there the keys are mostly late, and the look is one more.)
+            const bool look_ahead = MX || !p.a.indices;
             uint32_t keys_there = 0;
             const auto product_o = [&](int i, bool first, int tile, uint32_t there) {  // O += P V of block i, the one before the last; `there`: P has been seen
                 const int buffer = i & 1;
@@ -882,7 +884,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                 fence_tmem_after();
                 const uint64_t a = operand(base + kOffsetP + buffer * kQueryChunk, 16);
                 const uint64_t b = operand(base + kOffsetKeys + stage_before * kKeyBytes, kKeyChunk);
-                keys_there = barrier_test(&rest.kv_full[stage_next], phase_next);
+                keys_there = look_ahead ? barrier_test(&rest.kv_full[stage_next], phase_next) : 0u;
 #pragma unroll
                 for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -912,7 +914,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
                     uint32_t p_there = 0;
 #pragma unroll
                     for (int chunk = 0; chunk < 8; ++chunk) {
-                        if (chunk == kLookChunk) p_there = pending ? barrier_test(&rest.p_full[buffer ^ 1], ((it - 1) >> 1) & 1) : 0u;
+                        if (chunk == kLookChunk) p_there = look_ahead && pending ? barrier_test(&rest.p_full[buffer ^ 1], ((it - 1) >> 1) & 1) : 0u;
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             multiply(tmem_scores + 64 * buffer, a + (chunk * kQueryChunk + 32 * k) / 16, b + (chunk * kKeyChunk + 32 * k) / 16, kKindS,
