@@ -33,11 +33,12 @@
 // that both take part in (cta_group::2: 64.9 cycles for the same 256 columns of 128 rows, 25.7 for 64); that form is timed as a bare product only, not built.
 // e4m3: 1024 tokens x 128 heads over 8192 keys 3.3 ms (700 TFLOP/s); 61 requests of up to 16384 keys, 64 heads, 154 us; one of 65536 keys, 128 heads, 46 us; a window
 // of 128 tokens, one request, 10.9 us, of which two thirds are the way in (plan, look-up, keys, q: each waits for memory that the one before names) and out.
-// 4 bits: 3.08 to 3.15 ms (740 TFLOP/s), 111 to 114 us, 44.7 us; 61 tokens x 128 heads of up to 512 listed keys 23.5 us, 509 of up to 2048 374 us.
+// 4 bits: 3.05 to 3.13 ms (755 TFLOP/s), 110 us, 44.3 us; 61 tokens x 128 heads of up to 512 listed keys 23.3 us, 509 of up to 2048 368 us.
 // Other forms that were built: blocks of 64 keys in two stages, 6.9 ms; two groups of readers in turn, 4.5 (4 bits: 3.11 | 3.06, 122 us | 116); eight softmax warps, 4.1
 // (this form then 3.9); two CTAs that share out keys and exchange S and P, 128 rows a product: 5.0, since each exchange takes 400 cycles one way; for the cache
 // in 4 bits readers that ask for the next block before they convert this one (124 us | 116), a lane for a whole group of 32 values (3.08 | 3.12 ms, 113 us | 116, 376 | 370), S in
-// two accumulators (the same), S and O from two issuing warps (3.3 | 3.1 ms), e2m1 by byte permutations instead of conversions (3.28 | 3.08), the issuer's products in a loop
+// two accumulators (the same), S and O from two issuing warps (3.3 | 3.1 ms), e2m1 by byte permutations alone (3.28 | 3.08), by products with f16 powers behind a look at
+// the codes' range (111.6 us | 111.3, 3.15 ms | 3.17; without the look, which the format does not allow, 108.8 and 3.04), the issuer's products in a loop
 // (3.8 | 3.1), O written out by the readers at the reuse of a tile's last stage (3.7 | 3.1: what it adds to their loop costs more than the 3 us a tile that it saves), a tile
 // counted as three to five blocks when they are dealt out (the same).
 #include <algorithm>
@@ -455,8 +456,16 @@ __device__ __forceinline__ uint32_t two_values(uint32_t word, uint32_t scale) {
 // `codes` has the code twice, one in each half.
 __device__ __forceinline__ uint32_t power_of_codes(uint32_t codes) { return __vmaxu2(codes << 7, 0x400040u); }
 
-// The same, but 255 is NaN.
-__device__ __forceinline__ uint32_t power_of_mx_codes(uint32_t codes) { return power_of_codes(codes) | (((codes + 0x00010001u) >> 2) & 0x00400040u); }
+// The same, but 255 is NaN; the code twice in the low half.
+__device__ __forceinline__ uint32_t power_of_mx_codes(uint32_t codes) {
+    uint32_t v;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.bf16x2.ue8m0x2 %0, l;\n\t}" : "=r"(v) : "r"(codes));
+    return v;
+}
+
+// Two fp32 values that bf16 holds, as a pair: a permutation of bytes, where the conversion shares a unit with the one to f16 in front of it (509 listed tokens 368 | 374 us,
+// 61 23.1 | 23.5, the others 0.3 to 0.7 % less; beside the conversions of e4m3 it costs 0 to 2 %).
+__device__ __forceinline__ uint32_t upper_halves(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }
 
 // Eight e2m1 values (the first in the low bits) times a power of two.
 __device__ __forceinline__ uint4 eight_values(uint32_t word, uint32_t scale) {
@@ -469,7 +478,7 @@ __device__ __forceinline__ uint4 eight_values(uint32_t word, uint32_t scale) {
     for (int i = 0; i < 4; ++i) {
         float lo, hi;
         asm("{.reg .f16 l, h; mov.b32 {l, h}, %2; cvt.f32.f16 %0, l; cvt.f32.f16 %1, h;}" : "=f"(lo), "=f"(hi) : "r"(h[i]));
-        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(v[i]) : "r"(pack_bf16x2(lo, hi)), "r"(scale));
+        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(v[i]) : "r"(upper_halves(lo, hi)), "r"(scale));
     }
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
@@ -764,8 +773,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attention_kernel(const Lau
         const uint32_t store_row = base + kOffsetKeys + key_a * 128, unit = 2 * (sub & 3);
         const bool coded = sub < 12;
         const int rotary_sub = sub ^ (8 * odd);  // (the two keys' halves, so that their stores use different banks)
-        // of a byte of a code word and of zeros: the byte in both halves
-        const uint32_t code_select = 0x4040u + 0x0101u * (MX ? (sub >> 1) & 3 : sub >> 2);
+        // of a byte of a code word and of zeros: the byte in both halves (4 bits: in both bytes of the low half)
+        const uint32_t code_select = MX ? 0x4400u + 0x11u * ((sub >> 1) & 3) : 0x4040u + 0x0101u * (sub >> 2);
         // 16 cached values to two 16-byte columns
         using Values = std::conditional_t<MX, uint2, uint4>;
         const auto convert = [&](const Values& v, uint32_t code_word, uint4& a, uint4& b) {
