@@ -747,6 +747,7 @@ void require_pool(Arguments& a, const Tensor& lens, const Tensor& table, const T
     if (!a.ok) return;
     REQUIRE(lens.size(0) <= 8192 && block > 0 && block <= 0x7fffffff);
     REQUIRE(table.dim() == 2 && is(table, at::kInt) && table.size(0) == lens.size(0) && table.stride(1) == 1 && on(table, lens));
+    if (!a.ok) return;
     REQUIRE(table.size(0) <= 1 || table.stride(0) >= table.size(1));
     REQUIRE(free.dim() == 1 && is(free, at::kInt) && free.is_contiguous() && on(free, lens));
     if (!a.ok) return;
