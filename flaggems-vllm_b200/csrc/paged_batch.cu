@@ -219,10 +219,11 @@ __global__ void __launch_bounds__(kMostThreads) release_block_tables_kernel(cons
     blocks = __reduce_add_sync(0xffffffffu, blocks), in_front = __reduce_add_sync(0xffffffffu, in_front);
     int64_t at = static_cast<int64_t>(top) + blocks - 1 - in_front;
     const bool plain = count == to - from && at < p.free_capacity;  // no entry is left out, and none has no place
-    for (int32_t i = from; i < to; i += 32 * kAtOnce) {
-        if (i != from) load(i, e);
+    for (int32_t done = 0; done < to - from; done += 32 * kAtOnce) {  // (from + done may pass 2^31 - 1 behind the last round, `done` cannot)
+        const int32_t i = from + done;
+        if (done > 0) load(i, e);
         if (plain) {
-            int32_t* place = p.free_to + (at - (i - from) - lane);
+            int32_t* place = p.free_to + (at - done - lane);
 #pragma unroll
             for (int k = 0; k < kAtOnce; ++k)
                 if (32 * k + lane < to - i) place[-32 * k] = e[k];

@@ -96,7 +96,7 @@ def test_extend_small(context, new, bs):
 
 @gpu
 @pytest.mark.parametrize("requests,chunk,context,bs", [(61, 1, 16384, 64), (128, 1, 500, 16), (129, 3, 500, 16), (513, 2, 90, 16), (1024, 1, 200, 32), (1025, 9, 77, 16), (300, 170, 999, 64),
-                                                       (4096, 7, 100, 16), (8192, 2, 40, 16), (1, 20000, 3, 64), (2, 40000, 100, 16)])
+                                                       (4096, 7, 100, 16), (8192, 2, 40, 16), (1, 20000, 3, 64), (2, 40000, 100, 16), (3, 400000, 70, 64)])
 def test_extend_large(requests, chunk, context, bs):
     r = random.Random(requests)
     Pool([r.randrange(context) for _ in range(requests)], [r.randint(0, chunk) for _ in range(requests)], bs, seed=requests, row=5).check()
@@ -244,6 +244,23 @@ def test_release(requests, context, bs, share, holes):
     got = fg.release_block_tables(lens, torch.tensor(finished, device=DEV), table, free, num_free, bs)
     want, count = released(p.context, finished, p.table, p.free, 13, bs)
     assert free.tolist() == want and got.tolist() == [count] and num_free.tolist() == [13] and torch.equal(table, before)
+
+
+@gpu
+def test_release_as_many_entries_as_a_table_can_have():
+    """2^31 - 1 entries of one row: the last warp's part ends where a 32-bit position does."""
+    n = INT_MAX
+    if torch.cuda.mem_get_info()[0] < 40 * 2**30:
+        pytest.skip("needs 40 GiB")
+    table, free = torch.arange(n, dtype=torch.int32, device=DEV)[None], torch.full((n,), -7, dtype=torch.int32, device=DEV)
+    got = fg.release_block_tables(i32([n]).to(DEV), torch.tensor([True], device=DEV), table, free, i32([0]).to(DEV), 1)
+    assert got.tolist() == [n]
+    for a in range(0, n, 1 << 28):
+        b = min(a + (1 << 28), n)
+        assert torch.equal(free[a:b], torch.arange(n - 1 - a, n - 1 - b, -1, dtype=torch.int32, device=DEV))
+    table[0, -1] = -1  # a part with a hole: entry by entry
+    got = fg.release_block_tables(i32([n]).to(DEV), torch.tensor([True], device=DEV), table, free, i32([0]).to(DEV), 1)
+    assert got.tolist() == [n - 1] and free[:2].tolist() == [n - 2, n - 3] and free[n - 3 :].tolist() == [1, 0, 0]
 
 
 @gpu
