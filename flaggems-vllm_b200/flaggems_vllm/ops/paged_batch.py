@@ -9,7 +9,8 @@ numbers count as none).  Entry i of its row of `block_table` is the cache block 
 
 Both only read numbers that are on the GPU, so a step can be captured in a graph with its lengths and its pool as state: `out.seq_lens` may be
 `context_lens` itself, and the `num_free` of a result `num_free` itself.  No other result may share memory with another argument: the library
-refuses that (`Dsv4Error`).
+refuses that (`Dsv4Error`).  Calls on one pool have to follow one another.  A count of free blocks below zero counts as none, one above the
+stack's capacity as all of it.
 """
 from __future__ import annotations
 

@@ -418,6 +418,7 @@ int dsv4_sparse_latent_attention_mxfp4(const void* q, int64_t q_stride_token, in
  *   position_ids, slot_mapping (int64), token_to_req_indices: of the new tokens, request by request, the num_tokens first; the slot is -1 where the token
  *     has no block.  Rows behind the last request's have position 0, slot -1 and request 0.
  *   num_free_out, num_missing: what is left on the stack, and how many entries of -1 were made
+ * (*num_free below 0 counts as 0, above free_capacity as that.  Calls on one stack have to follow one another.)
  * seq_lens may be context_lens itself and num_free_out num_free itself; otherwise no result may share memory with another argument
  * (DSV4_ERR_OVERLAP).  int32 where not said otherwise, on boundaries of their type; num_reqs <= 8192 and num_reqs *
  * max_blocks_per_seq < 2^31 (DSV4_ERR_TOO_LARGE).  No counterpart in the reference.
