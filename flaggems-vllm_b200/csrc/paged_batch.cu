@@ -23,6 +23,7 @@ namespace dsv4 {
 namespace {
 
 constexpr int kMostThreads = 1024, kMostCluster = 8, kMostCtas = 148;
+constexpr int kBytesPerRequest = 12;  // of the shared memory of extend_block_tables_kernel; the other kernel has 4
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
@@ -244,7 +245,8 @@ cudaError_t launch(void (*kernel)(const Launched<PagedBatch>), const PagedBatch&
                    cudaStream_t stream) {
     const unsigned threads = items <= 128 ? 128 : items <= 512 ? 512 : kMostThreads;
     if (shared_bytes > 40 * 1024) {
-        const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared_bytes));
+        // The same number each time, the most that any call takes, so that a call on another thread with fewer requests does not take it back.
+        const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytesPerRequest * kMostRequests);
         if (rc != cudaSuccess) return rc;
     }
     const cudaError_t rc = launch_dependent_cluster(kernel, dim3(ctas), dim3(threads), cluster ? ctas : 1, shared_bytes, stream, p);
@@ -261,7 +263,7 @@ cudaError_t launch_extend_block_tables(const PagedBatch& p, cudaStream_t stream)
     unsigned ctas = 1;
     while (ctas < most && p.num_tokens > ctas * static_cast<int64_t>(kMostThreads)) ctas *= 2;
     if (ctas > most) ctas = static_cast<unsigned>(most);
-    return launch(extend_block_tables_kernel, p, p.num_tokens > p.num_reqs ? p.num_tokens : p.num_reqs, ctas, in_place, 12 * static_cast<size_t>(p.num_reqs), stream);
+    return launch(extend_block_tables_kernel, p, p.num_tokens > p.num_reqs ? p.num_tokens : p.num_reqs, ctas, in_place, kBytesPerRequest * static_cast<size_t>(p.num_reqs), stream);
 }
 
 cudaError_t launch_release_block_tables(const PagedBatch& p, cudaStream_t stream) {
