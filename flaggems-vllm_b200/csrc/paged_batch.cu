@@ -128,9 +128,10 @@ __global__ void __launch_bounds__(kMostThreads) extend_block_tables_kernel(const
             position = c + (t - start_of(token_ends, r));
             if (position <= 0x7fffffffLL) {
                 const uint32_t page = fast_div(static_cast<uint32_t>(position), p.block_mul, p.block_shift);
-                const int32_t held = blocks_of(p, c);
-                if (page < static_cast<uint32_t>(p.max_blocks)) {
-                    const int64_t block = static_cast<int32_t>(page) < held ? p.block_table[r * p.table_stride + page] : taken(start_of(block_ends, r) + static_cast<int32_t>(page) - held);
+                const int32_t held = blocks_of(p, c), before = start_of(block_ends, r);
+                // Not behind those that the request has now: lengths end at 2^31 - 1, and with a block of as many tokens position 2^31 - 1 is on a page that is not counted.
+                if (page < static_cast<uint32_t>(held + block_ends[r] - before)) {
+                    const int64_t block = static_cast<int32_t>(page) < held ? p.block_table[r * p.table_stride + page] : taken(before + static_cast<int32_t>(page) - held);
                     if (block >= 0) slot = block * p.block_size + (static_cast<uint32_t>(position) - page * p.block_size);
                 }
             }
