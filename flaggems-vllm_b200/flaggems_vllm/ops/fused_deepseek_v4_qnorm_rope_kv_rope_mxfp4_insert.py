@@ -64,8 +64,9 @@ def fused_deepseek_v4_qnorm_rope_kv_rope_mxfp4_insert(
 
         code = ceil(log2(max(amax, 6 * 2^-126) / 6)) + 127,   value = e2m1(x / 2^(code - 127)), to nearest, ties to even
 
-    so a value is off by at most a fifth of its group's maximum.  e2m1 has neither infinities nor NaN: a group with one gets the code 255,
-    which stands for NaN, and the readers make all 32 values NaN.
+    so a value is off by at most a fifth of its group's maximum, and by at most 2^-128 in a group whose maximum is below 1.25 * 2^-126, for which the
+    scale has no smaller step.  Values from 3.5 * 2^126 on, finite ones, are stored as 2^128, which the readers, whose keys are bfloat16, take for infinite.
+    e2m1 has neither infinities nor NaN: a group with one gets the code 255, which stands for NaN, and the readers make all 32 values NaN.
 
     Args:
         q: [num_tokens, num_heads, 512] bfloat16, contiguous, modified in place

@@ -19,7 +19,7 @@ second product takes them (2^-8 of each; their sum is that of the unrounded ones
 
 `paged_latent_attention_mxfp4` and `sparse_latent_attention_mxfp4` are the same over the cache in 4 bits that
 `fused_deepseek_v4_qnorm_rope_kv_rope_mxfp4_insert` writes (368 bytes a token instead of 584).  A scale code of 255 makes its 32 values NaN; values of 2^128 and
-more, which bfloat16 cannot hold (scale codes of 253 and 254; written only for magnitudes above 3.5 * 2^126), are infinite.
+more, which bfloat16 cannot hold (scale codes of 253 and 254; written only for magnitudes from 3.5 * 2^126 on), are infinite.
 
 q is bfloat16 [tokens, heads, 512] with unit inner stride, any number of heads; rows, cache and cache blocks on 16-byte boundaries.  `out`
 (like q) and `lse` (float32 [tokens, heads]) are written where given; `out` is allocated otherwise, and returned.  Neither may share memory with the

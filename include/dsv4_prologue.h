@@ -394,7 +394,7 @@ int dsv4_sparse_latent_attention(const void* q, int64_t q_stride_token, int64_t 
                                  int64_t lse_stride_head, int64_t num_tokens, int64_t num_heads, void* workspace, void* cuda_stream);
 
 /* The same over the cache in 4 bits that dsv4_qnorm_rope_kv_insert_mxfp4 writes.  A scale code of 255 makes its 32 values NaN.  Values of 2^128 and more, which
- * bf16 cannot hold (scale codes of 253 and 254; written only for magnitudes above 3.5 * 2^126), are infinite. */
+ * bf16 cannot hold (scale codes of 253 and 254; written only for magnitudes from 3.5 * 2^126 on), are infinite. */
 int dsv4_paged_latent_attention_mxfp4(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_cache, int64_t num_blocks,
                                       int64_t kv_block_stride_bytes, int64_t cache_block_size, const int32_t* block_table,
                                       int64_t block_table_stride, int64_t max_blocks_per_seq, const int32_t* seq_lens,
