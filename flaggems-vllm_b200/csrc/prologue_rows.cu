@@ -287,8 +287,8 @@ __global__ void __launch_bounds__(WARPS * 32) prologue_rows_any_alignment_kernel
     for (int b = 0; b < 4; ++b) data[kNopeDim + 4 * lane + b] = static_cast<uint8_t>((rot >> (8 * b)) & 0xffu);
 }
 
-template <int RPW, int WARPS, int MIN_CTAS, bool MXFP4 = false>
-cudaError_t launch(const PrologueParams& p, bool checked, cudaStream_t stream) {
+template <int RPW, int WARPS, int MIN_CTAS, bool CHECKED, bool MXFP4 = false>
+cudaError_t launch(const PrologueParams& p, cudaStream_t stream) {
     constexpr int TILE = RPW * WARPS;
     const int64_t kv_ctas = (p.num_tokens_insert + WARPS - 1) / WARPS;
     const int64_t total_rows = p.num_tokens * p.num_heads;
@@ -296,9 +296,9 @@ cudaError_t launch(const PrologueParams& p, bool checked, cudaStream_t stream) {
     const int64_t grid = kv_ctas + q_ctas;
     if (grid == 0) return cudaSuccess;
     if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-    if (checked) {
-        if constexpr (MXFP4) return cudaErrorNotSupported;
-        else prologue_rows_kernel<RPW, WARPS, MIN_CTAS, true, false><<<static_cast<unsigned>(grid), WARPS * 32, 0, stream>>>(p, kv_ctas);
+    if constexpr (CHECKED) {
+        static_assert(!MXFP4, "no range-checked form over the cache in 4 bits");
+        prologue_rows_kernel<RPW, WARPS, MIN_CTAS, true, false><<<static_cast<unsigned>(grid), WARPS * 32, 0, stream>>>(p, kv_ctas);
     } else if (p.pdl) {
         const auto kernel = p.pdl == 2 ? (p.table_staging ? prologue_rows_kernel<RPW, WARPS, MIN_CTAS, false, false, 2, true, MXFP4>
                                                           : prologue_rows_kernel<RPW, WARPS, MIN_CTAS, false, false, 2, false, MXFP4>)
@@ -355,15 +355,16 @@ cudaError_t launch_prologue_rows_any_alignment(const PrologueParams& p, bool mxf
 
 cudaError_t launch_prologue_rows(const PrologueParams& p, bool checked, cudaStream_t stream) {
 #ifdef DSV4_ROWS_RPW
-    return launch<DSV4_ROWS_RPW, DSV4_ROWS_WARPS, DSV4_ROWS_MIN_CTAS>(p, checked, stream);
+    return checked ? launch<DSV4_ROWS_RPW, DSV4_ROWS_WARPS, DSV4_ROWS_MIN_CTAS, true>(p, stream)
+                   : launch<DSV4_ROWS_RPW, DSV4_ROWS_WARPS, DSV4_ROWS_MIN_CTAS, false>(p, stream);
 #else
     // 2 rows per warp, 4 warps, 10 CTAs per SM (48 registers): the fastest of the swept shapes on B200
-    return launch<2, 4, 10>(p, checked, stream);
+    return checked ? launch<2, 4, 10, true>(p, stream) : launch<2, 4, 10, false>(p, stream);
 #endif
 }
 
-// The same shape: at the sizes where its speed matters, all but the first 1 in 8 to 128 of its CTAs are those of q.
-cudaError_t launch_prologue_rows_mxfp4(const PrologueParams& p, cudaStream_t stream) { return launch<2, 4, 10, true>(p, false, stream); }
+// The same shape: where every token is inserted, 1 in 1 + heads / 2 of its CTAs are those of latent rows (1 in 65 of 128 heads, 1 in 5 of 8), the others those of q.
+cudaError_t launch_prologue_rows_mxfp4(const PrologueParams& p, cudaStream_t stream) { return launch<2, 4, 10, false, true>(p, stream); }
 
 cudaError_t launch_prologue_rows_padded(const PrologueParams& p, cudaStream_t stream) { return launch_padded<2, 4, 10>(p, stream); }
 
