@@ -31,9 +31,10 @@
 // At a tile's end O goes out in 6000 to 7000 cycles of the four softmax warps, in which no product runs; the next tile's keys and first S are there before that.
 // In one CTA 128 rows would need 128 KiB for q and 512 columns for O, and leave nothing for S.  A pair of CTAs with 64 rows of q each needs neither, in products
 // that both take part in (cta_group::2: 64.9 cycles for the same 256 columns of 128 rows, 25.7 for 64); that form is timed as a bare product only, not built.
-// e4m3: 1024 tokens x 128 heads over 8192 keys 3.3 ms (700 TFLOP/s); 61 requests of up to 16384 keys, 64 heads, 154 us; one of 65536 keys, 128 heads, 46 us; a window
-// of 128 tokens, one request, 10.9 us, of which two thirds are the way in (plan, look-up, keys, q: each waits for memory that the one before names) and out.
-// 4 bits: 3.05 to 3.13 ms (755 TFLOP/s), 110 us, 44.3 us; 61 tokens x 128 heads of up to 512 listed keys 23.3 us, 509 of up to 2048 368 us.
+// e4m3 | 4 bits, one behind the other on the same GPU: 1024 tokens x 128 heads over 8192 keys 3.05 to 3.28 | 2.93 to 3.12 ms (720 | 760 TFLOP/s; 1.84 | 1.87 GHz at the power limit); 61 requests of up to
+// 16384 keys, 64 heads, 120 | 110 us with 444 thousand keys in all, 146 | 134 us with 578 thousand, with 8 heads 138 | 128 us, with a window of 128 tokens and 4 first ones 13.2 | 12.8 us; one
+// request of 65536 keys, 128 heads, 46.2 | 44.4 us; 61 tokens x 128 heads of up to 512 listed keys 24.2 | 23.6 us, 509 of up to 2048 377 | 370 us; a window of 128 tokens, one request, 11.1 us
+// both, of which two thirds are the way in (plan, look-up, keys, q: each waits for memory that the one before names) and out.
 // Other forms that were built: blocks of 64 keys in two stages, 6.9 ms; two groups of readers in turn, 4.5 (4 bits: 3.11 | 3.06, 122 us | 116); eight softmax warps, 4.1
 // (this form then 3.9); two CTAs that share out keys and exchange S and P, 128 rows a product: 5.0, since each exchange takes 400 cycles one way; for the cache
 // in 4 bits readers that ask for the next block before they convert this one (124 us | 116), a lane for a whole group of 32 values (3.08 | 3.12 ms, 113 us | 116, 376 | 370), S in

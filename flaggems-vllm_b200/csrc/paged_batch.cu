@@ -7,15 +7,15 @@
 // Every CTA makes the sums of all requests for itself (eight bytes a request to read), holds them in shared memory and finds a token's (an entry's) request
 // by bisection, so that none waits for another.  What is read and written is a few bytes a token: the time is that of the dependent loads (lengths, then
 // entries) and of the launch.  Where a result stands in the place of an argument (num_free, seq_lens), the CTAs are one cluster, whose barrier keeps those two
-// back until every CTA has read them; otherwise there is a CTA for every 1024 tokens.
+// back until every CTA has read them, and a cluster has eight at most; otherwise there is a CTA for every 1024 tokens, rounded up to a power of two, up to the number of SMs.
 //
 // release_block_tables: the entries e_0, e_1, ... of the finished requests' rows, in order, go to free[top + count - 1 - i]: what undoes the taking.  Entries
 // that are negative (blocks that were missing) are left out.  The rows' entries are one list, which the warps of a cluster share out evenly: each counts
 // its part, the counts go to all CTAs, and each writes behind those in front of it.
 //
-// GPU time of a call, one behind another in a graph: extend, 1 request 2.4 us, 61 3.3 us, 1021 with 65 thousand new tokens 5.3 us (one cluster for every
-// size: 15.2 us).  Release, 61 requests 5.1 us, half of 1021 with 262 thousand entries 17.3 us, bound by the instructions of eight SMs (a search for every entry,
-// and a vote for every 32 where none is missing: 25 us; a warp a request 24.8 us, and more where one is long).  A cluster costs about 2 us more than a CTA.
+// GPU time of a call, one behind another in a graph: extend, 1 request 2.4 to 2.6 us, 61 3.3 to 3.5 us, 1021 with 65 thousand new tokens 5.3 to 5.5 us; with its state in place 2.5 to 2.9,
+// 3.2 to 3.8 and 14 us (eight CTAs instead of 64).  Release, 61 requests 5.2 to 5.5 us, half of 1021 with 259 thousand entries 17.2 us, bound by the instructions of eight SMs (a search
+// for every entry, and a vote for every 32 where none is missing: 25 us; a warp a request 24.8 us, and more where one is long).
 #include "dsv4_common.cuh"
 #include "paged_batch.cuh"
 
@@ -268,7 +268,9 @@ cudaError_t launch_extend_block_tables(const PagedBatch& p, cudaStream_t stream)
 }
 
 cudaError_t launch_release_block_tables(const PagedBatch& p, cudaStream_t stream) {
-    // How many entries there are is known on the GPU alone: a CTA for 16 requests.
+    // How many entries there are is known on the GPU alone: a CTA for 16 requests.  With 1 | 2 | 4 | 8 CTAs: 1 request, 16 entries 3.7 | 4.0 | 4.3 | 4.2 us, 16 requests, 176 entries
+    // 4.5 | 4.9 | 4.8 | 4.8, 61 requests, 1019 entries 4.9 | 5.3 | 5.5 | 5.1, and 7393 entries 6.5 | 6.0 | 5.7 | 5.3, 256 requests, 2952 entries 5.8 in all four, 1021 requests, 259 thousand
+    // entries 102 | 54 | 30 | 17.  Few requests with long rows pay for the rule: 16 with 65536 entries 17.5 | 11.1 | 7.4 | 5.4.
     unsigned ctas = 1;
     while (ctas < kMostCluster && p.num_reqs > ctas * 16) ctas *= 2;
     return launch(release_block_tables_kernel, p, kMostThreads, ctas, true, 4 * static_cast<size_t>(p.num_reqs), stream);
